@@ -27,6 +27,7 @@ from .layers import (ColumnParallelLinear, Embedding, Linear, MergedColumnParall
                      RMSNorm, RowParallelLinear)
 
 PAGE_SIZE = 128
+KV_DTYPES = ("auto", "fp8")   # KV cache: the model's own type, or e4m3 codes with one scale per token and head
 
 
 @dataclass
@@ -131,6 +132,10 @@ class Attention(nn.Module):
         """The same from an already projected ``q | k | v`` (``[T, (heads_local + 2 kv_heads_local) * d]``, changed in place)."""
         d = self.cfg.head_dim
         T = qkv.shape[0]
+        if cache.dtype == torch.uint8:   # 8-bit cache: the append normalises, rotates and quantises in one launch
+            qn, kn = (self.q_norm.weight, self.k_norm.weight) if self.cfg.qk_norm else (None, None)
+            q = ops.rope_kv_write_fp8_(qkv, self.hq, self.hkv, d, cs, cache, m.slot_mapping, qn, kn, self.cfg.rms_norm_eps)
+            return ops.attention_paged_fp8(q, cache, m.block_table, m.kv_len, m.cu_q, m.max_q_len).view(T, self.hq * d)
         if self.cfg.qk_norm:
             qk = qkv[:, : (self.hq + self.hkv) * d]
             normed_q = self.q_norm(qkv[:, : self.hq * d].reshape(-1, d)).view(T, self.hq * d)
@@ -288,16 +293,28 @@ class QwenLLM(nn.Module):
     def kv_heads_local(self) -> int:
         return self.layers[0].self_attn.hkv
 
-    def alloc_kv_cache(self, num_pages: int) -> list[torch.Tensor]:
+    def alloc_kv_cache(self, num_pages: int, kv_dtype: str = "auto") -> list[torch.Tensor]:
         """One zero-initialised cache ``[pages, 2, Hkv_local, 128, d]`` per layer, all views of one allocation
         ``[layers, pages, 2, Hkv_local, 128, d]`` (kept as ``self.kv_backing``) so that another executor can map the
-        whole cache with one handle and copy pages of every layer in one launch."""
+        whole cache with one handle and copy pages of every layer in one launch.  ``kv_dtype="fp8"``: the 8-bit cache of
+        :func:`ops.kv_cache_fp8`, ``[layers, pages, 2, Hkv_local, 128 * (d + 4)]`` bytes, which the layers recognise by
+        its type."""
+        if kv_dtype not in KV_DTYPES:
+            raise ValueError(f"kv_dtype must be one of {KV_DTYPES}, got {kv_dtype!r}")
+        if kv_dtype == "fp8":
+            d, n = self.cfg.head_dim, self.cfg.num_hidden_layers
+            if self.device.type == "cuda" and d not in ops.KV_FP8_HEAD_DIMS:
+                raise ValueError(f"the 8-bit KV cache takes head widths {ops.KV_FP8_HEAD_DIMS}, this model has {d}")
+            flat = ops.kv_cache_fp8(n * num_pages, self.kv_heads_local, d, self.device)
+            self.kv_backing = flat.view(n, num_pages, *flat.shape[1:])
+            return list(self.kv_backing.unbind(0))
         shape = (self.cfg.num_hidden_layers, num_pages, 2, self.kv_heads_local, PAGE_SIZE, self.cfg.head_dim)
         self.kv_backing = torch.zeros(shape, device=self.device, dtype=self.embed_tokens.weight.dtype)
         return list(self.kv_backing.unbind(0))
 
-    def kv_bytes_per_page(self) -> int:
-        return 2 * self.kv_heads_local * PAGE_SIZE * self.cfg.head_dim * 2 * self.cfg.num_hidden_layers
+    def kv_bytes_per_page(self, kv_dtype: str = "auto") -> int:
+        row = self.cfg.head_dim + 4 if kv_dtype == "fp8" else 2 * self.cfg.head_dim
+        return 2 * self.kv_heads_local * PAGE_SIZE * row * self.cfg.num_hidden_layers
 
     def embed(self, m: BatchMeta) -> torch.Tensor:
         x = self.embed_tokens(m.input_ids)

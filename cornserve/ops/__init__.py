@@ -17,7 +17,7 @@ from .reference import ACTS
 
 __all__ = [
     "linear", "swiglu_linear", "rms_norm", "layer_norm", "rope_", "mrope_table", "rope_kv_write_",
-    "attention_varlen", "attention_paged", "act_mul", "gather_rows", "scatter_rows_", "argmax",
+    "attention_varlen", "attention_paged", "kv_cache_fp8", "kv_cache_fp8_views", "rope_kv_write_fp8_", "attention_paged_fp8", "act_mul", "gather_rows", "scatter_rows_", "argmax",
     "flow_step_", "pcm16", "decode_advance_", "l2_flush", "check_error", "kernel_launches", "reset_launch_count",
     "count_path", "path_counts", "push_bytes_", "apply_penalties_", "count_tokens_",
     "head_norm_rope_", "softmax_rows", "im2col3x3", "im2col1d", "dwconv1d", "to_rgb8", "conv3x3", "conv1d_causal",
@@ -438,6 +438,143 @@ def attention_paged(q, cache, block_table, kv_len, cu_q, max_q_len: int, scale: 
     )
     _chk(rc, "cs_attention(paged)")
     _count(2 if kv_splits > 1 else 1)
+    return out
+
+
+# --------------------------------------------------------------------------------------------
+# 8-bit paged KV cache: e4m3 codes with one fp32 scale per token and head
+# --------------------------------------------------------------------------------------------
+KV_FP8_PAGE = reference.KV_FP8_PAGE
+KV_FP8_HEAD_DIMS = (64, 128)     # head widths the CUDA kernels are built for
+
+
+def kv_cache_fp8(num_pages: int, kv_heads: int, d: int, device: torch.device | str | None = None) -> torch.Tensor:
+    """A zeroed 8-bit cache of ``num_pages`` pages of 128 tokens: bytes ``[pages, 2, kv_heads, 128 * (d + 4)]``.
+
+    The block of one page, of keys (0) or values (1) and of one head holds 128 rows of ``d`` e4m3 codes and then their
+    128 fp32 scales; :func:`kv_cache_fp8_views` gives both as tensors.  A token costs ``d + 4`` bytes per head instead of
+    the ``2 d`` of a bf16 cache."""
+    return torch.zeros((num_pages, 2, kv_heads, KV_FP8_PAGE * (d + 4)), device=device, dtype=torch.uint8)
+
+
+def kv_cache_fp8_views(cache: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(codes [pages, 2, kv_heads, 128, d] float8_e4m3fn, scales [pages, 2, kv_heads, 128] fp32)``, views of ``cache``:
+    row ``r`` of a page stands for ``codes[..., r, :] * scales[..., r]``."""
+    _kv_fp8_dim(cache)
+    return reference.kv_cache_fp8_views(cache)
+
+
+def _kv_fp8_dim(cache: torch.Tensor) -> int:
+    if cache.dtype != torch.uint8 or cache.dim() != 4 or cache.shape[1] != 2 or cache.shape[3] % KV_FP8_PAGE or \
+            cache.shape[3] <= 4 * KV_FP8_PAGE or not cache.is_contiguous():
+        raise ValueError("an 8-bit KV cache is a contiguous uint8 tensor [pages, 2, kv_heads, 128 * (d + 4)] "
+                         f"(see kv_cache_fp8); got {cache.dtype} {tuple(cache.shape)}")
+    return cache.shape[3] // KV_FP8_PAGE - 4
+
+
+def _need(cond: bool, what: str) -> None:
+    if not cond:
+        raise ValueError(what)
+
+
+def _need_i32(name: str, t: torch.Tensor, shape: tuple, device: torch.device) -> None:
+    _need(t.dtype == torch.int32 and tuple(t.shape) == shape and t.device == device and t.stride(-1) == 1,
+          f"{name} must be int32 {list(shape)} on {device} with contiguous rows; got {t.dtype} {list(t.shape)} on {t.device}")
+
+
+def _kv_fp8_on_device(cache: torch.Tensor, d: int) -> None:
+    _on_current_device(cache)
+    _need(d in KV_FP8_HEAD_DIMS, f"the 8-bit cache kernels take head widths {KV_FP8_HEAD_DIMS}, got {d}")
+    _need(cache.data_ptr() % 16 == 0, "the cache must start on a 16-byte boundary")
+
+
+def rope_kv_write_fp8_(qkv: torch.Tensor, Hq: int, Hkv: int, d: int, cs: torch.Tensor, cache: torch.Tensor, slot: torch.Tensor,
+                       q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, eps: float = 1e-6) -> torch.Tensor:
+    """Rotate the queries and keys of ``qkv`` ``[T, (Hq + 2 Hkv) * d]`` and append keys and values to the 8-bit ``cache``.
+
+    ``cs`` is the cos / sin table ``[T, 2, d/2]`` (fp32); ``slot [T]`` (int32) is ``page * 128 + row`` of every token,
+    negative for tokens that are not cached (where a slot occurs twice, its row ends up as a mix of the two).  With ``q_norm`` and ``k_norm``
+    (weights ``[d]``) every query / key head is RMS-normalised first.  A cached row is stored as ``x / s`` in e4m3 with
+    ``s = max(|x|) / 448`` in fp32 (rows with a largest magnitude below 2^-40 take that one's scale; a row with an infinity
+    or NaN takes the scale NaN).  Returns the queries ``[T, Hq, d]`` as a new tensor; ``qkv`` is only read.
+
+    A slot beyond the cache raises on the CPU; on a GPU its token is skipped and :func:`check_error` reports it."""
+    T = qkv.shape[0]
+    _need(_kv_fp8_dim(cache) == d and cache.shape[2] == Hkv, f"cache {list(cache.shape)} does not hold {Hkv} heads of width {d}")
+    _need(qkv.dim() == 2 and qkv.shape[1] == (Hq + 2 * Hkv) * d, f"qkv must be [T, {(Hq + 2 * Hkv) * d}], got {list(qkv.shape)}")
+    _need(cs.dtype == torch.float32 and tuple(cs.shape) == (T, 2, d // 2) and cs.is_contiguous() and cs.device == qkv.device,
+          f"cs must be a contiguous fp32 table [{T}, 2, {d // 2}] on {qkv.device}")
+    _need(cache.device == qkv.device, f"qkv on {qkv.device}, cache on {cache.device}")
+    _need_i32("slot", slot, (T,), qkv.device)
+    _need((q_norm is None) == (k_norm is None), "q_norm and k_norm go together")
+    if q_norm is not None:
+        for w in (q_norm, k_norm):
+            _need(tuple(w.shape) == (d,) and w.dtype == qkv.dtype and w.device == qkv.device and w.is_contiguous(),
+                  f"norm weights must be contiguous {qkv.dtype} [{d}] on {qkv.device}")
+    if not qkv.is_cuda:
+        return reference.rope_kv_write_fp8(qkv, Hq, Hkv, d, cs, cache, slot, q_norm, k_norm, eps)
+    _kv_fp8_on_device(cache, d)
+    _need(qkv.dtype == torch.bfloat16, "the CUDA kernel takes bf16 qkv")
+    if qkv.stride(1) != 1 or qkv.stride(0) % 8 or qkv.data_ptr() % 16:
+        qkv = qkv.clone(memory_format=torch.contiguous_format)
+    q = torch.empty((T, Hq, d), device=qkv.device, dtype=torch.bfloat16)
+    if T == 0:
+        return q
+    if q_norm is not None:
+        q_norm, k_norm = (w if w.data_ptr() % 16 == 0 else w.clone() for w in (q_norm, k_norm))
+    if cs.data_ptr() % 16:
+        cs = cs.clone()
+    lib = _lib.load()
+    _chk(lib.cs_rope_kv_write_fp8(qkv.data_ptr(), qkv.stride(0), T, Hq, Hkv, d, cs.data_ptr(), _ptr(q_norm), _ptr(k_norm), float(eps),
+                                  slot.data_ptr(), q.data_ptr(), cache.data_ptr(), cache.shape[0], _stream()), "cs_rope_kv_write_fp8")
+    _count()
+    return q
+
+
+def attention_paged_fp8(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, kv_len: torch.Tensor, cu_q: torch.Tensor,
+                        max_q_len: int, scale: float | None = None, causal: bool = True, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of packed queries ``[Tq, Hq, d]`` over the 8-bit paged ``cache`` (see :func:`kv_cache_fp8`).
+
+    ``block_table [B, blocks]``, ``kv_len [B]`` and ``cu_q [B + 1]`` (int32) are those of :func:`attention_paged`:
+    ``kv_len[s]`` counts the keys of sequence ``s`` including the ones just appended for its queries, which are rows
+    ``[cu_q[s], cu_q[s + 1])`` of ``q``, at most ``max_q_len`` of them.  A causal query sees the keys up to its own
+    position; one that sees none gives zeros.  Rows of ``out`` behind the last sequence are not written.
+
+    Keys beyond the table or pages outside the cache raise on the CPU; on a GPU they are not read (the result of that
+    sequence is then meaningless) and :func:`check_error` reports them."""
+    d = _kv_fp8_dim(cache)
+    _need(q.dim() == 3 and q.shape[2] == d, f"q must be [Tq, Hq, {d}], got {list(q.shape)}")
+    Tq, Hq, _ = q.shape
+    Hkv, B = cache.shape[2], kv_len.numel()
+    _need(Hq > 0 and Hkv > 0 and Hq % Hkv == 0, f"{Hq} query heads cannot share {Hkv} key heads")
+    _need(cache.device == q.device, f"q on {q.device}, cache on {cache.device}")
+    _need(block_table.dim() == 2, "block_table must be [B, blocks]")
+    _need_i32("kv_len", kv_len, (B,), q.device)
+    _need_i32("cu_q", cu_q, (B + 1,), q.device)
+    _need(block_table.dtype == torch.int32 and block_table.shape[0] == B and block_table.device == q.device and
+          (block_table.stride(1) == 1 or block_table.shape[1] <= 1),
+          f"block_table must be int32 [{B}, blocks] on {q.device} with contiguous rows")
+    _need(max_q_len >= 0, "max_q_len must not be negative")
+    _need(out is None or (out.shape == q.shape and out.dtype == q.dtype and out.device == q.device),
+          f"out must be {q.dtype} {list(q.shape)} on {q.device}")
+    scale = scale if scale is not None else 1.0 / math.sqrt(d)
+    if not q.is_cuda:
+        return reference.attention_paged_fp8(q, cache, block_table, kv_len, cu_q, scale, causal, out)
+    _kv_fp8_on_device(cache, d)
+    _need(q.dtype == torch.bfloat16, "the CUDA kernel takes bf16 queries")
+    if q.stride(2) != 1:
+        q = q.contiguous()
+    if out is None:
+        out = torch.empty((Tq, Hq, d), device=q.device, dtype=torch.bfloat16)
+    if Tq == 0 or B == 0 or max_q_len == 0:
+        return out
+    _need(out.stride(2) == 1, "out needs contiguous channels")
+    lib = _lib.load()
+    _chk(lib.cs_attention_paged_fp8(q.data_ptr(), q.stride(0), q.stride(1), cache.data_ptr(), cache.shape[0], out.data_ptr(), out.stride(0),
+                                    out.stride(1), cu_q.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(), block_table.stride(0),
+                                    block_table.shape[1], B, Tq, Hq, Hkv, d, float(scale), 1 if causal else 0, _stream()),
+         "cs_attention_paged_fp8")
+    _count()
     return out
 
 

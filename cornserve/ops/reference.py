@@ -181,6 +181,89 @@ def rope_kv_write(qkv, Hq, Hkv, d, cs, cache, slot, page):
     return q
 
 
+# -- 8-bit paged cache: blocks of 128 rows of e4m3 codes followed by their 128 fp32 scales ------------------------
+KV_FP8_PAGE = 128
+KV_FP8_MAX = 448.0
+KV_FP8_AMAX_FLOOR = 2.0 ** -40
+
+
+def kv_cache_fp8_views(cache):
+    d = cache.shape[-1] // KV_FP8_PAGE - 4
+    codes = cache[..., : KV_FP8_PAGE * d].view(torch.float8_e4m3fn).unflatten(-1, (KV_FP8_PAGE, d))
+    return codes, cache[..., KV_FP8_PAGE * d:].view(torch.float32)
+
+
+def quantize_kv_rows(x):
+    """Rows ``[..., d]`` as (codes e4m3, scales fp32 [...]): the largest magnitude of a row maps to 448; a row that holds
+    an infinity or NaN has the scale NaN and codes 0."""
+    x = x.float()
+    amax = x.abs().amax(dim=-1)
+    ok = torch.isfinite(amax)
+    scale = amax.clamp_min(KV_FP8_AMAX_FLOOR) * (1.0 / KV_FP8_MAX)
+    y = (x * (1.0 / scale)[..., None]).clamp(-KV_FP8_MAX, KV_FP8_MAX)
+    y = torch.where(ok[..., None], y, torch.zeros_like(y))
+    return y.to(torch.float8_e4m3fn), torch.where(ok, scale, torch.full_like(scale, float("nan")))
+
+
+def rope_kv_write_fp8(qkv, Hq, Hkv, d, cs, cache, slot, q_norm=None, k_norm=None, eps=1e-6):
+    x = qkv.float().view(qkv.shape[0], Hq + 2 * Hkv, d)
+    qk, v = x[:, : Hq + Hkv], x[:, Hq + Hkv:]
+    if q_norm is not None:
+        w = torch.cat([q_norm.float().expand(Hq, d), k_norm.float().expand(Hkv, d)])
+        qk = qk * torch.rsqrt(qk.pow(2).mean(-1, keepdim=True) + eps) * w
+    qk = rope(qk, cs)
+    codes, scales = kv_cache_fp8_views(cache)
+    raw = codes.view(torch.uint8)      # indexed stores move bytes
+    ok = slot >= 0
+    at = slot[ok].long()
+    if at.numel() and int(at.max()) >= cache.shape[0] * KV_FP8_PAGE:
+        raise ValueError(f"slot {int(at.max())} lies outside a cache of {cache.shape[0]} pages")
+    page, row = torch.div(at, KV_FP8_PAGE, rounding_mode="floor"), at % KV_FP8_PAGE
+    for i, rows in enumerate((qk[:, Hq:][ok], v[ok])):
+        c, s = quantize_kv_rows(rows)
+        raw[page, i, :, row] = c.view(torch.uint8)
+        scales[page, i, :, row] = s
+    return qk[:, :Hq].to(qkv.dtype)
+
+
+def gather_kv_fp8(cache, block_table, kv_len, seq):
+    """Keys and values ``[kv_len, Hkv, d]`` (fp32) of sequence ``seq``."""
+    codes, scales = kv_cache_fp8_views(cache)
+    n = int(kv_len[seq])
+    ids = block_table[seq, : -(-n // KV_FP8_PAGE)].long()
+    if n > block_table.shape[1] * KV_FP8_PAGE or bool(((ids < 0) | (ids >= cache.shape[0])).any()):
+        raise ValueError(f"sequence {seq}: {n} keys do not lie in pages of this cache")
+    raw = codes.view(torch.uint8)
+    out = []
+    for i in (0, 1):
+        c = raw[ids, i].view(torch.float8_e4m3fn).float() * scales[ids, i][..., None]   # [blocks, Hkv, page, d]
+        out.append(c.transpose(1, 2).flatten(0, 1)[:n])
+    return out
+
+
+def attention_paged_fp8(q, cache, block_table, kv_len, cu_q, scale, causal=True, out=None):
+    if out is None:
+        out = torch.zeros_like(q, memory_format=torch.contiguous_format)
+    cu = cu_q.tolist()
+    rep = q.shape[1] // cache.shape[2]
+    for s in range(len(cu) - 1):
+        n = cu[s + 1] - cu[s]
+        if n == 0:
+            continue
+        k, v = (t.repeat_interleave(rep, dim=1) for t in gather_kv_fp8(cache, block_table, kv_len, s))   # [keys, Hq, d]
+        sc = torch.einsum("qhd,khd->hqk", q[cu[s]: cu[s + 1]].float(), k) * scale
+        last = torch.arange(n)[:, None] + (k.shape[0] - n) if causal else torch.full((n, 1), k.shape[0])
+        hidden = torch.arange(k.shape[0])[None, :] > last
+        # a row that sees no key is zero
+        pr = torch.softmax(sc.masked_fill(hidden, float("-inf")), dim=-1).masked_fill(hidden.all(dim=1, keepdim=True), 0.0)
+        bad = torch.isnan(v)
+        o = torch.einsum("hqk,khd->qhd", pr, v.masked_fill(bad, 0.0))
+        if bool(bad.any()):   # 0 * NaN is not 0: only queries that see such a value become NaN
+            o = o.masked_fill(torch.einsum("qk,khd->qhd", (~hidden).float(), bad.float()) > 0, float("nan"))
+        out[cu[s]: cu[s + 1]] = o.to(out.dtype)
+    return out
+
+
 def act_mul(gu, act="silu"):
     n = gu.shape[-1] // 2
     return (act_fn(gu[..., :n].float(), act) * gu[..., n:].float()).to(gu.dtype)

@@ -151,6 +151,7 @@ class EngineConfig:
     use_cuda_graph: bool = True
     graph_batch_sizes: tuple[int, ...] = (1, 2, 4, 8, 16, 32, 64, 128, 256)
     max_model_len: int = 32768
+    kv_cache_dtype: str = "auto"   # "fp8": e4m3 cache, about half the bytes per token
 
 
 @dataclass
@@ -234,8 +235,9 @@ class LLMEngine:
         self.on_gpu = self.device.type == "cuda"
         model.prefill_rows_hint = max(getattr(model, "prefill_rows_hint", 0), self.cfg.max_batched_tokens)
         self.blocks = BlockManager(self.cfg.num_pages)
-        self.kv_caches = model.alloc_kv_cache(self.cfg.num_pages)
-        self.kv_backing: torch.Tensor = model.kv_backing  # [layers, pages, 2, heads, 128, d]; kv_caches are its views
+        self.kv_caches = model.alloc_kv_cache(self.cfg.num_pages, self.cfg.kv_cache_dtype)
+        # [layers, pages, 2, heads, 128, d] (8-bit cache: [layers, pages, 2, heads, 128 * (d + 4)]); kv_caches are its views
+        self.kv_backing: torch.Tensor = model.kv_backing
         self.max_blocks = -(-self.cfg.max_model_len // PAGE_SIZE)
         self.waiting: deque[Sequence] = deque()
         self.running: list[Sequence] = []

@@ -80,6 +80,8 @@ def parse_args(argv: list[str] | None = None) -> argparse.Namespace:
     ap.add_argument("--quantization", default=None, choices=[None, "fp8"],
                     help="fp8: attention and MLP projections as e4m3 with 128x128 block scales (also chosen when the "
                          "checkpoint's quantization_config says fp8)")
+    ap.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "fp8"],
+                    help="fp8: keys and values cached as e4m3 with one scale per token and head (about twice the tokens)")
     ap.add_argument("--gpu-memory-utilization", type=float, default=0.9)
     ap.add_argument("--num-kv-pages", type=int, default=0, help="0 = size the cache from free memory")
     ap.add_argument("--decode-burst", type=int, default=4)
@@ -250,7 +252,7 @@ def build_engine(args: argparse.Namespace, group: ParallelGroup | None = None) -
         if device.type == "cuda":
             free, _ = torch.cuda.mem_get_info(device)
             budget = int(free * args.gpu_memory_utilization) - (4 << 30)
-            pages = max(64, budget // model.kv_bytes_per_page())
+            pages = max(64, budget // model.kv_bytes_per_page(args.kv_cache_dtype))
         else:
             pages = 64
     if group is not None and group.size > 1:
@@ -259,7 +261,7 @@ def build_engine(args: argparse.Namespace, group: ParallelGroup | None = None) -
         pages = agree_on_min(int(pages), group)
     ecfg = EngineConfig(num_pages=int(pages), max_batched_tokens=args.max_num_batched_tokens, max_num_seqs=args.max_num_seqs,
                         decode_burst=args.decode_burst, max_model_len=args.max_model_len,
-                        use_cuda_graph=device.type == "cuda")
+                        use_cuda_graph=device.type == "cuda", kv_cache_dtype=args.kv_cache_dtype)
     engine = LLMEngine(model, ecfg)
     if os.environ.get("CORNSERVE_LLM_PRECAPTURE", "1") == "1":
         t0 = time.perf_counter()

@@ -1,0 +1,27 @@
+// Layout of the 8-bit paged key-value cache, shared by the kernels that fill it and the kernels that read it.
+//
+// A cache is [pages, 2, Hkv] blocks of 128 * (d + 4) bytes; block (page, kv, head) holds the 128 rows of one page of the
+// keys (kv = 0) or values (kv = 1) of one head:
+//
+//   byte 0        : 128 rows of d e4m3 codes
+//   byte 128 * d  : 128 fp32 scales; row r stands for  code[r][:] * scale[r]
+//
+// A row and its scale travel with the page (pages are what executors copy from one cache to another), a block is one run
+// of bytes, and both parts of it start on a 512-byte boundary relative to the cache.  The scale is per token and head:
+// it needs no calibration, and a token with large keys costs no other token any precision.
+#pragma once
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+constexpr int KV8_PAGE = 128;
+
+__host__ __device__ __forceinline__ constexpr long long kv8_block_bytes(int d) { return static_cast<long long>(KV8_PAGE) * (d + 4); }
+
+// Two e4m3 codes (low byte first) as two fp16 numbers: every finite code is exact in fp16.
+__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t two_codes) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo;\n\tcvt.u16.u32 lo, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(two_codes));
+  return r;
+}

@@ -1,0 +1,441 @@
+"""The 8-bit paged key-value cache on the GPU: the append and the attention against their definitions in 64 bits.
+
+Tolerances.  A stored code is off by at most half a step of e4m3: 2^-4 of the value, 2^-10 among the subnormal codes.  A
+bf16 output is off by 2^-8 of its value.  Inside the attention a key's weight (probability times value scale) may be rounded
+to fp16: off by 2^-11 of it, or by half a step of the subnormals, 2^-25, where the largest weight is at least 2^6; so by
+2^-31 of the largest, for every code of the row.  Scores are fp32 sums whose error is at most (d + 4) * 2^-24 times the sum of the magnitudes of
+their products, and an error e of a score changes its probability, and at most as much the normaliser, by e.
+"""
+
+import math
+
+import pytest
+import torch
+
+from cornserve import ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.fixture(autouse=True)
+def _no_kernel_error():
+    yield
+    torch.cuda.synchronize()
+    ops.check_error("after test")
+
+
+def _i32(a):
+    return torch.tensor(a, dtype=torch.int32, device=DEV)
+
+
+def _cs(T, d, start=0):
+    ang = (start + torch.arange(T, dtype=torch.float64, device=DEV))[:, None] * \
+        1e6 ** (-torch.arange(d // 2, dtype=torch.float64, device=DEV) * 2 / d)
+    return torch.stack([ang.cos(), ang.sin()], dim=1).float().contiguous()
+
+
+def _rows(cache, slots):
+    codes, scales = ops.kv_cache_fp8_views(cache)
+    p, r = slots.long() // 128, slots.long() % 128
+    return codes.view(torch.uint8)[p, :, :, r].view(torch.float8_e4m3fn).double(), scales[p, :, :, r].double()
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# append
+# ---------------------------------------------------------------------------------------------------------------------
+def _append_definition(qkv, Hq, Hkv, d, cs, wq, wk, eps):
+    x = qkv.double().view(qkv.shape[0], Hq + 2 * Hkv, d)
+    qk = x[:, : Hq + Hkv]
+    if wq is not None:
+        w = torch.cat([wq.double().expand(Hq, d), wk.double().expand(Hkv, d)])
+        qk = qk / (qk.square().mean(-1, True) + eps).sqrt() * w
+    c, s = cs.double()[:, None, 0], cs.double()[:, None, 1]
+    a, b = qk[..., : d // 2], qk[..., d // 2:]
+    qk = torch.cat([a * c - b * s, b * c + a * s], -1)
+    return qk[:, :Hq], torch.stack([qk[:, Hq:], x[:, Hq + Hkv:]], 1)      # [T, Hq, d], [T, 2, Hkv, d]
+
+
+@pytest.mark.parametrize("T,Hq,Hkv,d", [(1, 28, 4, 128), (1, 1, 1, 64), (5, 16, 2, 64), (300, 28, 4, 128), (129, 3, 3, 64), (2049, 32, 8, 128)])
+@pytest.mark.parametrize("norm", [False, True])
+def test_append_matches_the_definition(T, Hq, Hkv, d, norm):
+    torch.manual_seed(T + d + norm)
+    pages = T // 128 + 4
+    qkv = (torch.randn(T, (Hq + 2 * Hkv) * d, device=DEV) * torch.exp(torch.randn(T, 1, device=DEV))).bfloat16()
+    cs = _cs(T, d, 77)
+    wq, wk = ((1 + 0.1 * torch.randn(d, device=DEV)).bfloat16() for _ in range(2)) if norm else (None, None)
+    cache = torch.randint(0, 120, ops.kv_cache_fp8(pages, Hkv, d).shape, device=DEV, dtype=torch.uint8)
+    slot = (100 + torch.randperm(pages * 128 - 100, device=DEV)[:T]).int()
+    slot[::9] = -1
+    before, qkv_before = cache.clone(), qkv.clone()
+    q = ops.rope_kv_write_fp8_(qkv, Hq, Hkv, d, cs, cache, slot, wq, wk, 1e-5)
+    want_q, want_kv = _append_definition(qkv, Hq, Hkv, d, cs, wq, wk, 1e-5)
+    assert torch.equal(qkv, qkv_before)
+    amp = want_q.abs().amax(-1, keepdim=True)
+    assert ((q.double() - want_q).abs() <= want_q.abs() * 2 ** -8 + amp * 2 ** -20).all()
+    kept = slot >= 0
+    codes, scales = _rows(cache, slot[kept])
+    want = want_kv[kept]
+    unit = want.abs().amax(-1).clamp_min(2.0 ** -40) / 448
+    assert ((scales - unit).abs() <= unit * 2 ** -20).all()
+    assert ((codes - want / unit[..., None]).abs() <= (want / unit[..., None]).abs() * (2 ** -4 + 2 ** -18) + 2 ** -10 + 2 ** -12).all()
+    # every byte that belongs to no kept token is as it was
+    c, s = ops.kv_cache_fp8_views(cache)
+    c0, s0 = ops.kv_cache_fp8_views(before)
+    p, r = slot[kept].long() // 128, slot[kept].long() % 128
+    c.view(torch.uint8)[p, :, :, r] = c0.view(torch.uint8)[p, :, :, r]
+    s.view(torch.int32)[p, :, :, r] = s0.view(torch.int32)[p, :, :, r]
+    assert torch.equal(cache, before)
+
+
+def test_append_zero_tiny_huge_and_non_finite_rows_match_the_cpu():
+    d, Hq, Hkv, T = 128, 1, 1, 8
+    qkv = torch.zeros(T, 3 * d, device=DEV).bfloat16()
+    qkv[1] = 1e-30
+    qkv[2, d + 3] = float("inf")
+    qkv[3, 2 * d + 4] = float("nan")
+    qkv[4] = 3e38
+    qkv[5, 2 * d:] = -2.0 ** -40
+    qkv[6, 2 * d + 7] = float("-inf")
+    qkv[7] = 2.0 ** -133
+    cs = _cs(T, d)
+    cache = ops.kv_cache_fp8(1, Hkv, d, DEV)
+    ops.rope_kv_write_fp8_(qkv, Hq, Hkv, d, cs, cache, _i32(list(range(T))))
+    host = ops.kv_cache_fp8(1, Hkv, d)
+    ops.rope_kv_write_fp8_(qkv.cpu().float(), Hq, Hkv, d, cs.cpu(), host, torch.arange(T, dtype=torch.int32))
+    (c, s), (hc, hs) = ops.kv_cache_fp8_views(cache), ops.kv_cache_fp8_views(host)
+    # rows 2, 3 and 6, and the key of row 4: its rotation by 4 radians reaches 3e38 * |cos 4 + sin 4| = 4.2e38, beyond fp32
+    assert torch.equal(torch.isnan(s).cpu(), torch.isnan(hs)) and int(torch.isnan(hs).sum()) == 4
+    ok = ~torch.isnan(hs)
+    assert torch.allclose(s.cpu()[ok], hs[ok], rtol=2 ** -20, atol=0)
+    # codes: at most one step apart (their fp32 inputs may differ in the last bit next to a rounding border)
+    assert ((c.cpu().double() - hc.double()).abs() <= hc.double().abs() * 2 ** -3 + 2 ** -9).all()
+
+
+def test_append_takes_strided_and_misaligned_rows_and_empty_batches():
+    torch.manual_seed(1)
+    d, Hq, Hkv, T = 64, 2, 1, 10
+    wide = torch.randn(T, 4 * d + 5, device=DEV).bfloat16()
+    cs, slot = _cs(T, d), torch.arange(T, device=DEV, dtype=torch.int32)
+    ref_cache = ops.kv_cache_fp8(1, Hkv, d, DEV)
+    ref_q = ops.rope_kv_write_fp8_(wide[:, 3: 3 + 4 * d].contiguous(), Hq, Hkv, d, cs, ref_cache, slot)
+    cache = ops.kv_cache_fp8(1, Hkv, d, DEV)
+    q = ops.rope_kv_write_fp8_(wide[:, 3: 3 + 4 * d], Hq, Hkv, d, cs, cache, slot)
+    assert torch.equal(q, ref_q) and torch.equal(cache, ref_cache)
+    q = ops.rope_kv_write_fp8_(wide[:0, : 4 * d], Hq, Hkv, d, cs[:0], cache, slot[:0])
+    assert q.shape == (0, Hq, d) and torch.equal(cache, ref_cache)
+
+
+def test_a_slot_beyond_the_cache_is_skipped_and_reported():
+    d = 64
+    cache = ops.kv_cache_fp8(2, 1, d, DEV)
+    x = torch.ones(3, 3 * d, device=DEV).bfloat16()
+    ops.rope_kv_write_fp8_(x, 1, 1, d, _cs(3, d), cache, _i32([256, 2**31 - 1, 5]))
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="bad argument"):
+        ops.check_error("append")
+    codes, _ = ops.kv_cache_fp8_views(cache)
+    assert int((codes.float().abs().sum(-1) > 0).sum()) == 2     # the key and value row of slot 5
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------------------------------------------------
+def _filled_cache(pages, Hkv, d, seed=0):
+    """Every byte of the cache is something: rows of different sizes, and rows no sequence may look at."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    cache = ops.kv_cache_fp8(pages, Hkv, d, DEV)
+    codes, scales = ops.kv_cache_fp8_views(cache)
+    raw = torch.randint(0, 256, codes.shape, device=DEV, generator=g, dtype=torch.int32).to(torch.uint8)
+    raw[(raw & 0x7F) == 0x7F] = 0x35
+    codes.view(torch.uint8).copy_(raw)
+    scales.copy_(torch.exp(0.7 * torch.randn(scales.shape, device=DEV, generator=g)) / 150)
+    return cache
+
+
+def _poison(cache, table, lens):
+    """NaN codes and NaN / infinite scales in every row that lies behind a sequence's keys."""
+    codes, scales = ops.kv_cache_fp8_views(cache)
+    used = torch.zeros(cache.shape[0], 128, dtype=torch.bool)
+    for row, n in zip(table.tolist(), lens):
+        for b in range(-(-n // 128)):
+            used[row[b], : min(128, n - 128 * b)] = True
+    hide = (~used).to(DEV)[:, None, None, :].expand(scales.shape)
+    codes.view(torch.uint8)[hide] = 0x7F
+    scales[hide] = float("nan")
+    scales[:, 1][hide[:, 1]] = float("inf")
+
+
+def _check(out, q, cache, table, lens, new, causal=True, scale=None):
+    codes, scales = ops.kv_cache_fp8_views(cache)
+    _, Hq, d = q.shape
+    Hkv = cache.shape[2]
+    group = Hq // Hkv
+    scale = scale if scale is not None else 1 / math.sqrt(d)
+    at = 0
+    for i, (n, L) in enumerate(zip(new, lens)):
+        ids = table[i, : -(-L // 128)].long()
+        k, v = ((codes[ids, j].double() * scales[ids, j].double()[..., None]).transpose(1, 2).reshape(-1, Hkv, d)[:L]
+                .repeat_interleave(group, dim=1) for j in (0, 1))
+        vs = scales[ids, 1].double().transpose(1, 2).reshape(-1, Hkv)[:L].repeat_interleave(group, dim=1)     # [keys, Hq]
+        qq = q[at: at + n].double()
+        got = out[at: at + n].double()
+        at += n
+        if n == 0:
+            continue
+        vis = torch.ones(n, L, dtype=torch.bool, device=DEV)
+        if causal:
+            vis = torch.arange(L, device=DEV)[None] <= torch.arange(n, device=DEV)[:, None] + (L - n)
+        dead = ~vis.any(dim=1)
+        s = torch.einsum("qhd,khd->hqk", qq, k) * scale
+        mag = torch.einsum("qhd,khd->hqk", qq.abs(), k.abs()) * abs(scale)
+        p = torch.softmax(s.masked_fill(~vis, float("-inf")), -1).masked_fill(dead[:, None], 0.0)
+        want = torch.einsum("hqk,khd->qhd", p, v)
+        size = torch.einsum("hqk,khd->qhd", p, v.abs())
+        es = (mag.masked_fill(~vis, 0.0).amax(-1) * (d + 4) * 2.0 ** -24).transpose(0, 1)[..., None] if L else 0.0
+        top = (p * vs.t()[:, None, :]).amax(-1).transpose(0, 1)[..., None] if L else 0.0     # the largest weight of a row
+        code_sum = torch.einsum("qk,khd->qhd", vis.double(), (v / vs[..., None]).abs()) if L else 0.0
+        tol = want.abs() * 2.0 ** -8 + size * (2.0 ** -11 + 2 * es + 2.0 ** -18) + top * code_sum * 2.0 ** -31
+        assert not got[dead].any()
+        err = (got - want).abs()
+        assert (err <= tol).all(), f"sequence {i}: {n} of {L} keys, error {err.max().item():.3g} beyond tolerance by {(err - tol).max().item():.3g}"
+
+
+def _setup(lens, new, Hq, Hkv, d, seed=0, spare=3, poison=True):
+    g = torch.Generator(device=DEV).manual_seed(seed + 1)
+    blocks = [-(-n // 128) for n in lens]
+    pages = sum(blocks) + spare
+    cache = _filled_cache(pages, Hkv, d, seed)
+    order = torch.randperm(pages, generator=torch.Generator().manual_seed(seed)).tolist()
+    table = torch.full((len(lens), max(blocks + [1]) + 1), -7, dtype=torch.int32)      # unused entries are never read as pages
+    for i, n in enumerate(blocks):
+        table[i, :n] = torch.tensor([order.pop() for _ in range(n)], dtype=torch.int32)
+    if poison:
+        _poison(cache, table, lens)
+    cu = [0]
+    for n in new:
+        cu.append(cu[-1] + n)
+    q = torch.randn(cu[-1], Hq, d, device=DEV, generator=g) * torch.exp(torch.randn(cu[-1], Hq, 1, device=DEV, generator=g))
+    return q.bfloat16(), cache, table.to(DEV), _i32(lens), _i32(cu)
+
+
+HEADS = [(28, 4, 128), (16, 16, 64), (8, 1, 128), (32, 2, 64), (6, 2, 64), (5, 1, 128), (20, 1, 64), (40, 2, 128)]
+
+
+@pytest.mark.parametrize("Hq,Hkv,d", HEADS)
+@pytest.mark.parametrize("lens", [[1], [128], [129, 64, 65, 63, 1, 0, 127], [700, 0, 3000, 17], [5000], [300] * 70])
+def test_decode_attention(Hq, Hkv, d, lens):
+    new = [1] * len(lens)
+    q, cache, table, kv_len, cu = _setup(lens, new, Hq, Hkv, d, seed=len(lens))
+    out = ops.attention_paged_fp8(q, cache, table, kv_len, cu, 1)
+    _check(out, q, cache, table, lens, new)
+
+
+@pytest.mark.parametrize("Hq,Hkv,d", HEADS)
+@pytest.mark.parametrize("lens,new", [([1], [1]), ([2], [2]), ([300], [300]), ([128, 129, 127, 1], [128, 129, 127, 1]),
+                                      ([500, 20, 0, 64, 900], [3, 20, 0, 30, 257]), ([10, 5, 300], [12, 9, 2]), ([4100], [37])])
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompt_attention(Hq, Hkv, d, lens, new, causal):
+    q, cache, table, kv_len, cu = _setup(lens, new, Hq, Hkv, d, seed=len(lens) + sum(new))
+    out = ops.attention_paged_fp8(q, cache, table, kv_len, cu, max(new), causal=causal)
+    _check(out, q, cache, table, lens, new, causal)
+
+
+def test_long_prompt_attention():
+    lens, new = [2500, 1700], [2500, 1025]
+    q, cache, table, kv_len, cu = _setup(lens, new, 14, 2, 128, seed=5)
+    _check(ops.attention_paged_fp8(q, cache, table, kv_len, cu, 2500), q, cache, table, lens, new)
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [40, 3, 77]])
+@pytest.mark.parametrize("scale", [None, 0.0, 0.5, -0.1])
+def test_strides_given_output_rows_behind_the_last_sequence_and_scale(new, scale):
+    lens = [200, 130, 90]
+    q, cache, table, kv_len, cu = _setup(lens, new, 8, 2, 64, seed=9)
+    T = q.shape[0]
+    wide = torch.full((T + 4, 8 * 64 + 11), 3.0, device=DEV, dtype=torch.bfloat16)
+    qs = wide[:, 5: 5 + 512].unflatten(1, (8, 64))       # odd row stride, odd start
+    qs[:T] = q
+    hs = torch.empty(8, T + 4, 64, device=DEV, dtype=torch.bfloat16).transpose(0, 1)     # heads outermost
+    hs[:T] = q
+    big_table = torch.full((3, 40), -9, device=DEV, dtype=torch.int32)
+    big_table[:, : table.shape[1]] = table
+    for x in (qs, hs):
+        out = torch.full((T + 4, 8, 100), 7.0, device=DEV, dtype=torch.bfloat16)
+        if new == [1, 1, 1]:
+            x, out = x[:T], out[:T]       # one token per sequence: as many rows as sequences
+        got = ops.attention_paged_fp8(x, cache, big_table, kv_len, cu, max(new), scale=scale, out=out[..., 9:73])
+        assert got.data_ptr() == out[..., 9:73].data_ptr()
+        assert (out[T:] == 7.0).all() and (out[..., :9] == 7.0).all() and (out[..., 73:] == 7.0).all()
+        _check(out[:T, :, 9:73], q, cache, table, lens, new, scale=scale)
+
+
+@pytest.mark.parametrize("n", [1, 20])
+def test_extreme_scores_scales_and_queries(n):
+    """One key that outweighs all others; value rows whose sizes differ by 2^60; queries of 2^-60 and 2^60."""
+    lens, new = [700, 700, 700, 700], [n] * 4
+    q, cache, table, kv_len, cu = _setup(lens, new, 8, 2, 64, seed=11)
+    codes, scales = ops.kv_cache_fp8_views(cache)
+    p = table[0].long()
+    scales[p[2], 0, :, 17] = 5.0                       # sequence 0: a key far larger than the others
+    scales[table[1, :5].long(), 1] *= 2.0 ** 40        # sequence 1: large values, and one page of tiny ones
+    scales[table[1, 1].long(), 1] *= 2.0 ** -60
+    scales[table[1, 5].long(), 1, :, : 700 - 640] *= 2.0 ** 40
+    q[2 * n: 3 * n] *= 2.0 ** -60
+    scales[table[3, :5].long(), 0] *= 2.0 ** -60       # sequence 3: tiny keys, huge queries
+    scales[table[3, 5].long(), 0, :, : 700 - 640] *= 2.0 ** -60
+    q[3 * n:] *= 2.0 ** 60
+    _check(ops.attention_paged_fp8(q, cache, table, kv_len, cu, n), q, cache, table, lens, new)
+
+
+@pytest.mark.parametrize("n", [1, 20])
+def test_a_nan_row_spreads_only_to_the_queries_that_see_it(n):
+    lens, new = [300, 300], [n, n]
+    q, cache, table, kv_len, cu = _setup(lens, new, 4, 2, 128, seed=12)
+    codes, scales = ops.kv_cache_fp8_views(cache)
+    page, row = int(table[0, 2]), 300 - 257                 # the last key of sequence 0
+    scales[page, 0, 1, row] = float("nan")                  # its key, second key head
+    scales[page, 1, 0, row] = float("nan")                  # its value, first key head
+    codes.view(torch.uint8)[page, :, :, row] = 0
+    out = ops.attention_paged_fp8(q, cache, table, kv_len, cu, n)
+    assert torch.isnan(out[n - 1]).all()
+    assert not torch.isnan(out[: n - 1]).any() and not torch.isnan(out[n:]).any()
+
+
+@pytest.mark.parametrize("new", [[1] * 6, [64, 3, 0, 5, 129, 40]])
+def test_tables_and_lengths_that_do_not_fit_are_reported(new):
+    lens = [300, 64, 10, 129, 500, 40]
+    q, cache, table, kv_len, cu = _setup(lens, new, 8, 2, 64, seed=13, poison=False)
+    good = ops.attention_paged_fp8(q, cache, table, kv_len, cu, max(new))
+    bad_table = table.clone()
+    bad_table[0, 1] = cache.shape[0]
+    bad_table[4, 2] = -1
+    ops.attention_paged_fp8(q, cache, bad_table, kv_len, cu, max(new))
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="bad argument"):
+        ops.check_error("pages")
+    bad_len = kv_len.clone()
+    bad_len[1] = 128 * table.shape[1] + 1
+    out = ops.attention_paged_fp8(q, cache, torch.where(table < 0, 0, table).int(), bad_len, cu, max(new))
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="bad argument"):
+        ops.check_error("length")
+    a, b = sum(new[:1]), sum(new[:2])
+    assert torch.equal(out[:a], good[:a]) and torch.equal(out[b:], good[b:])     # the others are unharmed
+
+
+def test_results_do_not_depend_on_the_run_or_the_batch_order():
+    lens = [5, 2000, 700, 333, 128]
+    q, cache, table, kv_len, cu = _setup(lens, [1] * 5, 28, 4, 128, seed=21)
+    a = ops.attention_paged_fp8(q, cache, table, kv_len, cu, 1)
+    for _ in range(5):
+        assert torch.equal(a, ops.attention_paged_fp8(q, cache, table, kv_len, cu, 1))
+
+
+def test_empty_calls():
+    q, cache, table, kv_len, cu = _setup([5], [1], 4, 2, 64)
+    assert ops.attention_paged_fp8(q[:0], cache, table[:0], kv_len[:0], cu[:1], 0).shape == (0, 4, 64)
+    zero = torch.zeros_like(kv_len)
+    assert not ops.attention_paged_fp8(q, cache, table, zero, cu, 1).any()
+    assert not ops.attention_paged_fp8(q, cache, table[:, :0], zero, cu, 1).any()
+    q3 = q.repeat(3, 1, 1)
+    assert not ops.attention_paged_fp8(q3, cache, table, zero, _i32([0, 3]), 3).any()
+    assert not ops.attention_paged_fp8(q3, cache, table[:, :0], zero, _i32([0, 3]), 3).any()
+
+
+def test_other_head_widths_are_refused_on_the_gpu():
+    cache = ops.kv_cache_fp8(1, 1, 32, DEV)
+    with pytest.raises(ValueError, match="head widths"):
+        ops.attention_paged_fp8(torch.zeros(1, 1, 32, device=DEV).bfloat16(), cache, _i32([[0]]), _i32([1]), _i32([0, 1]), 1)
+    cache = ops.kv_cache_fp8(1, 1, 64, DEV)
+    with pytest.raises(ValueError):
+        ops.attention_paged_fp8(torch.zeros(1, 1, 64, device=DEV), cache, _i32([[0]]), _i32([1]), _i32([0, 1]), 1)
+    with pytest.raises(ValueError):
+        ops.attention_paged_fp8(torch.zeros(1, 1, 64).bfloat16(), cache, _i32([[0]]), _i32([1]), _i32([0, 1]), 1)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# together: append then attend, on other streams and from graphs
+# ---------------------------------------------------------------------------------------------------------------------
+def _step(qkv, cs, cache, slot, table, kv_len, cu, n, Hq, Hkv, d):
+    q = ops.rope_kv_write_fp8_(qkv, Hq, Hkv, d, cs, cache, slot)
+    return ops.attention_paged_fp8(q, cache, table, kv_len, cu, n)
+
+
+def test_prompt_then_decode_steps_match_one_pass_over_all_tokens():
+    torch.manual_seed(2)
+    d, Hq, Hkv, T, tail = 128, 8, 2, 333, 6
+    qkv = torch.randn(T, (Hq + 2 * Hkv) * d, device=DEV).bfloat16()
+    cs = _cs(T, d)
+    table = _i32([[2, 0, 3]])
+    slot = (table[0].long()[torch.arange(T, device=DEV) // 128] * 128 + torch.arange(T, device=DEV) % 128).int()
+    one = ops.kv_cache_fp8(4, Hkv, d, DEV)
+    want = _step(qkv, cs, one, slot, table, _i32([T]), _i32([0, T]), T, Hq, Hkv, d)
+    cache = ops.kv_cache_fp8(4, Hkv, d, DEV)
+    m = T - tail
+    parts = [_step(qkv[:100], cs[:100], cache, slot[:100], table, _i32([100]), _i32([0, 100]), 100, Hq, Hkv, d),
+             _step(qkv[100:m], cs[100:m], cache, slot[100:m], table, _i32([m]), _i32([0, m - 100]), m - 100, Hq, Hkv, d)]
+    for t in range(m, T):
+        parts.append(_step(qkv[t: t + 1], cs[t: t + 1], cache, slot[t: t + 1], table, _i32([t + 1]), _i32([0, 1]), 1, Hq, Hkv, d))
+    assert torch.equal(cache, one)
+    got = torch.cat(parts)
+    codes, scales = ops.kv_cache_fp8_views(one)
+    v = (codes[table[0].long(), 1].double() * scales[table[0].long(), 1].double()[..., None]).abs().amax()
+    # both are within their tolerance of the definition
+    assert ((got.double() - want.double()).abs() <= want.double().abs() * 2 ** -7 + v * 2 ** -9).all()
+    assert torch.nn.functional.cosine_similarity(got.float().flatten(), want.float().flatten(), dim=0) > 0.9999
+
+
+@pytest.mark.parametrize("n", [1, 30])
+def test_graphs_replayed_at_once_on_two_streams_and_with_new_lengths(n):
+    Hq, Hkv, d, B = 28, 4, 128, 3
+    sets = []
+    for seed in (31, 32):
+        q, cache, table, kv_len, cu = _setup([2000, 900, 1500], [n] * B, Hq, Hkv, d, seed=seed, poison=False)
+        table = table.clamp_min(0)
+        want = ops.attention_paged_fp8(q, cache, table, kv_len, cu, n).clone()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            ops.attention_paged_fp8(q, cache, table, kv_len, cu, n)
+        side.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = ops.attention_paged_fp8(q, cache, table, kv_len, cu, n)
+        sets.append((g, out, want, side, q, cache, table, kv_len, cu))
+    for _ in range(20):
+        for g, _, _, side, *_ in sets:
+            with torch.cuda.stream(side):
+                g.replay()
+    torch.cuda.synchronize()
+    for _, out, want, *_ in sets:
+        assert torch.equal(out, want)
+    # the graph reads the lengths on the device: shorter sequences need no new capture
+    g, out, _, _, q, cache, table, kv_len, cu = sets[0]
+    lens = [40, 900, 777]
+    kv_len.copy_(_i32(lens))
+    g.replay()
+    torch.cuda.synchronize()
+    _check(out, q, cache, table, lens, [n] * B)
+
+
+def test_engine_with_an_8_bit_cache_decodes_from_graphs_like_it_does_eagerly():
+    import numpy as np
+
+    from cornserve.models.qwen_llm import LLMConfig, QwenLLM
+    from cornserve.task_executors.llm.engine import EngineConfig, LLMEngine, SamplingParams, Sequence
+
+    torch.manual_seed(0)
+    cfg = LLMConfig(hidden_size=512, num_hidden_layers=2, num_attention_heads=8, num_key_value_heads=2, head_dim=64, intermediate_size=1024,
+                    vocab_size=1024, mrope_section=None, qk_norm=True, attention_bias=False, eos_token_id=1023)
+    model = QwenLLM(cfg, device=DEV).eval()
+    prompts = [np.arange(3, 3 + n, dtype=np.int32) for n in (5, 140, 260)]
+    got = []
+    for graph in (True, False):
+        eng = LLMEngine(model, EngineConfig(num_pages=32, decode_burst=4, max_model_len=512, kv_cache_dtype="fp8", use_cuda_graph=graph))
+        assert eng.kv_backing.dtype == torch.uint8
+        got.append(eng.generate([Sequence(f"s{i}", p, SamplingParams(max_tokens=9, ignore_eos=True)) for i, p in enumerate(prompts)]))
+    assert all(len(t) == 9 for t in got[0].values())
+    # the graph pads the batch to its bucket, which changes no row of the attention but may change the projections' kernel
+    same = sum(a == b for k in got[0] for a, b in zip(got[0][k], got[1][k]))
+    assert same >= 3 and got[0]["s0"][0] == got[1]["s0"][0]
