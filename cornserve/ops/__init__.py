@@ -562,7 +562,7 @@ def attention_paged_fp8(q: torch.Tensor, cache: torch.Tensor, block_table: torch
         return reference.attention_paged_fp8(q, cache, block_table, kv_len, cu_q, scale, causal, out)
     _kv_fp8_on_device(cache, d)
     _need(q.dtype == torch.bfloat16, "the CUDA kernel takes bf16 queries")
-    if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+    if q.stride(2) != 1 or q.stride(1) != d or q.stride(0) % 8 or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
     if out is None:
         out = torch.empty((Tq, Hq, d), device=q.device, dtype=torch.bfloat16)
@@ -574,7 +574,7 @@ def attention_paged_fp8(q: torch.Tensor, cache: torch.Tensor, block_table: torch
         # scratch of this call alone: calls on several streams, and captured graphs, never share it
         nbytes = lib.cs_attention_decode_fp8_ws_bytes(Hq, Hkv, d)
         ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8)
-        _chk(lib.cs_attention_decode_fp8(q.data_ptr(), q.stride(0), q.stride(1), cache.data_ptr(), cache.shape[0], out.data_ptr(),
+        _chk(lib.cs_attention_decode_fp8(q.data_ptr(), q.stride(0), cache.data_ptr(), cache.shape[0], out.data_ptr(),
                                          out.stride(0), out.stride(1), kv_len.data_ptr(), block_table.data_ptr(), block_table.stride(0),
                                          block_table.shape[1], B, Hq, Hkv, d, float(scale), ws.data_ptr(), nbytes, _stream()),
              "cs_attention_decode_fp8")

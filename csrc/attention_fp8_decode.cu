@@ -9,50 +9,59 @@
 //
 // The kernel is bound by the cache's bytes, and everything is arranged around reading them once, without a pause:
 //
-//   * Work is counted in units of 64 keys of one (sequence, key head); the list of all units of the batch is cut into
-//     equal runs, one per CTA, on the device from kv_len.  So any mix of lengths loads every SM alike (a captured graph
-//     adapts to the lengths of each replay), and a single long sequence is spread over the whole GPU.  A CTA has at most
-//     two items that it does not own alone, the first and the last of its run: these leave partial sums in a workspace
-//     and a second small kernel joins them in the order of the CTAs (no atomics, the result does not depend on timing).
-//   * One producer warp keeps a ring of stages full by TMA (K and V codes through a tensor map with a swizzle, scales by
-//     plain bulk copies).
-//   * Eight consumer warps: warp w takes keys 16 (w % 4) .. + 15 of every second unit, entirely in registers: S^T = K Q^T
-//     and O^T += V^T P with mma.m16n8k16, keys (channels) on the 16 side and up to 8 query heads per n tile on the other.
-//     mma.sync and not tcgen05 on purpose: e4m3 becomes fp16 on the way from shared memory to a register fragment, while
-//     a tcgen05 operand would have to be written back to shared memory twice as wide; tensor time is not what is scarce
-//     at 8 to 16 heads per byte of K.  The warps share nothing until an item ends; then their sums meet in shared memory.
+//   * Work is counted in units of 64 keys (128 for the narrow heads) of one (sequence, key head); the list of all units
+//     of the batch is cut into equal runs, one per CTA, on the device from kv_len.  So any mix of lengths loads every SM
+//     alike (a captured graph adapts to the lengths of each replay), and a single long sequence is spread over the whole
+//     GPU.  A CTA has at most two items that it does not own alone, the first and the last of its run: these leave partial
+//     sums in a workspace and a second small kernel joins them in the order of the CTAs (no atomics, the result does not
+//     depend on timing).
+//   * A CTA is three (or two) teams of four consumer warps and one producer warp.  A team has its own ring of stages, kept
+//     full by TMA: one copy brings the K and V codes of a unit (through a tensor map with a swizzle), one its scales.
+//     Long visits to an item are shared by the teams, unit by unit; short ones are dealt whole to one team each, so that
+//     the end of one sequence overlaps the reading of others.
+//   * Consumer warp w of a team takes a quarter of the unit's keys, entirely in registers: S^T = K Q^T and O^T += V^T P
+//     with mma.m16n8k16, keys (channels) on the 16 side and up to 8 query heads per n tile on the other.  mma.sync and
+//     not tcgen05 on purpose: e4m3 becomes fp16 on the way from shared memory to a register fragment, while a tcgen05
+//     operand would have to be written back to shared memory twice as wide; tensor time is not what is scarce at 8 to 16
+//     heads per byte of K.  The warps share nothing until a visit ends; then their sums meet in shared memory.
 #include <math.h>
 
 #include "kv_fp8.cuh"
 
-int cs_encode_tmap_3d_u8(CUtensorMap* out, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t s1_bytes,
-                         uint64_t s2_bytes, uint32_t b0, uint32_t b1, uint32_t b2, int swizzle_bytes);
+int cs_encode_tmap_nd(CUtensorMap* out, int elem_bytes, int rank, const void* base, const uint64_t* dims, const uint64_t* strides,
+                      const uint32_t* box, int swizzle_bytes);
 
 namespace {
 
-constexpr int UNIT = 64;                     // keys per unit of work
-constexpr int CONSUMERS = 8;                 // warps
-constexpr int DEC_THREADS = (CONSUMERS + 1) * 32;
 constexpr int MAX_CTAS = 512;
+constexpr int SHARED_VISIT = 8;              // visits of at least this many units are shared by the teams of a CTA
 constexpr float M_NONE = -3.0e38f;           // running maximum before the first key (finite: differences stay defined)
 
-// Shared memory of one instantiation.
+// One instantiation.  TEAMS: as many as registers allow (128 a thread with three teams, 168 with two).
 template <int D, int NT>
 struct DecShape {
   static constexpr int HEADS = 8 * NT;
+  static constexpr int TEAMS = (D == 128 && NT == 2) ? 2 : 3;
+  static constexpr int KT = D == 128 ? 1 : 2;                // 16-key tiles per consumer warp and unit
+  static constexpr int UNIT = 64 * KT;                       // keys
+  static constexpr int WARPS = 4 * TEAMS;                    // consumers
+  static constexpr int THREADS = (WARPS + TEAMS) * 32;
   static constexpr int TILE = UNIT * D;                      // bytes of codes of K (or V) per stage
-  static constexpr int JOIN_LD = D + 4;                      // floats between two heads of a warp's partial sum
-  static constexpr int JOIN = CONSUMERS * HEADS * JOIN_LD * 4;
   static constexpr int STAGE = 2 * TILE + 2 * UNIT * 4;
-  static constexpr int FIT = (227 * 1024 - 2048 - 2 * CONSUMERS * HEADS * 4 - JOIN) / STAGE;
-  static constexpr int STAGES = FIT < 16 ? FIT : 16;
-  static constexpr int SMEM = 1024 + STAGES * STAGE + JOIN;
+  static constexpr int JOIN_LD = D + 4;                      // floats between two heads of a warp's partial sum
+  static constexpr int JOIN = WARPS * HEADS * JOIN_LD * 4;
+  static constexpr int Q = HEADS * D * 2;                    // queries of one visit
+  static constexpr int QSLOTS = 2;                           // per team
+  static constexpr int FIT = (227 * 1024 - 1024 - 4096 - JOIN - TEAMS * QSLOTS * Q) / STAGE;
+  static constexpr int RING = FIT / TEAMS < 8 ? FIT / TEAMS : 8;   // stages per team
+  static constexpr int SMEM = 1024 + TEAMS * RING * STAGE + TEAMS * QSLOTS * Q + JOIN;
+  static_assert(RING >= 3, "a stage in use and two on their way");
 };
 
 struct DecParams {
-  const __nv_bfloat16* q; long long q_tok, q_head;     // strides in elements, rows on 16-byte boundaries
+  const __nv_bfloat16* q; long long q_tok;             // heads follow each other; every token on a 16-byte boundary
   __nv_bfloat16* o; long long o_tok, o_head; int o_vec; // o_vec: 8-byte stores are aligned
-  const uint8_t* cache; int num_pages;
+  int num_pages;
   const int* block_table; long long bt_stride; int bt_width;
   const int* kv_len;
   int B, Hq, Hkv, G, head_blocks;                      // G query heads per key head, in blocks of 8 NT
@@ -69,14 +78,14 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
   uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
@@ -99,6 +108,18 @@ __device__ __forceinline__ void bulk_load(uint32_t smem_dst, const void* src, ui
                "r"(bytes), "r"(smem_u32(bar))
                : "memory");
 }
+__device__ __forceinline__ void tma_load_4d(uint32_t smem_dst, const CUtensorMap* m, int x, int y, int z, int w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_5d(uint32_t smem_dst, const CUtensorMap* m, int x, int y, int z, int w, int v, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v), "r"(smem_u32(bar))
+      : "memory");
+}
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -110,13 +131,27 @@ __device__ __forceinline__ int dec_len(const DecParams& p, int b) {
   const long long cap = static_cast<long long>(p.bt_width) * KV8_PAGE;
   return n < 0 ? 0 : (n > cap ? static_cast<int>(cap) : n);
 }
-__device__ __forceinline__ int dec_units(const DecParams& p, int b) { return (dec_len(p, b) + UNIT - 1) / UNIT; }
+
+// Four channels of one head: sums divided by the normaliser (0 when no key took part).
+__device__ __forceinline__ void store_head(const DecParams& p, int seq, int head, int lane, const float4& acc, float sum) {
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  __nv_bfloat16* dst = p.o + seq * p.o_tok + head * p.o_head + lane * 4;
+  const uint2 v = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+  if (p.o_vec) {
+    *reinterpret_cast<uint2*>(dst) = v;
+  } else {
+    unsigned short* d16 = reinterpret_cast<unsigned short*>(dst);
+    d16[0] = v.x & 0xffffu; d16[1] = v.x >> 16; d16[2] = v.y & 0xffffu; d16[3] = v.y >> 16;
+  }
+}
 
 // One visit of a CTA to an item: units [u, u + n) of `units` of sequence `seq`, head block `head` (of Hkv * head_blocks).
 // Every role of the CTA walks the same list of visits.
+template <int UNIT>
 struct Walk {
   int seq, head, units, len, u, n;
   long long left;   // units of the CTA's run not yet handed out, this visit included
+  uint32_t dealt;   // short visits and units of shared visits so far: deals the next ones to the teams in turn
   __device__ __forceinline__ bool settle(const DecParams& p) {   // on to a sequence with keys
     for (; seq < p.B; ++seq) {
       len = dec_len(p, seq);
@@ -128,7 +163,9 @@ struct Walk {
     }
     return false;
   }
+  __device__ __forceinline__ bool shared() const { return n >= SHARED_VISIT; }
   __device__ __forceinline__ bool next(const DecParams& p) {
+    dealt += shared() ? n : 1;
     left -= n;
     if (left <= 0) return false;
     u = 0;
@@ -136,59 +173,76 @@ struct Walk {
     n = static_cast<int>(min(static_cast<long long>(units), left));
     return true;
   }
+  // the units of this visit that belong to `team`: first, first + step, ... below u + n
+  template <int TEAMS>
+  __device__ __forceinline__ bool mine(int team, int& first, int& step) const {
+    const int turn = static_cast<int>((team + TEAMS - dealt % TEAMS) % TEAMS);
+    step = shared() ? TEAMS : 1;
+    first = u + (shared() ? turn : 0);
+    return shared() || turn == 0;
+  }
 };
 
 template <int D, int NT>
-__global__ void __launch_bounds__(DEC_THREADS, 1)
-attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm, const DecParams p) {
+__global__ void __launch_bounds__(DecShape<D, NT>::THREADS, 1)
+attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_codes, const __grid_constant__ CUtensorMap tm_scales, const DecParams p) {
   using Shape = DecShape<D, NT>;
-  constexpr int HEADS = Shape::HEADS, STAGES = Shape::STAGES, TILE = Shape::TILE, JOIN_LD = Shape::JOIN_LD;
+  constexpr int HEADS = Shape::HEADS, TEAMS = Shape::TEAMS, KT = Shape::KT, UNIT = Shape::UNIT, WARPS = Shape::WARPS;
+  constexpr int THREADS = Shape::THREADS, ALL_WARPS = THREADS / 32, RING = Shape::RING, QSLOTS = Shape::QSLOTS;
+  constexpr int TILE = Shape::TILE, JOIN_LD = Shape::JOIN_LD;
   constexpr int KSTEPS = D / 16, MT = D / 16, VPER = D / 8;   // VPER: channels of a value row per thread
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* s_codes = smem;                                              // STAGES x (K tile, V tile)
-  float* s_scale = reinterpret_cast<float*>(smem + STAGES * 2 * TILE);  // STAGES x (64 key scales, 64 value scales)
-  float* s_join = s_scale + STAGES * 2 * UNIT;                          // [warp][head][JOIN_LD]
-  __shared__ uint64_t full[STAGES], empty[STAGES];
-  __shared__ float s_m[CONSUMERS][HEADS], s_l[CONSUMERS][HEADS];
+  uint8_t* s_codes = smem;                                                   // [team][stage] K tile, V tile
+  uint8_t* s_scale = s_codes + TEAMS * RING * 2 * TILE;                      // [team][stage] key scales, value scales
+  uint8_t* s_q = s_scale + TEAMS * RING * 2 * UNIT * 4;                      // [team][slot][head][D] bf16
+  float* s_join = reinterpret_cast<float*>(s_q + TEAMS * QSLOTS * Shape::Q); // [warp][head][JOIN_LD]
+  __shared__ uint64_t full[TEAMS][RING], empty[TEAMS][RING], q_full[TEAMS][QSLOTS], q_empty[TEAMS][QSLOTS];
+  __shared__ float s_m[WARPS][HEADS], s_l[WARPS][HEADS];
   __shared__ int abort_flag, s_start_seq;
-  __shared__ long long s_warp_sum[CONSUMERS + 1], s_start_off;
+  __shared__ long long s_warp_sum[ALL_WARPS], s_start_off;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     abort_flag = 0;
     s_start_seq = 0;
     s_start_off = 0;
-    for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], CONSUMERS / 2); }
+    for (int w = 0; w < TEAMS; ++w) {
+      for (int s = 0; s < RING; ++s) { mbar_init(&full[w][s], 1); mbar_init(&empty[w][s], 4); }
+      for (int s = 0; s < QSLOTS; ++s) { mbar_init(&q_full[w][s], 1); mbar_init(&q_empty[w][s], 4); }
+    }
     mbar_fence_init();
-    tma_prefetch_desc(&tm);
+    tma_prefetch_desc(&tm_codes);
+    tma_prefetch_desc(&tm_scales);
   }
   // the lengths, the queries and the cache rows of this step come from the kernels ahead in the stream
   pdl_wait();
   pdl_launch_dependents();
+  if (threadIdx.x == 0) p.ws_item[blockIdx.x * 2] = p.ws_item[blockIdx.x * 2 + 1] = -1;
 
   // ------------------------------- this CTA's run of units -------------------------------
   const int heads = p.Hkv * p.head_blocks;
+  auto units_of = [&](int b) { return (dec_len(p, b) + UNIT - 1) / UNIT; };
   long long mine = 0;
-  for (int b = threadIdx.x; b < p.B; b += DEC_THREADS) mine += dec_units(p, b);
+  for (int b = threadIdx.x; b < p.B; b += THREADS) mine += units_of(b);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
   if (lane == 0) s_warp_sum[warp] = mine;
   __syncthreads();
   long long total = 0;
 #pragma unroll
-  for (int w = 0; w <= CONSUMERS; ++w) total += s_warp_sum[w];
+  for (int w = 0; w < ALL_WARPS; ++w) total += s_warp_sum[w];
   total *= heads;
   // no CTA of the first `active` is without a unit, so the CTAs that share an item are consecutive
   const long long active = min(total, static_cast<long long>(gridDim.x));
   long long r0 = 0, r1 = 0;
   if (blockIdx.x < active) { r0 = total * blockIdx.x / active; r1 = total * (blockIdx.x + 1) / active; }
   long long before = 0;   // units (all heads) of the sequences ahead of this chunk
-  for (int base = 0; base < p.B && r1 > r0; base += DEC_THREADS) {
+  for (int base = 0; base < p.B && r1 > r0; base += THREADS) {
     __syncthreads();
     const int b = base + threadIdx.x;
-    const long long units = b < p.B ? static_cast<long long>(dec_units(p, b)) * heads : 0;
+    const long long units = b < p.B ? static_cast<long long>(units_of(b)) * heads : 0;
     long long incl = units;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -200,61 +254,65 @@ attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm, const DecPar
     for (int w = 0; w < warp; ++w) incl += s_warp_sum[w];
     incl += before;
     if (r0 < incl && r0 >= incl - units) { s_start_seq = b; s_start_off = r0 - (incl - units); }
-    for (int w = 0; w <= CONSUMERS; ++w) before += s_warp_sum[w];
+    for (int w = 0; w < ALL_WARPS; ++w) before += s_warp_sum[w];
     if (before > r0) break;
   }
   __syncthreads();
   volatile int* abortp = &abort_flag;
-  Walk wk{};
+  Walk<UNIT> wk{};
   wk.seq = s_start_seq;
   wk.left = r1 - r0;
-  const int start_units = max(1, dec_units(p, wk.seq));
+  const int start_units = max(1, units_of(wk.seq));
   wk.head = static_cast<int>(s_start_off / start_units);
   wk.u = static_cast<int>(s_start_off - static_cast<long long>(wk.head) * start_units);
   const bool any = r1 > r0 && wk.settle(p);
-  if (threadIdx.x == 0) p.ws_item[blockIdx.x * 2] = p.ws_item[blockIdx.x * 2 + 1] = -1;
 
-  if (warp == CONSUMERS) {
-    // ------------------------------- producer -------------------------------
-    if (any) {
-      uint32_t n = 0;
-      bool ok = true;
-      do {
-        const int hk = wk.head / p.head_blocks;
-        const int* table = p.block_table + wk.seq * p.bt_stride;
-        int page_lane = 0, page_base = -64;   // the 32 table entries held by the lanes start at page_base
-        for (int u = wk.u; u < wk.u + wk.n && ok; ++u, ++n) {
-          const int blk = u / (KV8_PAGE / UNIT), half = u % (KV8_PAGE / UNIT);
-          if (blk >= page_base + 32 || page_base < 0) {
-            page_base = blk;
-            page_lane = blk + lane < (wk.len + KV8_PAGE - 1) / KV8_PAGE ? table[blk + lane] : 0;
-          }
-          int page = __shfl_sync(0xffffffffu, page_lane, blk - page_base);
-          if (lane == 0) {
-            if (page < 0 || page >= p.num_pages) { cs_set_error(p.err, CS_ERR_BAD_ARG); page = 0; }
-            const uint32_t s = n % STAGES;
-            if (mbar_wait(&empty[s], ((n / STAGES) & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT)) {
-              const int block = (page * 2) * p.Hkv + hk;
-              uint8_t* codes = s_codes + s * 2 * TILE;
-              float* scale = s_scale + s * 2 * UNIT;
-              const uint8_t* src = p.cache + block * kv8_block_bytes(D) + KV8_PAGE * D + half * UNIT * 4;
-              mbar_arrive_expect_tx(&full[s], 2 * TILE + 2 * UNIT * 4);
-              tma_load_3d(codes, &tm, 0, half * UNIT, block, &full[s]);
-              bulk_load(smem_u32(scale), src, UNIT * 4, &full[s]);
-              tma_load_3d(codes + TILE, &tm, 0, half * UNIT, block + p.Hkv, &full[s]);
-              bulk_load(smem_u32(scale + UNIT), src + p.Hkv * kv8_block_bytes(D), UNIT * 4, &full[s]);
-            } else {
-              ok = false;
-            }
-          }
-          ok = __shfl_sync(0xffffffffu, ok, 0);
+  if (warp >= WARPS) {
+    // ------------------------------- producer of one team -------------------------------
+    const int team = warp - WARPS;
+    uint32_t n = 0, nv = 0;   // running counts: units, visits
+    bool ok = true;
+    if (any) do {
+      int first, step;
+      if (!wk.template mine<TEAMS>(team, first, step)) continue;
+      const int hk = wk.head / p.head_blocks, hb = wk.head - hk * p.head_blocks;
+      if (lane == 0) {
+        const uint32_t slot = nv % QSLOTS;
+        ok = mbar_wait(&q_empty[team][slot], ((nv / QSLOTS) & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
+        if (ok) {
+          const uint32_t bytes = min(HEADS, p.G - hb * HEADS) * D * 2;
+          mbar_arrive_expect_tx(&q_full[team][slot], bytes);
+          bulk_load(smem_u32(s_q + (team * QSLOTS + slot) * Shape::Q), p.q + wk.seq * p.q_tok + (hk * p.G + hb * HEADS) * D, bytes,
+                    &q_full[team][slot]);
         }
-      } while (ok && wk.next(p));
-    }
+      }
+      ++nv;
+      const int* table = p.block_table + wk.seq * p.bt_stride;
+      int page_lane = 0, page_base = -64;   // the 32 table entries held by the lanes start at page_base
+      for (int u = first; u < wk.u + wk.n; u += step, ++n) {
+        const int blk = u / (KV8_PAGE / UNIT), part = u % (KV8_PAGE / UNIT);
+        if (blk >= page_base + 32 || page_base < 0) {
+          page_base = blk;
+          page_lane = blk + lane < (wk.len + KV8_PAGE - 1) / KV8_PAGE ? table[blk + lane] : 0;
+        }
+        int page = __shfl_sync(0xffffffffu, page_lane, blk - page_base);
+        if (lane == 0 && ok) {
+          if (page < 0 || page >= p.num_pages) { cs_set_error(p.err, CS_ERR_BAD_ARG); page = 0; }
+          const uint32_t s = n % RING;
+          ok = mbar_wait(&empty[team][s], ((n / RING) & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
+          if (ok) {
+            const int stage = team * RING + s;
+            mbar_arrive_expect_tx(&full[team][s], Shape::STAGE);
+            tma_load_5d(smem_u32(s_codes + stage * 2 * TILE), &tm_codes, 0, part * UNIT, hk, 0, page, &full[team][s]);
+            tma_load_4d(smem_u32(s_scale + stage * 2 * UNIT * 4), &tm_scales, part * UNIT, hk, 0, page, &full[team][s]);
+          }
+        }
+      }
+    } while (wk.next(p));
   } else {
     // ------------------------------- consumers -------------------------------
     const int g = lane >> 2, t = lane & 3;
-    const int kw = (warp & 3) * 16, team = warp >> 2;
+    const int team = warp >> 2, kw = (warp & 3) * 16 * KT;
     // Fragment row r (0..7) of a 16-key tile holds key ord(r) (and row r + 8 key ord(r) + 8).  The order is such that the
     // eight threads of a shared-memory phase touch all banks: the K rows of neighbouring fragment rows (their 16-byte
     // chunks differ by the swizzle), and the V rows ord(2t), ord(2t + 1) of the threads of a quad.
@@ -267,28 +325,32 @@ attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm, const DecPar
     auto at = [](int row, int c) { return row * D + ((D == 128 ? c ^ (row & 7) : c ^ ((row >> 1) & 3)) << 4); };
     const int key0 = kw + ord(g);
     const int va = kw + ord(2 * t), vb = kw + ord(2 * t + 1);
-    const uint32_t codes0 = smem_u32(s_codes), scale0 = smem_u32(s_scale);
     const uint32_t k_off = at(key0, t);                                             // chunks t and (D = 128) t + 4: ^ 64
     const uint32_t v_off_a = TILE + (D == 128 ? at(va, g) : at(va, g >> 1) + (g & 1) * 8);
     const uint32_t v_off_b = TILE + (D == 128 ? at(vb, g) : at(vb, g >> 1) + (g & 1) * 8);
 
-    uint32_t n = 0;   // running unit of this CTA
+    uint32_t n = 0, nv = 0;   // running counts of this team: units, visits
     if (any) do {
+      int first, step;
+      if (!wk.template mine<TEAMS>(team, first, step)) continue;
       const int hk = wk.head / p.head_blocks, hb = wk.head - hk * p.head_blocks;
       const int h0 = hk * p.G + hb * HEADS, n_heads = min(HEADS, p.G - hb * HEADS);
       // queries of this item as B fragments: thread (g, t) holds head g (+ 8), the channels of chunks t (and t + 4)
       uint32_t qf[NT][KSTEPS][2];
       float qs[NT][2];   // scale * log2(e) / power of two of heads 2t and 2t + 1
+      const uint32_t slot = nv % QSLOTS;
+      mbar_wait(&q_full[team][slot], (nv / QSLOTS) & 1, abortp, p.err, CS_ERR_TIMEOUT_TMA);
+      ++nv;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const int h = nt * 8 + g;
         uint32_t raw[KSTEPS * 2];
-        const __nv_bfloat16* src = p.q + wk.seq * p.q_tok + (h0 + h) * p.q_head + t * 16;
+        const uint32_t src = smem_u32(s_q + (team * QSLOTS + slot) * Shape::Q) + (h * D + t * 16) * 2;
 #pragma unroll
         for (int c = 0; c < KSTEPS / 4; ++c)
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            const uint4 v = h < n_heads ? *reinterpret_cast<const uint4*>(src + c * 64 + half * 8) : make_uint4(0, 0, 0, 0);
+            const uint4 v = h < n_heads ? lds128(src + c * 128 + half * 16) : make_uint4(0, 0, 0, 0);
             raw[c * 8 + half * 4] = v.x; raw[c * 8 + half * 4 + 1] = v.y;
             raw[c * 8 + half * 4 + 2] = v.z; raw[c * 8 + half * 4 + 3] = v.w;
           }
@@ -309,6 +371,7 @@ attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm, const DecPar
         qs[nt][0] = __shfl_sync(0xffffffffu, down, t * 8);
         qs[nt][1] = __shfl_sync(0xffffffffu, down, t * 8 + 4);
       }
+      if (lane == 0) mbar_arrive(&q_empty[team][slot]);
       float o[NT][MT][4], m[NT][2], l[NT][2];   // m: the reference exponent is m - 6, so weights reach up to 2^14
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -318,85 +381,100 @@ attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm, const DecPar
         for (int i = 0; i < MT; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
       }
 
-      for (int u = wk.u; u < wk.u + wk.n; ++u, ++n) {
-        if ((n & 1) != team) continue;
-        const uint32_t s = n % STAGES;
-        mbar_wait(&full[s], (n / STAGES) & 1, abortp, p.err, CS_ERR_TIMEOUT_TMA);
-        const int valid = wk.len - u * UNIT;   // keys of the unit that exist (may exceed 64)
+      for (int u = first; u < wk.u + wk.n; u += step, ++n) {
+        const uint32_t s = n % RING;
+        const uint32_t codes = smem_u32(s_codes + (team * RING + s) * 2 * TILE);
+        const uint32_t scale = smem_u32(s_scale + (team * RING + s) * 2 * UNIT * 4);
+        mbar_wait(&full[team][s], (n / RING) & 1, abortp, p.err, CS_ERR_TIMEOUT_TMA);
+        const int valid = wk.len - u * UNIT;   // keys of the unit that exist (may exceed UNIT)
         if (kw < valid) {
-          const uint32_t codes = codes0 + s * 2 * TILE, scale = scale0 + s * 2 * UNIT * 4;
-          // ---- S^T = K Q^T for 16 keys
-          uint32_t k0[KSTEPS], k1[KSTEPS];   // codes of keys key0 and key0 + 8, four channels per word
+          // ---- S^T = K Q^T for KT tiles of 16 keys; two chains of products per tile
+          float c[KT][NT][4], ks[KT][2], lv[KT][2];
 #pragma unroll
-          for (int c = 0; c < KSTEPS / 4; ++c) {
-            const uint4 x = lds128(codes + (k_off ^ (c * 64))), y = lds128(codes + (k_off ^ (c * 64)) + 8 * D);
-            k0[c * 4] = x.x; k0[c * 4 + 1] = x.y; k0[c * 4 + 2] = x.z; k0[c * 4 + 3] = x.w;
-            k1[c * 4] = y.x; k1[c * 4 + 1] = y.y; k1[c * 4 + 2] = y.z; k1[c * 4 + 3] = y.w;
-          }
-          const float ks0 = lds32(scale + key0 * 4), ks1 = lds32(scale + (key0 + 8) * 4);
-          const float vs0 = lds32(scale + (UNIT + key0) * 4), vs1 = lds32(scale + (UNIT + key0 + 8) * 4);
-          float c[NT][4];
+          for (int kt = 0; kt < KT; ++kt) {
+            uint32_t k0[KSTEPS], k1[KSTEPS];   // codes of keys key0 and key0 + 8, four channels per word
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.f;
-#pragma unroll
-          for (int i = 0; i < KSTEPS; ++i) {
-            const uint32_t a0 = e4m3x2_to_half2(k0[i]), a1 = e4m3x2_to_half2(k1[i]);
-            const uint32_t a2 = e4m3x2_to_half2(k0[i] >> 16), a3 = e4m3x2_to_half2(k1[i] >> 16);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma16816(c[nt], a0, a1, a2, a3, qf[nt][i][0], qf[nt][i][1]);
-          }
-          // the value rows of this thread: keys va, vb and those 8 further
-          uint32_t x[4][VPER / 4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const uint32_t addr = codes + ((r & 1) ? v_off_b : v_off_a) + (r >> 1) * 8 * D;
-            if constexpr (D == 128) {
-              const uint4 v = lds128(addr);
-              x[r][0] = v.x; x[r][1] = v.y; x[r][2] = v.z; x[r][3] = v.w;
-            } else {
-              const uint2 v = lds64(addr);
-              x[r][0] = v.x; x[r][1] = v.y;
+            for (int i = 0; i < KSTEPS / 4; ++i) {
+              const uint32_t addr = codes + (k_off ^ (i * 64)) + kt * 16 * D;
+              const uint4 x = lds128(addr), y = lds128(addr + 8 * D);
+              k0[i * 4] = x.x; k0[i * 4 + 1] = x.y; k0[i * 4 + 2] = x.z; k0[i * 4 + 3] = x.w;
+              k1[i * 4] = y.x; k1[i * 4 + 1] = y.y; k1[i * 4 + 2] = y.z; k1[i * 4 + 3] = y.w;
             }
-          }
-          const float lv0 = vs0 < 1.2e-38f ? -126.f : __log2f(vs0), lv1 = vs1 < 1.2e-38f ? -126.f : __log2f(vs1);
-          float tt[NT][4];
+            const uint32_t sc = scale + (key0 + kt * 16) * 4;
+            ks[kt][0] = lds32(sc); ks[kt][1] = lds32(sc + 32);
+            lv[kt][0] = lds32(sc + UNIT * 4); lv[kt][1] = lds32(sc + UNIT * 4 + 32);
+            float c2[NT][4];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            c[nt][0] *= ks0 * qs[nt][0]; c[nt][1] *= ks0 * qs[nt][1];
-            c[nt][2] *= ks1 * qs[nt][0]; c[nt][3] *= ks1 * qs[nt][1];
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) c[kt][nt][j] = c2[nt][j] = 0.f;
+#pragma unroll
+            for (int i = 0; i < KSTEPS; ++i) {
+              uint32_t a0, a1, a2, a3;
+              e4m3x4_to_half2x2(k0[i], a0, a2);
+              e4m3x4_to_half2x2(k1[i], a1, a3);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma16816((i & 1) ? c2[nt] : c[kt][nt], a0, a1, a2, a3, qf[nt][i][0], qf[nt][i][1]);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) c[kt][nt][j] = (c[kt][nt][j] + c2[nt][j]) * (ks[kt][j >> 1] * qs[nt][j & 1]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) lv[kt][j] = lv[kt][j] < 1.2e-38f ? -126.f : __log2f(lv[kt][j]);
           }
+          // the value rows of this thread: keys va, vb and those 8 further, per tile
+          uint32_t x[KT][4][VPER / 4];
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const uint32_t addr = codes + ((r & 1) ? v_off_b : v_off_a) + (kt * 16 + (r >> 1) * 8) * D;
+              if constexpr (D == 128) {
+                const uint4 v = lds128(addr);
+                x[kt][r][0] = v.x; x[kt][r][1] = v.y; x[kt][r][2] = v.z; x[kt][r][3] = v.w;
+              } else {
+                const uint2 v = lds64(addr);
+                x[kt][r][0] = v.x; x[kt][r][1] = v.y;
+              }
+            }
           if (valid < UNIT) {   // the sequence ends in this unit: what lies behind it may be anything
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              if (key0 >= valid) c[nt][0] = c[nt][1] = -INFINITY;
-              if (key0 + 8 >= valid) c[nt][2] = c[nt][3] = -INFINITY;
+            for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+                if (key0 + kt * 16 + j * 8 >= valid) {
+                  lv[kt][j] = 0.f;
+#pragma unroll
+                  for (int nt = 0; nt < NT; ++nt) c[kt][nt][2 * j] = c[kt][nt][2 * j + 1] = -INFINITY;
+                }
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (((r & 1) ? vb : va) + kt * 16 + (r >> 1) * 8 >= valid) {
+#pragma unroll
+                  for (int j = 0; j < VPER / 4; ++j) x[kt][r][j] = 0u;
+                }
             }
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (((r & 1) ? vb : va) + (r >> 1) * 8 >= valid) {
-#pragma unroll
-                for (int j = 0; j < VPER / 4; ++j) x[r][j] = 0u;
-              }
           }
-          const float w0 = key0 < valid ? lv0 : 0.f, w1 = key0 + 8 < valid ? lv1 : 0.f;
           bool grow = false;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            tt[nt][0] = c[nt][0] + w0; tt[nt][1] = c[nt][1] + w0;
-            tt[nt][2] = c[nt][2] + w1; tt[nt][3] = c[nt][3] + w1;
-            grow |= fmaxf(tt[nt][0], tt[nt][2]) > m[nt][0] + 8.f || fmaxf(tt[nt][1], tt[nt][3]) > m[nt][1] + 8.f;
-          }
+          for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) grow |= c[kt][nt][j] + lv[kt][j >> 1] > m[nt][j & 1] + 8.f;
           // The reference moves only when a weight would pass 2^14, which after the first tiles is rare
           if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int j = 0; j < 2; ++j) {
-                float mx = fmaxf(tt[nt][j], tt[nt][2 + j]);
+                float mx = m[nt][j];
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) mx = fmaxf(mx, fmaxf(c[kt][nt][j] + lv[kt][0], c[kt][nt][2 + j] + lv[kt][1]));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                mx = fmaxf(mx, m[nt][j]);
                 const float alpha = ex2(m[nt][j] - mx);
                 m[nt][j] = mx;
                 l[nt][j] *= alpha;
@@ -404,31 +482,39 @@ attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm, const DecPar
                 for (int i = 0; i < MT; ++i) { o[nt][i][j] *= alpha; o[nt][i][2 + j] *= alpha; }
               }
           }
-          uint32_t b0[NT], b1[NT];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const float r0_ = m[nt][0] - 6.f, r1_ = m[nt][1] - 6.f;
-            l[nt][0] += ex2(c[nt][0] - r0_) + ex2(c[nt][2] - r0_);
-            l[nt][1] += ex2(c[nt][1] - r1_) + ex2(c[nt][3] - r1_);
-            b0[nt] = transpose8x8(pack_half2(ex2(tt[nt][0] - r0_), ex2(tt[nt][1] - r1_)));
-            b1[nt] = transpose8x8(pack_half2(ex2(tt[nt][2] - r0_), ex2(tt[nt][3] - r1_)));
-          }
-          // ---- O^T += V^T P: fragment row g of tile i is channel VPER g + 2 i, row g + 8 the next one
+          for (int kt = 0; kt < KT; ++kt) {
+            uint32_t b0[NT], b1[NT];
 #pragma unroll
-          for (int i = 0; i < MT; ++i) {
-            const uint32_t sel = (i & 1) ? 0x7362u : 0x5140u;
-            const uint32_t ab = __byte_perm(x[0][i >> 1], x[1][i >> 1], sel), cd = __byte_perm(x[2][i >> 1], x[3][i >> 1], sel);
-            const uint32_t a0 = e4m3x2_to_half2(ab), a1 = e4m3x2_to_half2(ab >> 16);
-            const uint32_t a2 = e4m3x2_to_half2(cd), a3 = e4m3x2_to_half2(cd >> 16);
+            for (int nt = 0; nt < NT; ++nt) {
+              float w[4];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][i], a0, a1, a2, a3, b0[nt], b1[nt]);
+              for (int j = 0; j < 4; ++j) {
+                const float e = c[kt][nt][j] - (m[nt][j & 1] - 6.f);
+                l[nt][j & 1] += ex2(e);
+                w[j] = ex2(e + lv[kt][j >> 1]);
+              }
+              b0[nt] = transpose8x8(pack_half2(w[0], w[1]));
+              b1[nt] = transpose8x8(pack_half2(w[2], w[3]));
+            }
+            // ---- O^T += V^T P: fragment row g of tile i is channel VPER g + 2 i, row g + 8 the next one
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              const uint32_t sel = (i & 1) ? 0x7362u : 0x5140u;
+              uint32_t a0, a1, a2, a3;
+              e4m3x4_to_half2x2(__byte_perm(x[kt][0][i >> 1], x[kt][1][i >> 1], sel), a0, a1);
+              e4m3x4_to_half2x2(__byte_perm(x[kt][2][i >> 1], x[kt][3][i >> 1], sel), a2, a3);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][i], a0, a1, a2, a3, b0[nt], b1[nt]);
+            }
           }
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[s]);
+        if (lane == 0) mbar_arrive(&empty[team][s]);
       }
 
-      // ---- the warps' sums meet: [warp][head][channel] in shared memory, then warp w finishes head w (and w + 8)
+      // ---- the warps' sums meet in shared memory, [warp][head][channel]; then every warp finishes some heads
+      const bool shared = wk.shared();
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -443,45 +529,36 @@ attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm, const DecPar
           for (int i = 0; i < MT; i += 2)
             *reinterpret_cast<float4*>(dst + 2 * i) = make_float4(o[nt][i][j], o[nt][i][2 + j], o[nt][i + 1][j], o[nt][i + 1][2 + j]);
         }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
+      auto meet = [&]() {
+        if (shared) asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory");
+        else asm volatile("bar.sync %0, 128;" ::"r"(2 + team) : "memory");
+      };
+      meet();
       const bool whole = wk.u == 0 && wk.n == wk.units;
-      const int slot = blockIdx.x * 2 + (wk.u == 0 ? 1 : 0);   // an item that began before the run is its first, one that goes on its last
-      const long long part = static_cast<long long>(slot) * HEADS;
-      if (!whole && threadIdx.x == 0) p.ws_item[slot] = wk.seq * heads + wk.head;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const int h = nt * 8 + warp;
-        if (h < n_heads) {
-          float mx = M_NONE, sum = 0.f, f[CONSUMERS];
-#pragma unroll
-          for (int w = 0; w < CONSUMERS; ++w) mx = fmaxf(mx, s_m[w][h]);
-#pragma unroll
-          for (int w = 0; w < CONSUMERS; ++w) { f[w] = ex2(s_m[w][h] - mx); sum += s_l[w][h] * f[w]; }
+      const int out_slot = blockIdx.x * 2 + (wk.u == 0 ? 1 : 0);   // an item that began before the run is its first, one that goes on its last
+      const long long part = static_cast<long long>(out_slot) * HEADS;
+      const int w0 = shared ? 0 : team * 4, w1 = shared ? WARPS : team * 4 + 4;   // the warps that took part
+      if (!whole && warp == w0 && lane == 0) p.ws_item[out_slot] = wk.seq * heads + wk.head;
+      for (int h = warp - w0; h < n_heads; h += w1 - w0) {
+        float mx = M_NONE, sum = 0.f;
+        for (int w = w0; w < w1; ++w) mx = fmaxf(mx, s_m[w][h]);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int w = w0; w < w1; ++w) {
+          const float f = ex2(s_m[w][h] - mx);
+          sum += s_l[w][h] * f;
           if (lane * 4 < D) {
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < CONSUMERS; ++w) {
-              const float4 v = *reinterpret_cast<const float4*>(s_join + (w * HEADS + h) * JOIN_LD + lane * 4);
-              acc.x += v.x * f[w]; acc.y += v.y * f[w]; acc.z += v.z * f[w]; acc.w += v.w * f[w];
-            }
-            if (whole) {
-              const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-              __nv_bfloat16* dst = p.o + wk.seq * p.o_tok + (h0 + h) * p.o_head + lane * 4;
-              const uint2 v = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
-              if (p.o_vec) {
-                *reinterpret_cast<uint2*>(dst) = v;
-              } else {
-                unsigned short* d16 = reinterpret_cast<unsigned short*>(dst);
-                d16[0] = v.x & 0xffffu; d16[1] = v.x >> 16; d16[2] = v.y & 0xffffu; d16[3] = v.y >> 16;
-              }
-            } else {
-              *reinterpret_cast<float4*>(p.ws_o + (part + h) * D + lane * 4) = acc;
-            }
+            const float4 v = *reinterpret_cast<const float4*>(s_join + (w * HEADS + h) * JOIN_LD + lane * 4);
+            acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
           }
-          if (!whole && lane == 0) { p.ws_ml[(part + h) * 2] = mx; p.ws_ml[(part + h) * 2 + 1] = sum; }
         }
+        if (lane * 4 < D) {
+          if (whole) store_head(p, wk.seq, h0 + h, lane, acc, sum);
+          else *reinterpret_cast<float4*>(p.ws_o + (part + h) * D + lane * 4) = acc;
+        }
+        if (!whole && lane == 0) { p.ws_ml[(part + h) * 2] = mx; p.ws_ml[(part + h) * 2 + 1] = sum; }
       }
-      asm volatile("bar.sync 1, 256;" ::: "memory");   // the join area is written again at the end of the next item
+      meet();   // the join area is written again at the end of the next visit
     } while (wk.next(p));
 
     // sequences without keys give zeros; lengths that do not fit the table are reported
@@ -489,7 +566,7 @@ attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm, const DecPar
       const int len = p.kv_len[b];
       if (len > static_cast<long long>(p.bt_width) * KV8_PAGE && threadIdx.x == 0) cs_set_error(p.err, CS_ERR_BAD_ARG);
       if (dec_len(p, b) == 0)
-        for (int i = threadIdx.x; i < p.Hq * D; i += CONSUMERS * 32) p.o[b * p.o_tok + (i / D) * p.o_head + i % D] = __float2bfloat16(0.f);
+        for (int i = threadIdx.x; i < p.Hq * D; i += WARPS * 32) p.o[b * p.o_tok + (i / D) * p.o_head + i % D] = __float2bfloat16(0.f);
     }
   }
 }
@@ -540,20 +617,11 @@ __global__ void __launch_bounds__(256 * NT) attention_decode_fp8_join_kernel(con
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane * 4 >= D) return;
-  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-  __nv_bfloat16* dst = p.o + seq * p.o_tok + (hk * p.G + hb * HEADS + h) * p.o_head + lane * 4;
-  const uint2 v = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
-  if (p.o_vec) {
-    *reinterpret_cast<uint2*>(dst) = v;
-  } else {
-    unsigned short* d16 = reinterpret_cast<unsigned short*>(dst);
-    d16[0] = v.x & 0xffffu; d16[1] = v.x >> 16; d16[2] = v.y & 0xffffu; d16[3] = v.y >> 16;
-  }
+  if (lane * 4 < D) store_head(p, seq, hk * p.G + hb * HEADS + h, lane, acc, sum);
 }
 
 template <int D, int NT>
-int launch_decode(const CUtensorMap& tm, const DecParams& p, int ctas, cudaStream_t stream) {
+int launch_decode(const void* cache, DecParams& p, int ctas, cudaStream_t stream) {
   using Shape = DecShape<D, NT>;
   static bool attr_done[64] = {false};
   int dev = 0;
@@ -563,7 +631,21 @@ int launch_decode(const CUtensorMap& tm, const DecParams& p, int ctas, cudaStrea
       return -10;
     attr_done[dev] = true;
   }
-  if (cs_launch_pdl(attention_decode_fp8_kernel<D, NT>, dim3(ctas), dim3(DEC_THREADS), Shape::SMEM, stream, tm, p) != cudaSuccess) return -10;
+  // no more CTAs than units that the tables could hold
+  const long long most = static_cast<long long>(p.B) * p.Hkv * p.head_blocks * p.bt_width * (KV8_PAGE / Shape::UNIT);
+  if (most < ctas) ctas = most > 0 ? static_cast<int>(most) : 1;
+  // one box = the K and V codes (or scales) of one unit of one head and page
+  CUtensorMap tm_codes, tm_scales;
+  const uint64_t blk = kv8_block_bytes(D), pages = p.num_pages, hkv = p.Hkv;
+  const uint64_t dims[5] = {D, KV8_PAGE, hkv, 2, pages}, strides[4] = {D, blk, hkv * blk, 2 * hkv * blk};
+  const uint32_t box[5] = {D, Shape::UNIT, 1, 2, 1};
+  const uint64_t sdims[4] = {KV8_PAGE, hkv, 2, pages}, sstrides[3] = {blk, hkv * blk, 2 * hkv * blk};
+  const uint32_t sbox[4] = {Shape::UNIT, 1, 2, 1};
+  if (cs_encode_tmap_nd(&tm_codes, 1, 5, cache, dims, strides, box, D)) return -3;
+  if (cs_encode_tmap_nd(&tm_scales, 4, 4, static_cast<const uint8_t*>(cache) + KV8_PAGE * D, sdims, sstrides, sbox, 0)) return -3;
+  if (cs_launch_pdl(attention_decode_fp8_kernel<D, NT>, dim3(ctas), dim3(Shape::THREADS), Shape::SMEM, stream, tm_codes, tm_scales, p) !=
+      cudaSuccess)
+    return -10;
   return cs_launch_pdl(attention_decode_fp8_join_kernel<D, NT>, dim3(ctas), dim3(256 * NT), 0, stream, p) == cudaSuccess ? 0 : -10;
 }
 
@@ -577,19 +659,20 @@ CS_API long long cs_attention_decode_fp8_ws_bytes(int Hq, int Hkv, int d) {
   return ctas * 2 * (heads * (d + 2LL) * 4 + 4);
 }
 
-// q, o: [B, Hq, d] with token and head strides in elements; q rows lie on 16-byte boundaries.  One query per sequence,
-// which sees all kv_len[b] keys.  ws: cs_attention_decode_fp8_ws_bytes of scratch that no call on another stream uses.
-CS_API int cs_attention_decode_fp8(const void* q, long long q_tok, long long q_head, const void* cache, long long num_pages, void* o,
-                                   long long o_tok, long long o_head, const void* kv_len, const void* block_table, long long bt_stride,
-                                   int bt_width, int B, int Hq, int Hkv, int d, float scale, void* ws, long long ws_bytes, void* stream) {
+// q: [B, Hq, d] with contiguous heads, tokens q_tok elements apart and on 16-byte boundaries; o: [B, Hq, d] with token and
+// head strides in elements.  One query per sequence, which sees all kv_len[b] keys.  ws: cs_attention_decode_fp8_ws_bytes
+// of scratch that no call on another stream uses.
+CS_API int cs_attention_decode_fp8(const void* q, long long q_tok, const void* cache, long long num_pages, void* o, long long o_tok,
+                                   long long o_head, const void* kv_len, const void* block_table, long long bt_stride, int bt_width, int B,
+                                   int Hq, int Hkv, int d, float scale, void* ws, long long ws_bytes, void* stream) {
   if (B <= 0) return 0;
-  if ((d != 64 && d != 128) || Hkv <= 0 || Hq <= 0 || Hq % Hkv != 0 || num_pages <= 0 || num_pages * 2 * Hkv > 0x7fffffffLL) return -1;
-  if ((reinterpret_cast<uintptr_t>(q) & 15) || (q_tok & 7) || (q_head & 7)) return -1;
+  if ((d != 64 && d != 128) || Hkv <= 0 || Hq <= 0 || Hq % Hkv != 0 || num_pages <= 0 || num_pages > 0x7fffffffLL) return -1;
+  if ((reinterpret_cast<uintptr_t>(q) & 15) || (q_tok & 7)) return -1;
   DecParams p{};
-  p.q = (const __nv_bfloat16*)q; p.q_tok = q_tok; p.q_head = q_head;
+  p.q = (const __nv_bfloat16*)q; p.q_tok = q_tok;
   p.o = (__nv_bfloat16*)o; p.o_tok = o_tok; p.o_head = o_head;
   p.o_vec = (reinterpret_cast<uintptr_t>(o) & 7) == 0 && (o_tok & 3) == 0 && (o_head & 3) == 0;
-  p.cache = (const uint8_t*)cache; p.num_pages = static_cast<int>(num_pages);
+  p.num_pages = static_cast<int>(num_pages);
   p.block_table = (const int*)block_table; p.bt_stride = bt_stride; p.bt_width = bt_width;
   p.kv_len = (const int*)kv_len;
   p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv;
@@ -599,16 +682,11 @@ CS_API int cs_attention_decode_fp8(const void* q, long long q_tok, long long q_h
   p.scale_log2 = scale * 1.4426950408889634f;
   p.err = cs_error_word();
   if (ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 15) || ws_bytes < cs_attention_decode_fp8_ws_bytes(Hq, Hkv, d)) return -5;
-  int ctas = cs_num_sms() < MAX_CTAS ? cs_num_sms() : MAX_CTAS;
+  const int ctas = cs_num_sms() < MAX_CTAS ? cs_num_sms() : MAX_CTAS;
   p.ws_o = reinterpret_cast<float*>(ws);
   p.ws_ml = p.ws_o + static_cast<long long>(ctas) * 2 * heads * d;
   p.ws_item = reinterpret_cast<int*>(p.ws_ml + static_cast<long long>(ctas) * 2 * heads * 2);
-  // no more CTAs than units that the tables could hold
-  const long long most = static_cast<long long>(B) * Hkv * p.head_blocks * bt_width * (KV8_PAGE / UNIT);
-  if (most < ctas) ctas = most > 0 ? static_cast<int>(most) : 1;
-  CUtensorMap tm;
-  if (cs_encode_tmap_3d_u8(&tm, cache, d, KV8_PAGE, static_cast<uint64_t>(num_pages) * 2 * Hkv, d, kv8_block_bytes(d), d, UNIT, 1, d)) return -3;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (d == 128) return heads == 8 ? launch_decode<128, 1>(tm, p, ctas, st) : launch_decode<128, 2>(tm, p, ctas, st);
-  return heads == 8 ? launch_decode<64, 1>(tm, p, ctas, st) : launch_decode<64, 2>(tm, p, ctas, st);
+  if (d == 128) return heads == 8 ? launch_decode<128, 1>(cache, p, ctas, st) : launch_decode<128, 2>(cache, p, ctas, st);
+  return heads == 8 ? launch_decode<64, 1>(cache, p, ctas, st) : launch_decode<64, 2>(cache, p, ctas, st);
 }

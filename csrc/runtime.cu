@@ -91,19 +91,25 @@ int cs_encode_tmap_3d(CUtensorMap* out, const void* base, uint64_t d0, uint64_t 
   return r == CUDA_SUCCESS ? 0 : -3;
 }
 
-// 3-D tiled byte map whose inner box is one swizzle span (64 or 128 bytes); strides of dims 1 and 2 in bytes.
-int cs_encode_tmap_3d_u8(CUtensorMap* out, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t s1_bytes,
-                         uint64_t s2_bytes, uint32_t b0, uint32_t b1, uint32_t b2, int swizzle_bytes) {
+// Tiled map of up to five dimensions over bytes or fp32: strides in bytes of dims 1 and up, swizzle of 128 or 64 bytes (the
+// inner box is then one such span) or 0 = none.
+int cs_encode_tmap_nd(CUtensorMap* out, int elem_bytes, int rank, const void* base, const uint64_t* dims, const uint64_t* strides,
+                      const uint32_t* box, int swizzle_bytes) {
   EncodeTiledFn enc = get_encode();
   if (!enc) return -1;
-  if ((reinterpret_cast<uintptr_t>(base) & 15) != 0 || (s1_bytes & 15) != 0 || (s2_bytes & 15) != 0) return -2;
-  cuuint64_t dims[3] = {d0, d1, d2};
-  cuuint64_t strides[2] = {s1_bytes, s2_bytes};
-  cuuint32_t box[3] = {b0, b1, b2};
-  cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
-                   CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (rank < 2 || rank > 5 || (elem_bytes != 1 && elem_bytes != 4) || (reinterpret_cast<uintptr_t>(base) & 15) != 0) return -2;
+  cuuint64_t d[5], s[4];
+  cuuint32_t b[5], estr[5] = {1, 1, 1, 1, 1};
+  for (int i = 0; i < rank; ++i) { d[i] = dims[i]; b[i] = box[i]; }
+  for (int i = 0; i + 1 < rank; ++i) {
+    if (strides[i] & 15) return -2;
+    s[i] = strides[i];
+  }
+  const CUtensorMapSwizzle sw = swizzle_bytes == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                                : swizzle_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                      : CU_TENSOR_MAP_SWIZZLE_NONE;
+  CUresult r = enc(out, elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, rank, const_cast<void*>(base),
+                   d, s, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : -3;
 }
 
