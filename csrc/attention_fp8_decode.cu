@@ -34,7 +34,7 @@ int cs_encode_tmap_nd(CUtensorMap* out, int elem_bytes, int rank, const void* ba
 namespace {
 
 constexpr int MAX_CTAS = 512;
-constexpr int SHARED_VISIT = 8;              // visits of at least this many units are shared by the teams of a CTA
+constexpr int SHARED_VISIT = 3;              // visits of at least this many units are shared by the teams of a CTA
 constexpr float M_NONE = -3.0e38f;           // running maximum before the first key (finite: differences stay defined)
 
 // One instantiation.  TEAMS: as many as registers allow (128 a thread with three teams, 168 with two).
@@ -132,10 +132,12 @@ __device__ __forceinline__ int dec_len(const DecParams& p, int b) {
   return n < 0 ? 0 : (n > cap ? static_cast<int>(cap) : n);
 }
 
+template <int N> struct Count { static constexpr int value = N; };
+
 // Four channels of one head: sums divided by the normaliser (0 when no key took part).
-__device__ __forceinline__ void store_head(const DecParams& p, int seq, int head, int lane, const float4& acc, float sum) {
+__device__ __forceinline__ void store_head(const DecParams& p, int seq, int head, int ch4, const float4& acc, float sum) {
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-  __nv_bfloat16* dst = p.o + seq * p.o_tok + head * p.o_head + lane * 4;
+  __nv_bfloat16* dst = p.o + seq * p.o_tok + head * p.o_head + ch4 * 4;
   const uint2 v = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
   if (p.o_vec) {
     *reinterpret_cast<uint2*>(dst) = v;
@@ -150,14 +152,14 @@ __device__ __forceinline__ void store_head(const DecParams& p, int seq, int head
 template <int UNIT>
 struct Walk {
   int seq, head, units, len, u, n;
-  long long left;   // units of the CTA's run not yet handed out, this visit included
+  int left;         // units of the CTA's run not yet handed out, this visit included
   uint32_t dealt;   // short visits and units of shared visits so far: deals the next ones to the teams in turn
   __device__ __forceinline__ bool settle(const DecParams& p) {   // on to a sequence with keys
     for (; seq < p.B; ++seq) {
       len = dec_len(p, seq);
       units = (len + UNIT - 1) / UNIT;
       if (u < units) {
-        n = static_cast<int>(min(static_cast<long long>(units - u), left));
+        n = min(units - u, left);
         return true;
       }
     }
@@ -170,7 +172,7 @@ struct Walk {
     if (left <= 0) return false;
     u = 0;
     if (++head == p.Hkv * p.head_blocks) { head = 0; ++seq; return settle(p); }
-    n = static_cast<int>(min(static_cast<long long>(units), left));
+    n = min(units, left);
     return true;
   }
   // the units of this visit that belong to `team`: first, first + step, ... below u + n
@@ -200,14 +202,12 @@ attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_codes, const 
   float* s_join = reinterpret_cast<float*>(s_q + TEAMS * QSLOTS * Shape::Q); // [warp][head][JOIN_LD]
   __shared__ uint64_t full[TEAMS][RING], empty[TEAMS][RING], q_full[TEAMS][QSLOTS], q_empty[TEAMS][QSLOTS];
   __shared__ float s_m[WARPS][HEADS], s_l[WARPS][HEADS];
-  __shared__ int abort_flag, s_start_seq;
-  __shared__ long long s_warp_sum[ALL_WARPS], s_start_off;
+  __shared__ int abort_flag, s_warp_sum[ALL_WARPS], s_start[2];   // s_start: sequence and unit (of all its heads) the run begins with
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     abort_flag = 0;
-    s_start_seq = 0;
-    s_start_off = 0;
+    s_start[0] = s_start[1] = 0;
     for (int w = 0; w < TEAMS; ++w) {
       for (int s = 0; s < RING; ++s) { mbar_init(&full[w][s], 1); mbar_init(&empty[w][s], 4); }
       for (int s = 0; s < QSLOTS; ++s) { mbar_init(&q_full[w][s], 1); mbar_init(&q_empty[w][s], 4); }
@@ -222,50 +222,47 @@ attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_codes, const 
   if (threadIdx.x == 0) p.ws_item[blockIdx.x * 2] = p.ws_item[blockIdx.x * 2 + 1] = -1;
 
   // ------------------------------- this CTA's run of units -------------------------------
-  const int heads = p.Hkv * p.head_blocks;
-  auto units_of = [&](int b) { return (dec_len(p, b) + UNIT - 1) / UNIT; };
-  long long mine = 0;
-  for (int b = threadIdx.x; b < p.B; b += THREADS) mine += units_of(b);
+  // Thread i counts the units of `per` consecutive sequences (one, unless the batch is huge); a scan over the threads
+  // gives the total and who owns the first unit of the run.  The host has checked that 32 bits hold every count.
+  const int heads = p.Hkv * p.head_blocks, per = (p.B + THREADS - 1) / THREADS;
+  auto units_of = [&](int b) { return b < p.B ? (dec_len(p, b) + UNIT - 1) / UNIT : 0; };
+  int mine = 0;
+  for (int i = 0; i < per; ++i) mine += units_of(threadIdx.x * per + i);
+  int incl = mine;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if (lane == 0) s_warp_sum[warp] = mine;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) s_warp_sum[warp] = incl;
   __syncthreads();
-  long long total = 0;
+  int total = 0;
 #pragma unroll
-  for (int w = 0; w < ALL_WARPS; ++w) total += s_warp_sum[w];
+  for (int w = 0; w < ALL_WARPS; ++w) {
+    if (w == warp) incl += total;
+    total += s_warp_sum[w];
+  }
   total *= heads;
   // no CTA of the first `active` is without a unit, so the CTAs that share an item are consecutive
-  const long long active = min(total, static_cast<long long>(gridDim.x));
-  long long r0 = 0, r1 = 0;
-  if (blockIdx.x < active) { r0 = total * blockIdx.x / active; r1 = total * (blockIdx.x + 1) / active; }
-  long long before = 0;   // units (all heads) of the sequences ahead of this chunk
-  for (int base = 0; base < p.B && r1 > r0; base += THREADS) {
-    __syncthreads();
-    const int b = base + threadIdx.x;
-    const long long units = b < p.B ? static_cast<long long>(units_of(b)) * heads : 0;
-    long long incl = units;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
-    }
-    if (lane == 31) s_warp_sum[warp] = incl;
-    __syncthreads();
-    for (int w = 0; w < warp; ++w) incl += s_warp_sum[w];
-    incl += before;
-    if (r0 < incl && r0 >= incl - units) { s_start_seq = b; s_start_off = r0 - (incl - units); }
-    for (int w = 0; w < ALL_WARPS; ++w) before += s_warp_sum[w];
-    if (before > r0) break;
+  const int active = max(1, min(total, static_cast<int>(gridDim.x))), c = blockIdx.x;
+  const int quota = total / active, extra = total - quota * active;
+  const int r0 = quota * c + min(c, extra), run = c < active ? quota + (c < extra ? 1 : 0) : 0;
+  int at0 = (incl - mine) * heads;
+  if (run > 0 && r0 >= at0 && r0 < incl * heads) {
+    int b = static_cast<int>(threadIdx.x) * per;
+    for (int u; b < (static_cast<int>(threadIdx.x) + 1) * per - 1 && r0 >= at0 + (u = units_of(b) * heads); ++b) at0 += u;
+    s_start[0] = b;
+    s_start[1] = r0 - at0;
   }
   __syncthreads();
   volatile int* abortp = &abort_flag;
   Walk<UNIT> wk{};
-  wk.seq = s_start_seq;
-  wk.left = r1 - r0;
+  wk.seq = s_start[0];
+  wk.left = run;
   const int start_units = max(1, units_of(wk.seq));
-  wk.head = static_cast<int>(s_start_off / start_units);
-  wk.u = static_cast<int>(s_start_off - static_cast<long long>(wk.head) * start_units);
-  const bool any = r1 > r0 && wk.settle(p);
+  wk.head = s_start[1] / start_units;
+  wk.u = s_start[1] - wk.head * start_units;
+  const bool any = run > 0 && wk.settle(p);
 
   if (warp >= WARPS) {
     // ------------------------------- producer of one team -------------------------------
@@ -276,9 +273,13 @@ attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_codes, const 
       int first, step;
       if (!wk.template mine<TEAMS>(team, first, step)) continue;
       const int hk = wk.head / p.head_blocks, hb = wk.head - hk * p.head_blocks;
+      const int* table = p.block_table + wk.seq * p.bt_stride;
+      const int blocks = (wk.len + KV8_PAGE - 1) / KV8_PAGE;
+      int page_base = first / (KV8_PAGE / UNIT);    // the 32 table entries held by the lanes start at page_base
+      int page_lane = page_base + lane < blocks ? table[page_base + lane] : 0;
       if (lane == 0) {
         const uint32_t slot = nv % QSLOTS;
-        ok = mbar_wait(&q_empty[team][slot], ((nv / QSLOTS) & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
+        ok = ok && mbar_wait(&q_empty[team][slot], ((nv / QSLOTS) & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
         if (ok) {
           const uint32_t bytes = min(HEADS, p.G - hb * HEADS) * D * 2;
           mbar_arrive_expect_tx(&q_full[team][slot], bytes);
@@ -287,13 +288,11 @@ attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_codes, const 
         }
       }
       ++nv;
-      const int* table = p.block_table + wk.seq * p.bt_stride;
-      int page_lane = 0, page_base = -64;   // the 32 table entries held by the lanes start at page_base
       for (int u = first; u < wk.u + wk.n; u += step, ++n) {
         const int blk = u / (KV8_PAGE / UNIT), part = u % (KV8_PAGE / UNIT);
-        if (blk >= page_base + 32 || page_base < 0) {
+        if (blk >= page_base + 32) {
           page_base = blk;
-          page_lane = blk + lane < (wk.len + KV8_PAGE - 1) / KV8_PAGE ? table[blk + lane] : 0;
+          page_lane = blk + lane < blocks ? table[blk + lane] : 0;
         }
         int page = __shfl_sync(0xffffffffu, page_lane, blk - page_base);
         if (lane == 0 && ok) {
@@ -535,29 +534,35 @@ attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_codes, const 
       };
       meet();
       const bool whole = wk.u == 0 && wk.n == wk.units;
-      const int out_slot = blockIdx.x * 2 + (wk.u == 0 ? 1 : 0);   // an item that began before the run is its first, one that goes on its last
-      const long long part = static_cast<long long>(out_slot) * HEADS;
-      const int w0 = shared ? 0 : team * 4, w1 = shared ? WARPS : team * 4 + 4;   // the warps that took part
-      if (!whole && warp == w0 && lane == 0) p.ws_item[out_slot] = wk.seq * heads + wk.head;
-      for (int h = warp - w0; h < n_heads; h += w1 - w0) {
-        float mx = M_NONE, sum = 0.f;
-        for (int w = w0; w < w1; ++w) mx = fmaxf(mx, s_m[w][h]);
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int w = w0; w < w1; ++w) {
-          const float f = ex2(s_m[w][h] - mx);
-          sum += s_l[w][h] * f;
-          if (lane * 4 < D) {
-            const float4 v = *reinterpret_cast<const float4*>(s_join + (w * HEADS + h) * JOIN_LD + lane * 4);
-            acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+      const int out_slot = c * 2 + (wk.u == 0 ? 1 : 0);   // an item that began before the run is its first, one that goes on its last
+      auto finish = [&](auto count, int w0) {             // `count` warps from w0 on took part and share the outputs
+        constexpr int W = decltype(count)::value;
+        const int part = out_slot * HEADS;
+        if (!whole && warp == w0 && lane == 0) p.ws_item[out_slot] = wk.seq * heads + wk.head;
+#pragma unroll
+        for (int i = 0; i < (HEADS * D / 4 + W * 32 - 1) / (W * 32); ++i) {
+          const int idx = (warp - w0 + i * W) * 32 + lane, h = idx / (D / 4), ch = idx % (D / 4);
+          if (h >= n_heads) continue;
+          float f[W], mx = M_NONE, sum = 0.f;
+#pragma unroll
+          for (int w = 0; w < W; ++w) { f[w] = s_m[w0 + w][h]; mx = fmaxf(mx, f[w]); }
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int w = 0; w < W; ++w) {
+            const float e = ex2(f[w] - mx);
+            sum += s_l[w0 + w][h] * e;
+            const float4 v = *reinterpret_cast<const float4*>(s_join + ((w0 + w) * HEADS + h) * JOIN_LD + ch * 4);
+            acc.x += v.x * e; acc.y += v.y * e; acc.z += v.z * e; acc.w += v.w * e;
+          }
+          if (whole) {
+            store_head(p, wk.seq, h0 + h, ch, acc, sum);
+          } else {
+            *reinterpret_cast<float4*>(p.ws_o + (part + h) * D + ch * 4) = acc;
+            if (ch == 0) { p.ws_ml[(part + h) * 2] = mx; p.ws_ml[(part + h) * 2 + 1] = sum; }
           }
         }
-        if (lane * 4 < D) {
-          if (whole) store_head(p, wk.seq, h0 + h, lane, acc, sum);
-          else *reinterpret_cast<float4*>(p.ws_o + (part + h) * D + lane * 4) = acc;
-        }
-        if (!whole && lane == 0) { p.ws_ml[(part + h) * 2] = mx; p.ws_ml[(part + h) * 2 + 1] = sum; }
-      }
+      };
+      if (shared) finish(Count<WARPS>{}, 0); else finish(Count<4>{}, team * 4);
       meet();   // the join area is written again at the end of the next visit
     } while (wk.next(p));
 
@@ -571,53 +576,55 @@ attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_codes, const 
   }
 }
 
-// Joins the items that several CTAs worked on: CTA c takes the item whose first part is the last of decode CTA c.  One
-// warp per head; the parts are read in the order of the CTAs.
+// Joins the items that several CTAs worked on: block (c, h) takes head h of the item whose first part is the last of
+// decode CTA c.  Its parts are slot 1 of CTA c and slot 0 of the CTAs behind it; warp w reads parts w, w + 4, ...
 template <int D, int NT>
-__global__ void __launch_bounds__(256 * NT) attention_decode_fp8_join_kernel(const DecParams p) {
+__global__ void __launch_bounds__(128) attention_decode_fp8_join_kernel(const DecParams p, int ctas) {
   constexpr int HEADS = 8 * NT;
+  __shared__ float s_acc[4][D], s_ml[4][2];
   pdl_wait();
   pdl_launch_dependents();
-  const int item = p.ws_item[blockIdx.x * 2 + 1];
+  const int c = blockIdx.x, h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int item = p.ws_item[c * 2 + 1];
+  int behind = c + 1 + threadIdx.x < ctas ? p.ws_item[(c + 1 + threadIdx.x) * 2] : -1;
   if (item < 0) return;
-  const int h = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int heads = p.Hkv * p.head_blocks, seq = item / heads, head = item - seq * heads;
   const int hk = head / p.head_blocks, hb = head - hk * p.head_blocks;
-  if (h >= min(HEADS, p.G - hb * HEADS)) return;
-  int end = blockIdx.x + 1;   // the parts are slot 1 of this CTA and slot 0 of those up to `end`
-  while (end < gridDim.x) {
-    const int c = end + lane;
-    const unsigned same = __ballot_sync(0xffffffffu, c < gridDim.x && p.ws_item[c * 2] == item);
-    end += __popc(same);     // the CTAs of an item are consecutive
-    if (same != 0xffffffffu) break;
+  if (hb * HEADS + h >= p.G) return;
+  int parts = 1 + __syncthreads_count(behind == item);
+  for (int first = c + 129; parts % 128 == 1 && parts > 1 && first < ctas; first += 128) {   // more than 128 CTAs on one item
+    behind = first + threadIdx.x < ctas ? p.ws_item[(first + threadIdx.x) * 2] : -1;
+    const int more = __syncthreads_count(behind == item);
+    parts += more;
+    if (more < 128) break;
   }
-  auto part = [&](int c) { return (static_cast<long long>(c) * 2 + (c == blockIdx.x ? 1 : 0)) * HEADS + h; };
-  float mx = M_NONE;
-  for (int c = blockIdx.x + lane; c < end; c += 32) mx = fmaxf(mx, p.ws_ml[part(c) * 2]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  float sum = 0.f;
+  float m = M_NONE, l = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int c0 = blockIdx.x; c0 < end; c0 += 32) {
-    const int c = c0 + lane;
-    float f = 0.f;
-    if (c < end) {
-      f = ex2(p.ws_ml[part(c) * 2] - mx);
-      sum += p.ws_ml[part(c) * 2 + 1] * f;
-    }
-    const int cnt = min(32, end - c0);
-#pragma unroll 8
-    for (int i = 0; i < cnt; ++i) {
-      const float fi = __shfl_sync(0xffffffffu, f, i);
-      if (lane * 4 < D) {
-        const float4 v = *reinterpret_cast<const float4*>(p.ws_o + part(c0 + i) * D + lane * 4);
-        acc.x += v.x * fi; acc.y += v.y * fi; acc.z += v.z * fi; acc.w += v.w * fi;
-      }
-    }
+#pragma unroll 4
+  for (int i = warp; i < parts; i += 4) {
+    const long long row = ((c + i) * 2 + (i == 0 ? 1 : 0)) * HEADS + h;
+    const float mi = p.ws_ml[row * 2], li = p.ws_ml[row * 2 + 1];
+    const float4 v = lane * 4 < D ? *reinterpret_cast<const float4*>(p.ws_o + row * D + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+    const float mx = fmaxf(m, mi), a = ex2(m - mx), b = ex2(mi - mx);
+    m = mx;
+    l = l * a + li * b;
+    acc.x = acc.x * a + v.x * b; acc.y = acc.y * a + v.y * b; acc.z = acc.z * a + v.z * b; acc.w = acc.w * a + v.w * b;
   }
+  if (lane * 4 < D) *reinterpret_cast<float4*>(&s_acc[warp][lane * 4]) = acc;
+  if (lane == 0) { s_ml[warp][0] = m; s_ml[warp][1] = l; }
+  __syncthreads();
+  if (warp != 0 || lane * 4 >= D) return;
+  m = fmaxf(fmaxf(s_ml[0][0], s_ml[1][0]), fmaxf(s_ml[2][0], s_ml[3][0]));
+  l = 0.f;
+  acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane * 4 < D) store_head(p, seq, hk * p.G + hb * HEADS + h, lane, acc, sum);
+  for (int w = 0; w < 4; ++w) {
+    const float e = ex2(s_ml[w][0] - m);
+    const float4 v = *reinterpret_cast<const float4*>(&s_acc[w][lane * 4]);
+    l += s_ml[w][1] * e;
+    acc.x += v.x * e; acc.y += v.y * e; acc.z += v.z * e; acc.w += v.w * e;
+  }
+  store_head(p, seq, hk * p.G + hb * HEADS + h, lane, acc, l);
 }
 
 template <int D, int NT>
@@ -646,7 +653,8 @@ int launch_decode(const void* cache, DecParams& p, int ctas, cudaStream_t stream
   if (cs_launch_pdl(attention_decode_fp8_kernel<D, NT>, dim3(ctas), dim3(Shape::THREADS), Shape::SMEM, stream, tm_codes, tm_scales, p) !=
       cudaSuccess)
     return -10;
-  return cs_launch_pdl(attention_decode_fp8_join_kernel<D, NT>, dim3(ctas), dim3(256 * NT), 0, stream, p) == cudaSuccess ? 0 : -10;
+  return cs_launch_pdl(attention_decode_fp8_join_kernel<D, NT>, dim3(ctas, p.G < Shape::HEADS ? p.G : Shape::HEADS), dim3(128), 0, stream, p,
+                       ctas) == cudaSuccess ? 0 : -10;
 }
 
 }  // namespace
@@ -678,6 +686,8 @@ CS_API int cs_attention_decode_fp8(const void* q, long long q_tok, const void* c
   p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv;
   const int heads = p.G <= 8 ? 8 : 16;
   p.head_blocks = (p.G + heads - 1) / heads;
+  // units of the whole batch, were every table full: counted in 32 bits on the device
+  if (bt_width > 0 && static_cast<long long>(B) * Hkv * p.head_blocks > 0x7fffffffLL / (2LL * bt_width)) return -1;
   if (static_cast<long long>(B) * Hkv * p.head_blocks > 0x7fffffffLL) return -1;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.err = cs_error_word();
