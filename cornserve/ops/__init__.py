@@ -446,6 +446,7 @@ def attention_paged(q, cache, block_table, kv_len, cu_q, max_q_len: int, scale: 
 # --------------------------------------------------------------------------------------------
 KV_FP8_PAGE = reference.KV_FP8_PAGE
 KV_FP8_HEAD_DIMS = (64, 128)     # head widths the CUDA kernels are built for
+KV_FP8_MAX_SPLITS = 16           # parts the pages of one prompt tile are cut into when there are few tiles
 
 
 def kv_cache_fp8(num_pages: int, kv_heads: int, d: int, device: torch.device | str | None = None) -> torch.Tensor:
@@ -580,11 +581,19 @@ def attention_paged_fp8(q: torch.Tensor, cache: torch.Tensor, block_table: torch
              "cs_attention_decode_fp8")
         _count(2)
         return out
-    _chk(lib.cs_attention_paged_fp8(q.data_ptr(), q.stride(0), q.stride(1), cache.data_ptr(), cache.shape[0], out.data_ptr(), out.stride(0),
-                                    out.stride(1), cu_q.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(), block_table.stride(0),
-                                    block_table.shape[1], B, Tq, Hq, Hkv, d, float(scale), 1 if causal else 0, _stream()),
-         "cs_attention_paged_fp8")
-    _count()
+    # few items (a pair of 128-row tiles of one sequence and key head each): their pages are spread over idle SMs
+    pair = 2 * (128 // min(Hq // Hkv, 128))
+    items = B * Hkv * -(-max_q_len // pair)
+    splits = max(1, min(lib.cs_sm_count() // items, block_table.shape[1] // 2, KV_FP8_MAX_SPLITS))
+    ws, nbytes = None, 0
+    if splits > 1:
+        nbytes = Tq * Hq * splits * (d + 2) * 4
+        ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8)
+    _chk(lib.cs_attention_prefill_fp8(q.data_ptr(), q.stride(0), cache.data_ptr(), cache.shape[0], out.data_ptr(), out.stride(0),
+                                      out.stride(1), cu_q.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(), block_table.stride(0),
+                                      block_table.shape[1], B, Tq, max_q_len, Hq, Hkv, d, float(scale), 1 if causal else 0, splits,
+                                      _ptr(ws), nbytes, _stream()), "cs_attention_prefill_fp8")
+    _count(2 if splits > 1 else 1)
     return out
 
 

@@ -1,129 +1,647 @@
-// Attention of packed queries over the 8-bit paged key-value cache (layout in kv_fp8.cuh):
+// Attention of packed prompts (or chunks of them) over the 8-bit paged key-value cache (layout in kv_fp8.cuh):
 //
-//   o_i = sum_j 2^(s_ij - m_i) vs_j vc_j / sum_j 2^(s_ij - m_i),   s_ij = scale * log2(e) * ks_j * (q_i . kc_j)
+//   o_i = sum_j w_ij vc_j / sum_j w_ij / vs_j,   w_ij = 2^(s_ij + log2 vs_j - M_i),   s_ij = scale * log2(e) * ks_j * (q_i . kc_j)
 //
-// over the keys j that query i sees (all, or those up to its own position), with the codes kc, vc and the scales ks, vs
-// of the cache.  One warp per (token, query head), all arithmetic in fp32.
+// over the keys j that query i sees (all, or those up to its own position), with the e4m3 codes kc, vc and the scales
+// ks, vs of the cache.  Codes are exact in fp16, so both products run as fp16 tcgen05.mma on the codes themselves; the
+// scales enter in fp32, as one fused multiply-add per score on the way into the exponential and one into the normaliser.
+// M_i follows the largest weight (not the largest score), so weights fit fp16 whatever the value scales are.  Queries
+// become fp16 too, scaled by a power of two that is common to a tile pair (exact for every element within 2^-38 of the
+// pair's largest).
+//
+// One CTA works on 2 x 128 query rows of one sequence and one key head (rows = tokens x the query heads that share the
+// key head) against pages of 128 keys:
+//   warps 0-3, 4-7 : softmax of tile 0 / tile 1, one thread per row; scores come from TMEM, weights go back to TMEM over
+//                    them and are the A operand of the second product there
+//   warps 8-11     : operand preparation: e4m3 codes from global memory through registers to fp16 tiles in shared memory
+//                    (128-byte swizzle), the scale vectors of a page, the queries of an item
+//   warp 12        : issues tcgen05.mma: S_t = Q_t K^T (t = 0, 1) and O_t += P_t V.  While one tile's softmax runs, the
+//                    tensor cores work for the other.
+// The codes are converted once per 256 query rows.  They are not staged in shared memory as bytes: its bandwidth is what
+// this kernel has least of (192 KB of operands per page and tile pair for the products alone), so the preparation warps
+// load them straight into registers, a tile ahead.  Few items (short chunks over a long cache) split the pages of an item
+// over several CTAs and a second kernel joins the parts.
 #include <math.h>
 
 #include "kv_fp8.cuh"
 
 namespace {
 
-struct PagedParams {
-  const __nv_bfloat16* q; long long q_tok, q_head;   // strides in elements
-  __nv_bfloat16* o; long long o_tok, o_head;
-  const uint8_t* cache; long long num_pages;
+constexpr int ATOM = 128 * 128;            // 128 rows x 64 fp16, 128-byte swizzle
+constexpr int RING = 4;                    // fp16 tiles (K0 V0 K1 V1 ...)
+constexpr int SRING = 4;                   // scale vectors of a page
+constexpr int THREADS = 512;
+constexpr float M_NONE = -3.0e38f;         // running maximum before the first key (finite: differences stay defined)
+// registers per thread after setmaxnreg; 2 * 128 * 176 + 128 * 112 + 128 * 48 = the 512 * 128 launched with
+constexpr int REGS_SOFTMAX = 176, REGS_PREP = 112, REGS_MMA = 48;
+
+struct PrefillParams {
+  const __nv_bfloat16* q; long long q_tok;              // heads follow each other; every token on a 16-byte boundary
+  __nv_bfloat16* o; long long o_tok, o_head; int o_vec; // o_vec: 16-byte stores are aligned
+  const uint8_t* cache; int num_pages;
   const int* block_table; long long bt_stride; int bt_width;
-  const int* kv_len;
-  const int* cu_q;
-  int B, Tq, Hq, Hkv, causal;
+  const int* kv_len; const int* cu_q;
+  int B, Hq, Hkv, G, head_blocks, causal;               // G query heads of a key head per tile row block
+  int tok_per_tile, max_pairs, total_items, splits;
   float scale_log2;
+  float* ws_o;     // [Tq * Hq, splits, D] sums of the parts
+  float* ws_ml;    // [Tq * Hq, splits, 2] their maximum and normaliser
+  uint32_t idesc_s, idesc_pv;
   int* err;
 };
 
+// One work item: a pair of query tiles of one sequence and key head (block), and a range of its pages.
+struct Item {
+  int seq, hk, h0, n_heads, q_beg, q_len, t0, k_len, shift, j0, n, split;
+  bool valid;
+};
+
+__device__ __forceinline__ Item get_item(const PrefillParams& p, int w) {
+  Item it;
+  it.split = w % p.splits;
+  w /= p.splits;
+  const int blocks = p.Hkv * p.head_blocks, hb = w % blocks;
+  w /= blocks;
+  it.seq = w % p.B;
+  const int back = w / p.B;                 // the last pairs of every sequence, which see the most keys, come first
+  it.hk = hb / p.head_blocks;
+  const int first = (hb - it.hk * p.head_blocks) * p.G, group = p.Hq / p.Hkv;
+  it.h0 = it.hk * group + first;
+  it.n_heads = min(p.G, group - first);
+  it.q_beg = p.cu_q[it.seq];
+  it.q_len = p.cu_q[it.seq + 1] - it.q_beg;
+  const int pair_tok = 2 * p.tok_per_tile, pairs = (it.q_len + pair_tok - 1) / pair_tok;
+  it.valid = back < pairs;
+  it.t0 = (pairs - 1 - back) * pair_tok;
+  const int len = p.kv_len[it.seq];
+  const long long cap = static_cast<long long>(p.bt_width) * KV8_PAGE;
+  it.k_len = len < 0 ? 0 : (len > cap ? static_cast<int>(cap) : len);
+  it.shift = len - it.q_len;                // causal: token i sees keys j <= i + shift
+  const int end = p.causal ? min(it.k_len, min(it.q_len, it.t0 + pair_tok) + it.shift) : it.k_len;
+  const int pages = it.valid && end > 0 ? (end + KV8_PAGE - 1) / KV8_PAGE : 0;
+  it.j0 = static_cast<int>(static_cast<long long>(it.split) * pages / p.splits);
+  it.n = static_cast<int>(static_cast<long long>(it.split + 1) * pages / p.splits) - it.j0;
+  return it;
+}
+
+// CTA b walks the items in a snake (0 .. g-1, then g-1 .. 0, ...): with items in falling order of size this evens out.
+__device__ __forceinline__ int item_at(int round) {
+  const int g = gridDim.x, b = blockIdx.x;
+  return round * g + ((round & 1) ? g - 1 - b : b);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// D[tmem] (+)= A[tmem] * B[smem], fp16 inputs, fp32 accumulate
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+template <int N>
+__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// Four codes as fp16 numbers times 2^-8, in the order (0, 2), (1, 3): the sign stays on top and the seven magnitude bits
+// move one place down, where e4m3's exponent is fp16's exponent minus 8 (subnormal codes become subnormal halves).  On
+// the integer pipe: the conversion instruction shares its pipe with the exponentials of the softmax.
+__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& r02, uint32_t& r13) {
+  const uint32_t e = w << 8;
+  r13 = (w & 0x80008000u) | ((w >> 1) & 0x3f803f80u);
+  r02 = (e & 0x80008000u) | ((e >> 1) & 0x3f803f80u);
+}
+
+// Shared memory: queries (two tiles), ring of fp16 tiles, scale vectors.
 template <int D>
-__global__ void __launch_bounds__(128) attention_paged_fp8_kernel(const PagedParams p) {
-  constexpr int PER = D / 32;   // channels per lane in the value product
-  __shared__ float sq[4][D];
+struct Shape {
+  static constexpr int ATOMS = D / 64, TILE = ATOMS * ATOM;
+  static constexpr int Q = 2 * TILE, SCALES = SRING * 3 * KV8_PAGE * 4;
+  static constexpr int SMEM = 1024 + Q + RING * TILE + SCALES;
+};
+
+template <int D>
+__global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const PrefillParams p) {
+  constexpr int TILE = Shape<D>::TILE, KSTEPS = D / 16;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* s_q = smem;
+  uint8_t* s_kv = smem + Shape<D>::Q;
+  float* s_scale = reinterpret_cast<float*>(s_kv + RING * TILE);      // [SRING][a, log2 vs, 1 / vs][128]
+  __shared__ uint64_t q_full, q_empty, kv_full[RING], kv_empty[RING], sc_full[SRING], sc_empty[SRING], s_full[2], p_full[2], o_full[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  __shared__ uint32_t s_max[4];
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    mbar_init(&q_full, 128);
+    mbar_init(&q_empty, 1);
+    for (int i = 0; i < RING; ++i) { mbar_init(&kv_full[i], 128); mbar_init(&kv_empty[i], 1); }
+    for (int i = 0; i < SRING; ++i) { mbar_init(&sc_full[i], 128); mbar_init(&sc_empty[i], 8); }
+    for (int t = 0; t < 2; ++t) { mbar_init(&s_full[t], 1); mbar_init(&p_full[t], 128); mbar_init(&o_full[t], 1); }
+    mbar_fence_init();
+  }
+  if (warp == 12) { tmem_alloc(&tmem_slot, 512); tmem_relinquish(); }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
   pdl_wait();
   pdl_launch_dependents();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long item = static_cast<long long>(blockIdx.x) * 4 + warp;
-  if (item >= static_cast<long long>(p.Tq) * p.Hq) return;
-  const int t = static_cast<int>(item / p.Hq), h = static_cast<int>(item % p.Hq), hk = h / (p.Hq / p.Hkv);
-  if (t >= p.cu_q[p.B]) return;   // a row behind the last sequence
-  int lo = 0, hi = p.B;           // the sequence with cu_q[lo] <= t < cu_q[lo + 1]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (p.cu_q[mid] <= t) lo = mid; else hi = mid;
-  }
-  const int seq = lo;
-  int k_len = p.kv_len[seq];
-  if (k_len > p.bt_width * KV8_PAGE) {
-    if (lane == 0) cs_set_error(p.err, CS_ERR_BAD_ARG);
-    k_len = p.bt_width * KV8_PAGE;
-  }
-  const int shift = p.kv_len[seq] - (p.cu_q[seq + 1] - p.cu_q[seq]);
-  const int lim = p.causal ? min(k_len, t - p.cu_q[seq] + shift + 1) : k_len;
-  const __nv_bfloat16* q = p.q + t * p.q_tok + h * p.q_head;
-  for (int i = lane; i < D; i += 32) sq[warp][i] = __bfloat162float(q[i]);
-  __syncwarp();
-  float m = -INFINITY, l = 0.f, acc[PER];
+  const uint32_t tmem = tmem_slot;      // S_0, S_1 at columns 0, 128 (P_t over the first half of S_t), O_0, O_1 at 256, 384
+  volatile int* abortp = &abort_flag;
+
+  // No role leaves its loops early when a wait gives up: later waits return at once, and all keep their barriers company.
+  if (warp >= 12) {
+    regs_dec<REGS_MMA>();
+    if (warp == 12 && lane == 0) {
+      // -------------------------------- MMA issuer --------------------------------
+      const uint32_t q_addr = smem_u32(s_q), kv_addr = smem_u32(s_kv);
+      uint32_t n_item = 0, n_kv = 0, n_p = 0;     // running counts: items, fp16 tiles consumed, softmax steps
+      auto wait_kv = [&](uint32_t n) {
+        mbar_wait(&kv_full[n % RING], (n / RING) & 1, abortp, p.err, CS_ERR_TIMEOUT_TMA);
+        tc_fence_after();
+      };
+      auto issue_s = [&](int t, uint32_t n) {
+        const uint32_t a = q_addr + t * TILE, b = kv_addr + (n % RING) * TILE;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) acc[i] = 0.f;
-  for (int base = 0; base < lim; base += 32) {
-    const int j = base + lane;
-    long long page = p.block_table[seq * p.bt_stride + (base / KV8_PAGE)];
-    if (page < 0 || page >= p.num_pages) {
-      if (lane == 0) cs_set_error(p.err, CS_ERR_BAD_ARG);
-      page = 0;
-    }
-    const uint8_t* kb = p.cache + (page * 2 * p.Hkv + hk) * kv8_block_bytes(D);
-    const uint8_t* vb = p.cache + ((page * 2 + 1) * p.Hkv + hk) * kv8_block_bytes(D);
-    float s = -INFINITY;
-    if (j < lim) {
-      const int r = j % KV8_PAGE;
-      float dot = 0.f;
-      for (int i = 0; i < D; i += 4) {
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(kb + r * D + i);
-        const uint32_t x = e4m3x2_to_half2(w & 0xffffu), y = e4m3x2_to_half2(w >> 16);
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x)), g = __half22float2(*reinterpret_cast<const __half2*>(&y));
-        dot += f.x * sq[warp][i] + f.y * sq[warp][i + 1] + g.x * sq[warp][i + 2] + g.y * sq[warp][i + 3];
-      }
-      s = dot * reinterpret_cast<const float*>(kb + KV8_PAGE * D)[r] * p.scale_log2;
-    }
-    float mx = s;
+        for (int kk = 0; kk < KSTEPS; ++kk) {
+          const uint32_t off = (kk >> 2) * ATOM + (kk & 3) * 32;
+          umma_f16_ss(tmem + t * 128, umma_smem_desc(a + off, 16, 1024), umma_smem_desc(b + off, 16, 1024), p.idesc_s, kk != 0);
+        }
+        umma_commit(&s_full[t]);
+      };
+      auto issue_pv = [&](int t, uint32_t n, bool first) {
+        const uint32_t b = kv_addr + (n % RING) * TILE;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    const float m_new = fmaxf(m, mx), m_use = m_new == -INFINITY ? 0.f : m_new;
-    const float alpha = exp2f(m - m_use), e = exp2f(s - m_use);
-    m = m_new;
-    l = l * alpha + e;
+        for (int kk = 0; kk < KV8_PAGE / 16; ++kk)
+          umma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, umma_smem_desc(b + kk * 2048, ATOM, 1024), p.idesc_pv,
+                      !(first && kk == 0));
+      };
+      for (int round = 0; round * static_cast<int>(gridDim.x) < p.total_items; ++round) {
+        const int w = item_at(round);
+        if (w >= p.total_items) continue;
+        const Item it = get_item(p, w);
+        if (it.n == 0) continue;
+        mbar_wait(&q_full, n_item & 1, abortp, p.err, CS_ERR_TIMEOUT_TMA);
+        ++n_item;
+        wait_kv(n_kv);
+        issue_s(0, n_kv);
+        issue_s(1, n_kv);
+        umma_commit(&kv_empty[n_kv % RING]);
+        if (it.n == 1) umma_commit(&q_empty);
+        for (int j = 0; j < it.n; ++j, ++n_p, n_kv += 2) {
+          const bool more = j + 1 < it.n;
+          wait_kv(n_kv + 1);                       // V of this page
+          if (more) wait_kv(n_kv + 2);             // K of the next
 #pragma unroll
-    for (int i = 0; i < PER; ++i) acc[i] *= alpha;
-    const int n = min(32, lim - base), r0 = base % KV8_PAGE;
-    for (int jj = 0; jj < n; ++jj) {
-      const float w = __shfl_sync(0xffffffffu, e, jj) * reinterpret_cast<const float*>(vb + KV8_PAGE * D)[r0 + jj];
-#pragma unroll
-      for (int i = 0; i < PER; i += 2) {
-        const uint32_t x = e4m3x2_to_half2(*reinterpret_cast<const uint16_t*>(vb + (r0 + jj) * D + lane * PER + i));
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x));
-        acc[i] += w * f.x;
-        acc[i + 1] += w * f.y;
+          for (int t = 0; t < 2; ++t) {
+            mbar_wait(&p_full[t], n_p & 1, abortp, p.err, CS_ERR_TIMEOUT_EPI);
+            tc_fence_after();
+            issue_pv(t, n_kv + 1, j == 0);
+            if (t == 1) umma_commit(&kv_empty[(n_kv + 1) % RING]);
+            if (more) issue_s(t, n_kv + 2); else umma_commit(&o_full[t]);
+          }
+          if (more) {
+            umma_commit(&kv_empty[(n_kv + 2) % RING]);
+            if (j + 2 == it.n) umma_commit(&q_empty);
+          }
+        }
       }
     }
-  }
+  } else if (warp >= 8) {
+    // ------------------------------ operand preparation ------------------------------
+    regs_dec<REGS_PREP>();
+    constexpr int CHUNKS = D / 16;                 // 16-byte chunks of codes per row
+    constexpr int ITER = CHUNKS;                   // chunks per thread and tile (128 rows, 128 threads)
+    const int tid = threadIdx.x - 256;
+    // Chunk `it` of this thread: the eight threads of a shared-memory phase write two rows of different parity, so that
+    // the swizzle sends their stores to different banks.
+    auto place = [&](int i, int& row, int& c) {
+      if (D == 128) {
+        const int g8 = (tid >> 3) & 3;
+        row = i * 16 + (tid >> 5) * 4 + (g8 >> 1) * 2 + ((tid >> 2) & 1);
+        c = (g8 & 1) * 4 + (tid & 3);
+      } else {
+        const int lin = i * 128 + tid;
+        row = lin >> 2;
+        c = lin & 3;
+      }
+    };
+    uint32_t n_kv = 0, n_sc = 0, n_item = 0;
+    uint4 cur[ITER], nxt[ITER];
+    float ks = 0.f, vs = 0.f;                      // scales of key `tid` of the page in `cur` / `nxt`
+    // codes of keys (kv = 0) or values (kv = 1) of page j of an item
+    auto fetch = [&](const Item& it, int j, int kv, uint4 (&dst)[ITER], float& scale) {
+      int page = p.block_table[it.seq * p.bt_stride + j];
+      if (page < 0 || page >= p.num_pages) {
+        if (tid == 0) cs_set_error(p.err, CS_ERR_BAD_ARG);
+        page = 0;
+      }
+      const uint8_t* src = p.cache + ((static_cast<long long>(page) * 2 + kv) * p.Hkv + it.hk) * kv8_block_bytes(D);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+      for (int i = 0; i < ITER; ++i) {
+        int row, c;
+        place(i, row, c);
+        dst[i] = __ldg(reinterpret_cast<const uint4*>(src + row * D + c * 16));
+      }
+      scale = __ldg(reinterpret_cast<const float*>(src + KV8_PAGE * D) + tid);
+    };
+    auto store = [&](const uint4 (&src)[ITER]) {
+      const uint32_t slot = n_kv % RING;
+      mbar_wait(&kv_empty[slot], ((n_kv / RING) & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
+      uint8_t* tile = s_kv + slot * TILE;
+#pragma unroll
+      for (int i = 0; i < ITER; ++i) {
+        int row, c;
+        place(i, row, c);
+        uint4 a, b;
+        codes_to_half(src[i].x, a.x, a.y);
+        codes_to_half(src[i].y, a.z, a.w);
+        codes_to_half(src[i].z, b.x, b.y);
+        codes_to_half(src[i].w, b.z, b.w);
+        uint8_t* dst = tile + (c >> 2) * ATOM + row * 128;
+        const int ch = (c & 3) * 2;
+        *reinterpret_cast<uint4*>(dst + ((ch ^ (row & 7)) << 4)) = a;
+        *reinterpret_cast<uint4*>(dst + (((ch + 1) ^ (row & 7)) << 4)) = b;
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&kv_full[slot]);
+      ++n_kv;
+    };
+    auto next_item = [&](int round) {              // the next round that gives an item with pages, or -1
+      for (; round * static_cast<int>(gridDim.x) < p.total_items; ++round) {
+        const int w = item_at(round);
+        if (w < p.total_items && get_item(p, w).n > 0) return round;
+      }
+      return -1;
+    };
+    int round = next_item(0);
+    if (round >= 0) {
+      const Item first = get_item(p, item_at(round));
+      fetch(first, first.j0, 0, nxt, ks);
+    }
+    while (round >= 0) {
+      const Item it = get_item(p, item_at(round));
+      // queries of both tiles: thread = row; largest magnitude of the finite rows first, then fp16 with a common scale
+      const int group = p.G;
+      float cq;
+      {
+        uint32_t mx = 0;
+        const __nv_bfloat16* src[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int tl = tid / group, g = tid - tl * group, tok = it.t0 + t * p.tok_per_tile + tl;
+          const bool ok = tl < p.tok_per_tile && tok < it.q_len && g < it.n_heads;
+          src[t] = ok ? p.q + (it.q_beg + tok) * p.q_tok + (it.h0 + g) * D : nullptr;
+          if (!ok) continue;
+          uint32_t m = 0;
+          for (int i = 0; i < D / 8; ++i) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(src[t]) + i);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) m = max(m, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
+          }
+          if (m < 0x7f80u) mx = max(mx, m);
+        }
+        mx = __reduce_max_sync(0xffffffffu, mx);
+        if (lane == 0) s_max[warp - 8] = mx;
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        mx = max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3]));
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        const int shift = min(max(127 + 14 - static_cast<int>(mx >> 7), -110), 110);   // the largest element into [2^14, 2^15)
+        const float up = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
+        cq = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + 8 - shift) << 23);   // 2^8: fp16 keys are code / 2^8
+        mbar_wait(&q_empty, (n_item & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
+        ++n_item;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          uint8_t* dst = s_q + t * TILE + tid * 128;
+          for (int i = 0; i < D / 8; ++i) {
+            const uint4 v = src[t] != nullptr ? __ldg(reinterpret_cast<const uint4*>(src[t]) + i) : make_uint4(0, 0, 0, 0);
+            uint4 h;   // channels in the order of the codes: (0, 2), (1, 3) of every four
+            h.x = half2_bits(bf16lo(v.x) * up, bf16lo(v.y) * up);
+            h.y = half2_bits(bf16hi(v.x) * up, bf16hi(v.y) * up);
+            h.z = half2_bits(bf16lo(v.z) * up, bf16lo(v.w) * up);
+            h.w = half2_bits(bf16hi(v.z) * up, bf16hi(v.w) * up);
+            *reinterpret_cast<uint4*>(dst + (i >> 3) * ATOM + (((i & 7) ^ (tid & 7)) << 4)) = h;
+          }
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(&q_full);
+      }
+      round = next_item(round + 1);
+      for (int j = 0; j < it.n; ++j) {
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) cur[i] = nxt[i];
+        const float k_scale = ks;
+        fetch(it, it.j0 + j, 1, nxt, vs);            // V while K is converted
+        store(cur);
+        const uint32_t s = n_sc % SRING;
+        mbar_wait(&sc_empty[s], ((n_sc / SRING) & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
+        float* sc = s_scale + s * 3 * KV8_PAGE + tid;
+        const float v = vs < 1.2e-38f ? 1.2e-38f : vs;
+        sc[0] = k_scale * cq;
+        sc[KV8_PAGE] = __log2f(v);
+        sc[2 * KV8_PAGE] = 1.0f / v;
+        mbar_arrive(&sc_full[s]);
+        ++n_sc;
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) cur[i] = nxt[i];
+        if (j + 1 < it.n) fetch(it, it.j0 + j + 1, 0, nxt, ks);
+        else if (round >= 0) {
+          const Item after = get_item(p, item_at(round));
+          fetch(after, after.j0, 0, nxt, ks);
+        }
+        store(cur);
+      }
+    }
+  } else {
+    // ---------------------------------- softmax -----------------------------------
+    regs_inc<REGS_SOFTMAX>();
+    const int t = warp >> 2, r = (warp & 3) * 32 + lane;         // tile, row == TMEM lane
+    const int tl = r / p.G, g = r - tl * p.G;                    // token in tile, head within group
+    const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + t * 128 + lane_off, tO = tmem + 256 + t * 128 + lane_off;
+    uint32_t n_step = 0, n_item = 0;
+    for (int round = 0; round * static_cast<int>(gridDim.x) < p.total_items; ++round) {
+      const int w = item_at(round);
+      if (w >= p.total_items) continue;
+      const Item it = get_item(p, w);
+      if (!it.valid) continue;
+      const int tok = it.t0 + t * p.tok_per_tile + tl;
+      const bool row_ok = tl < p.tok_per_tile && tok < it.q_len && g < it.n_heads;
+      const int lim = p.causal ? min(it.k_len, tok + it.shift + 1) : it.k_len;     // keys [0, lim) are visible
+      float m = M_NONE;
+      uint64_t l2 = pack2(0.f, 0.f);
+      for (int j = 0; j < it.n; ++j, ++n_step) {
+        const uint32_t s = n_step % SRING;
+        mbar_wait(&sc_full[s], (n_step / SRING) & 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
+        mbar_wait(&s_full[t], n_step & 1, abortp, p.err, CS_ERR_TIMEOUT_MMA);
+        tc_fence_after();
+        uint32_t x[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, x[c]);
+        tmem_wait_ld();
+        // t = s + log2 vs, in place
+        const float* sc = s_scale + s * 3 * KV8_PAGE;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(sc + c * 32 + i);
+            const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(sc + KV8_PAGE + c * 32 + i);
+            float y0, y1;
+            unpack2(fma2(pack2(__uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1])), a.x, b.x), y0, y1);
+            x[c][i] = __float_as_uint(y0);
+            x[c][i + 1] = __float_as_uint(y1);
+            unpack2(fma2(pack2(__uint_as_float(x[c][i + 2]), __uint_as_float(x[c][i + 3])), a.y, b.y), y0, y1);
+            x[c][i + 2] = __float_as_uint(y0);
+            x[c][i + 3] = __float_as_uint(y1);
+          }
+        const int nvalid = lim - (it.j0 + j) * KV8_PAGE;
+        if (nvalid < KV8_PAGE) {                     // hidden keys: whatever their scales were
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (c * 32 + i >= nvalid) x[c][i] = 0xff800000u;
+        }
+        float mx[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          mx[c] = __uint_as_float(x[c][0]);
+#pragma unroll
+          for (int i = 1; i < 32; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(x[c][i]));
+        }
+        const float mx_all = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        // The reference m - 6 moves only when a weight would pass 2^14
+        const float m_new = mx_all > m + 8.f ? mx_all : m;
+        const float alpha = ex2(m - m_new);
+        if (__any_sync(0xffffffffu, m_new != m)) {   // tcgen05.ld / st are warp-wide: the warp decides together
+          float lo, hi;
+          unpack2(l2, lo, hi);
+          l2 = pack2(lo * alpha, hi * alpha);
+          if (j > 0) {                               // PV of the last page is complete: S of this one was issued behind it
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t o[16];
+              tmem_ld16(tO + c * 16, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st16(tO + c * 16, o);
+            }
+          }
+        }
+        m = m_new;
+        const uint64_t ref = pack2(6.f - m, 6.f - m);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {       // 64 keys at a time: their weights go straight to TMEM
+          uint32_t pk[32];
+#pragma unroll
+          for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              const int c = half * 2 + cc, k = c * 32 + i;
+              ulonglong2 iv = *reinterpret_cast<const ulonglong2*>(sc + 2 * KV8_PAGE + k);
+              float e0, e1, e2, e3;
+              unpack2(add2(pack2(__uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1])), ref), e0, e1);
+              unpack2(add2(pack2(__uint_as_float(x[c][i + 2]), __uint_as_float(x[c][i + 3])), ref), e2, e3);
+              e0 = ex2(e0); e1 = ex2(e1); e2 = ex2(e2); e3 = ex2(e3);
+              if (nvalid < KV8_PAGE) {               // 0 / vs of a hidden key may not be 0
+                float i0, i1, i2, i3;
+                unpack2(iv.x, i0, i1);
+                unpack2(iv.y, i2, i3);
+                iv.x = pack2(k < nvalid ? i0 : 0.f, k + 1 < nvalid ? i1 : 0.f);
+                iv.y = pack2(k + 2 < nvalid ? i2 : 0.f, k + 3 < nvalid ? i3 : 0.f);
+              }
+              l2 = fma2(pack2(e0, e1), iv.x, l2);
+              l2 = fma2(pack2(e2, e3), iv.y, l2);
+              pk[cc * 16 + (i >> 1)] = half2_bits(e0, e1);
+              pk[cc * 16 + (i >> 1) + 1] = half2_bits(e2, e3);
+            }
+          tmem_st32(tS + half * 32, pk);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sc_empty[s]);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&p_full[t]);
+      }
+      // ---------------------------------- output ------------------------------------
+      if (it.n > 0) {
+        mbar_wait(&o_full[t], n_item & 1, abortp, p.err, CS_ERR_TIMEOUT_MMA);
+        ++n_item;
+        tc_fence_after();
+      }
+      float l_lo, l_hi;
+      unpack2(l2, l_lo, l_hi);
+      const float l = l_lo + l_hi;
+      const long long row = static_cast<long long>(it.q_beg + tok) * p.Hq + it.h0 + g;
+      if (p.splits > 1 && row_ok) {
+        p.ws_ml[(row * p.splits + it.split) * 2] = m;
+        p.ws_ml[(row * p.splits + it.split) * 2 + 1] = l;
+      }
+      const float inv = p.splits > 1 ? 256.f : (l == 0.f ? 0.f : 256.f / l);          // 2^8: fp16 values are code / 2^8
+      __nv_bfloat16* dst = p.o + static_cast<long long>(it.q_beg + tok) * p.o_tok + (it.h0 + g) * p.o_head;
+      float* part = p.splits > 1 ? p.ws_o + (row * p.splits + it.split) * D : nullptr;
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) {
+        uint32_t o[16];
+        if (it.n > 0) {
+          tmem_ld16(tO + c * 16, o);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i] = 0u;
+        }
+        if (!row_ok) continue;
+        float f[16];   // back from (0, 2), (1, 3)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(o[(i & ~3) + ((i & 1) << 1) + ((i >> 1) & 1)]) * inv;
+        if (p.splits > 1) {
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(part + c * 16 + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+        } else if (p.o_vec) {
+#pragma unroll
+          for (int i = 0; i < 16; i += 8)
+            *reinterpret_cast<uint4*>(dst + c * 16 + i) = make_uint4(pack_bf16x2(f[i], f[i + 1]), pack_bf16x2(f[i + 2], f[i + 3]),
+                                                                     pack_bf16x2(f[i + 4], f[i + 5]), pack_bf16x2(f[i + 6], f[i + 7]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) dst[c * 16 + i] = __float2bfloat16(f[i]);
+        }
+      }
+      tc_fence_before();
+    }
+    // lengths that do not fit the table are reported
+    for (int b = blockIdx.x * 256 + threadIdx.x; b < p.B; b += gridDim.x * 256)
+      if (p.kv_len[b] > static_cast<long long>(p.bt_width) * KV8_PAGE) cs_set_error(p.err, CS_ERR_BAD_ARG);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) { tc_fence_after(); tmem_dealloc(tmem, 512); }
+}
+
+// Joins the parts of the rows of an item that was split: one warp per (token, head) row, parts in order.
+template <int D>
+__global__ void __launch_bounds__(256) attention_prefill_fp8_join_kernel(const PrefillParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const long long row = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= static_cast<long long>(p.cu_q[p.B]) * p.Hq || row < static_cast<long long>(p.cu_q[0]) * p.Hq) return;
+  float mx = M_NONE, l = 0.f;
+  for (int s = 0; s < p.splits; ++s) mx = fmaxf(mx, p.ws_ml[(row * p.splits + s) * 2]);
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int s = 0; s < p.splits; ++s) {
+    const long long at = row * p.splits + s;
+    const float e = ex2(p.ws_ml[at * 2] - mx);
+    l += p.ws_ml[at * 2 + 1] * e;
+    if (lane * 4 < D) {
+      const float4 v = *reinterpret_cast<const float4*>(p.ws_o + at * D + lane * 4);
+      acc.x += v.x * e; acc.y += v.y * e; acc.z += v.z * e; acc.w += v.w * e;
+    }
+  }
+  if (lane * 4 >= D) return;
   const float inv = l == 0.f ? 0.f : 1.0f / l;
-  __nv_bfloat16* out = p.o + t * p.o_tok + h * p.o_head + lane * PER;
+  __nv_bfloat16* dst = p.o + row / p.Hq * p.o_tok + row % p.Hq * p.o_head + lane * 4;
+  const float f[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+  if (p.o_vec) {
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
+  } else {
 #pragma unroll
-  for (int i = 0; i < PER; ++i) out[i] = __float2bfloat16(acc[i] * inv);
+    for (int i = 0; i < 4; ++i) dst[i] = __float2bfloat16(f[i]);
+  }
+}
+
+template <int D>
+int launch_prefill(const PrefillParams& p, int grid, long long rows, cudaStream_t stream) {
+  static bool ready[64] = {false};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -10;
+  if (!ready[dev]) {
+    // the register split after setmaxnreg must fit what the block is launched with
+    cudaFuncAttributes a{};
+    if (cudaFuncGetAttributes(&a, attention_prefill_fp8_kernel<D>) != cudaSuccess) return -10;
+    if (a.numRegs * THREADS < 256 * REGS_SOFTMAX + 128 * REGS_PREP + 128 * REGS_MMA) return -6;
+    if (cudaFuncSetAttribute(attention_prefill_fp8_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::SMEM) != cudaSuccess)
+      return -10;
+    ready[dev] = true;
+  }
+  if (cs_launch_pdl(attention_prefill_fp8_kernel<D>, dim3(grid), dim3(THREADS), Shape<D>::SMEM, stream, p) != cudaSuccess) return -10;
+  if (p.splits == 1) return 0;
+  return cs_launch_pdl(attention_prefill_fp8_join_kernel<D>, dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256), 0, stream, p) == cudaSuccess
+             ? 0 : -10;
 }
 
 }  // namespace
 
-// q, o: [Tq, Hq, d] with token and head strides in elements (channels contiguous); d is 64 or 128.
-CS_API int cs_attention_paged_fp8(const void* q, long long q_tok, long long q_head, const void* cache, long long num_pages, void* o,
-                                  long long o_tok, long long o_head, const void* cu_q, const void* kv_len, const void* block_table,
-                                  long long bt_stride, int bt_width, int B, int Tq, int Hq, int Hkv, int d, float scale, int causal,
-                                  void* stream) {
-  if (B <= 0 || Tq <= 0) return 0;
-  if ((d != 64 && d != 128) || Hkv <= 0 || Hq % Hkv != 0) return -1;
-  PagedParams p{};
-  p.q = (const __nv_bfloat16*)q; p.q_tok = q_tok; p.q_head = q_head;
+// q: [Tq, Hq, d] with contiguous heads, tokens q_tok elements apart and on 16-byte boundaries; o: [Tq, Hq, d] with token and
+// head strides in elements; d is 64 or 128.  No sequence has more than max_q_len queries.  splits > 1 cuts the pages of
+// every item into that many parts; ws then holds Tq * Hq * splits * (d + 2) floats that no call on another stream uses.
+CS_API int cs_attention_prefill_fp8(const void* q, long long q_tok, const void* cache, long long num_pages, void* o, long long o_tok,
+                                    long long o_head, const void* cu_q, const void* kv_len, const void* block_table, long long bt_stride,
+                                    int bt_width, int B, int Tq, int max_q_len, int Hq, int Hkv, int d, float scale, int causal, int splits,
+                                    void* ws, long long ws_bytes, void* stream) {
+  if (B <= 0 || Tq <= 0 || max_q_len <= 0) return 0;
+  if ((d != 64 && d != 128) || Hkv <= 0 || Hq <= 0 || Hq % Hkv != 0 || num_pages <= 0 || num_pages > 0x7fffffffLL) return -1;
+  if ((reinterpret_cast<uintptr_t>(q) & 15) || (q_tok & 7)) return -1;
+  PrefillParams p{};
+  p.q = (const __nv_bfloat16*)q; p.q_tok = q_tok;
   p.o = (__nv_bfloat16*)o; p.o_tok = o_tok; p.o_head = o_head;
-  p.cache = (const uint8_t*)cache; p.num_pages = num_pages;
+  p.o_vec = (reinterpret_cast<uintptr_t>(o) & 15) == 0 && (o_tok & 7) == 0 && (o_head & 7) == 0;
+  p.cache = (const uint8_t*)cache; p.num_pages = static_cast<int>(num_pages);
   p.block_table = (const int*)block_table; p.bt_stride = bt_stride; p.bt_width = bt_width;
   p.kv_len = (const int*)kv_len; p.cu_q = (const int*)cu_q;
-  p.B = B; p.Tq = Tq; p.Hq = Hq; p.Hkv = Hkv; p.causal = causal;
+  const int group = Hq / Hkv;
+  p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.G = group < 128 ? group : 128; p.causal = causal;
+  p.head_blocks = (group + p.G - 1) / p.G;
+  p.tok_per_tile = 128 / p.G;
+  p.max_pairs = (max_q_len + 2 * p.tok_per_tile - 1) / (2 * p.tok_per_tile);
   p.scale_log2 = scale * 1.4426950408889634f;
   p.err = cs_error_word();
-  const long long blocks = (static_cast<long long>(Tq) * Hq + 3) / 4;
-  if (blocks > 0x7fffffffLL) return -1;
-  cudaError_t e;
-  if (d == 128) e = cs_launch_pdl(attention_paged_fp8_kernel<128>, dim3((unsigned)blocks), dim3(128), 0, (cudaStream_t)stream, p);
-  else e = cs_launch_pdl(attention_paged_fp8_kernel<64>, dim3((unsigned)blocks), dim3(128), 0, (cudaStream_t)stream, p);
-  return e == cudaSuccess ? 0 : -10;
+  p.idesc_s = umma_idesc_f16(128, 128, 0, 0);
+  p.idesc_pv = umma_idesc_f16(128, d, 0, 1);
+  p.splits = splits < 1 ? 1 : splits;
+  const long long rows = static_cast<long long>(Tq) * Hq;
+  if (p.splits > 1) {
+    if (ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 15) || rows * p.splits * (d + 2) * 4 > ws_bytes) return -5;
+    p.ws_o = reinterpret_cast<float*>(ws);
+    p.ws_ml = p.ws_o + rows * p.splits * d;
+  }
+  const long long total = static_cast<long long>(p.max_pairs) * B * Hkv * p.head_blocks * p.splits;
+  if (total > 0x3fffffffLL || (rows + 7) / 8 > 0x7fffffffLL) return -1;
+  p.total_items = static_cast<int>(total);
+  const int grid = p.total_items < cs_num_sms() ? p.total_items : cs_num_sms();
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  return d == 128 ? launch_prefill<128>(p, grid, rows, st) : launch_prefill<64>(p, grid, rows, st);
 }
