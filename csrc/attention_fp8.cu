@@ -30,10 +30,8 @@ namespace {
 constexpr int ATOM = 128 * 128;            // 128 rows x 64 fp16, 128-byte swizzle
 constexpr int RING = 4;                    // fp16 tiles (K0 V0 K1 V1 ...)
 constexpr int SRING = 4;                   // scale vectors of a page
-constexpr int THREADS = 512;
+constexpr int THREADS = 13 * 32;
 constexpr float M_NONE = -3.0e38f;         // running maximum before the first key (finite: differences stay defined)
-// registers per thread after setmaxnreg; 2 * 128 * 176 + 128 * 112 + 128 * 48 = the 512 * 128 launched with
-constexpr int REGS_SOFTMAX = 176, REGS_PREP = 112, REGS_MMA = 48;
 
 struct PrefillParams {
   const __nv_bfloat16* q; long long q_tok;              // heads follow each other; every token on a 16-byte boundary
@@ -123,10 +121,6 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
       "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-template <int N>
-__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N>
-__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 // Four codes as fp16 numbers times 2^-8, in the order (0, 2), (1, 3): the sign stays on top and the seven magnitude bits
 // move one place down, where e4m3's exponent is fp16's exponent minus 8 (subnormal codes become subnormal halves).  On
@@ -147,7 +141,7 @@ struct Shape {
 
 template <int D>
 __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const PrefillParams p) {
-  constexpr int TILE = Shape<D>::TILE, KSTEPS = D / 16;
+  constexpr int TILE = Shape<D>::TILE;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* s_q = smem;
@@ -179,8 +173,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
 
   // No role leaves its loops early when a wait gives up: later waits return at once, and all keep their barriers company.
   if (warp >= 12) {
-    regs_dec<REGS_MMA>();
-    if (warp == 12 && lane == 0) {
+    if (warp == 12 && elect_one()) {
       // -------------------------------- MMA issuer --------------------------------
       const uint32_t q_addr = smem_u32(s_q), kv_addr = smem_u32(s_kv);
       uint32_t n_item = 0, n_kv = 0, n_p = 0;     // running counts: items, fp16 tiles consumed, softmax steps
@@ -188,21 +181,23 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         mbar_wait(&kv_full[n % RING], (n / RING) & 1, abortp, p.err, CS_ERR_TIMEOUT_TMA);
         tc_fence_after();
       };
+      // (short loops: three roles run through their code in turn, and what does not stay in the instruction cache costs
+      // more than the loop does)
       auto issue_s = [&](int t, uint32_t n) {
-        const uint32_t a = q_addr + t * TILE, b = kv_addr + (n % RING) * TILE;
+        uint64_t a = umma_smem_desc(q_addr + t * TILE, 16, 1024), b = umma_smem_desc(kv_addr + (n % RING) * TILE, 16, 1024);
+#pragma unroll 1
+        for (int atom = 0; atom < D / 64; ++atom, a += ATOM / 16, b += ATOM / 16)
 #pragma unroll
-        for (int kk = 0; kk < KSTEPS; ++kk) {
-          const uint32_t off = (kk >> 2) * ATOM + (kk & 3) * 32;
-          umma_f16_ss(tmem + t * 128, umma_smem_desc(a + off, 16, 1024), umma_smem_desc(b + off, 16, 1024), p.idesc_s, kk != 0);
-        }
+          for (int kk = 0; kk < 4; ++kk) umma_f16_ss(tmem + t * 128, a + kk * 2, b + kk * 2, p.idesc_s, (atom | kk) != 0);
         umma_commit(&s_full[t]);
       };
       auto issue_pv = [&](int t, uint32_t n, bool first) {
-        const uint32_t b = kv_addr + (n % RING) * TILE;
+        uint64_t b = umma_smem_desc(kv_addr + (n % RING) * TILE, ATOM, 1024);
+        uint32_t a = tmem + t * 128;
+#pragma unroll 1
+        for (int k4 = 0; k4 < 2; ++k4, a += 32, b += 4 * 128)
 #pragma unroll
-        for (int kk = 0; kk < KV8_PAGE / 16; ++kk)
-          umma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, umma_smem_desc(b + kk * 2048, ATOM, 1024), p.idesc_pv,
-                      !(first && kk == 0));
+          for (int kk = 0; kk < 4; ++kk) umma_f16_ts(tmem + 256 + t * 128, a + kk * 8, b + kk * 128, p.idesc_pv, !(first && (k4 | kk) == 0));
       };
       for (int round = 0; round * static_cast<int>(gridDim.x) < p.total_items; ++round) {
         const int w = item_at(round);
@@ -220,7 +215,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
           const bool more = j + 1 < it.n;
           wait_kv(n_kv + 1);                       // V of this page
           if (more) wait_kv(n_kv + 2);             // K of the next
-#pragma unroll
+#pragma unroll 1
           for (int t = 0; t < 2; ++t) {
             mbar_wait(&p_full[t], n_p & 1, abortp, p.err, CS_ERR_TIMEOUT_EPI);
             tc_fence_after();
@@ -237,59 +232,43 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
     }
   } else if (warp >= 8) {
     // ------------------------------ operand preparation ------------------------------
-    regs_dec<REGS_PREP>();
     constexpr int CHUNKS = D / 16;                 // 16-byte chunks of codes per row
     constexpr int ITER = CHUNKS;                   // chunks per thread and tile (128 rows, 128 threads)
     const int tid = threadIdx.x - 256;
-    // Chunk `it` of this thread: the eight threads of a shared-memory phase write two rows of different parity, so that
-    // the swizzle sends their stores to different banks.
-    auto place = [&](int i, int& row, int& c) {
-      if (D == 128) {
-        const int g8 = (tid >> 3) & 3;
-        row = i * 16 + (tid >> 5) * 4 + (g8 >> 1) * 2 + ((tid >> 2) & 1);
-        c = (g8 & 1) * 4 + (tid & 3);
-      } else {
-        const int lin = i * 128 + tid;
-        row = lin >> 2;
-        c = lin & 3;
-      }
-    };
+    // This thread's chunks are chunk c0 of rows row0, row0 + STEP, ...  The eight threads of a shared-memory phase write
+    // two rows of different parity, so that the swizzle sends their stores to different banks.
+    constexpr int STEP = 128 / CHUNKS;
+    const int row0 = D == 128 ? (tid >> 5) * 4 + ((tid >> 4) & 1) * 2 + ((tid >> 2) & 1) : tid >> 2;
+    const int c0 = D == 128 ? ((tid >> 3) & 1) * 4 + (tid & 3) : tid & 3;
+    const int off_a = (c0 >> 2) * ATOM + row0 * 128 + ((((c0 & 3) * 2) ^ (row0 & 7)) << 4), off_b = off_a ^ 16;   // STEP is a multiple of 8
     uint32_t n_kv = 0, n_sc = 0, n_item = 0;
-    uint4 cur[ITER], nxt[ITER];
-    float ks = 0.f, vs = 0.f;                      // scales of key `tid` of the page in `cur` / `nxt`
-    // codes of keys (kv = 0) or values (kv = 1) of page j of an item
-    auto fetch = [&](const Item& it, int j, int kv, uint4 (&dst)[ITER], float& scale) {
-      int page = p.block_table[it.seq * p.bt_stride + j];
+    uint4 cur[ITER], nxt[ITER];                    // codes: tile in hand, next tile
+    float next_scale = 0.f;                        // scale of key `tid` of the next tile
+    // codes of the keys (kv = 0) or values (kv = 1) of page j of a sequence
+    auto fetch = [&](int seq, int hk, int j, int kv) {
+      int page = p.block_table[seq * p.bt_stride + j];
       if (page < 0 || page >= p.num_pages) {
         if (tid == 0) cs_set_error(p.err, CS_ERR_BAD_ARG);
         page = 0;
       }
-      const uint8_t* src = p.cache + ((static_cast<long long>(page) * 2 + kv) * p.Hkv + it.hk) * kv8_block_bytes(D);
+      const uint8_t* src = p.cache + ((static_cast<long long>(page) * 2 + kv) * p.Hkv + hk) * kv8_block_bytes(D);
 #pragma unroll
-      for (int i = 0; i < ITER; ++i) {
-        int row, c;
-        place(i, row, c);
-        dst[i] = __ldg(reinterpret_cast<const uint4*>(src + row * D + c * 16));
-      }
-      scale = __ldg(reinterpret_cast<const float*>(src + KV8_PAGE * D) + tid);
+      for (int i = 0; i < ITER; ++i) nxt[i] = __ldg(reinterpret_cast<const uint4*>(src + row0 * D + c0 * 16 + i * STEP * D));
+      next_scale = __ldg(reinterpret_cast<const float*>(src + KV8_PAGE * D) + tid);
     };
-    auto store = [&](const uint4 (&src)[ITER]) {
+    auto store = [&]() {
       const uint32_t slot = n_kv % RING;
       mbar_wait(&kv_empty[slot], ((n_kv / RING) & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
       uint8_t* tile = s_kv + slot * TILE;
 #pragma unroll
       for (int i = 0; i < ITER; ++i) {
-        int row, c;
-        place(i, row, c);
         uint4 a, b;
-        codes_to_half(src[i].x, a.x, a.y);
-        codes_to_half(src[i].y, a.z, a.w);
-        codes_to_half(src[i].z, b.x, b.y);
-        codes_to_half(src[i].w, b.z, b.w);
-        uint8_t* dst = tile + (c >> 2) * ATOM + row * 128;
-        const int ch = (c & 3) * 2;
-        *reinterpret_cast<uint4*>(dst + ((ch ^ (row & 7)) << 4)) = a;
-        *reinterpret_cast<uint4*>(dst + (((ch + 1) ^ (row & 7)) << 4)) = b;
+        codes_to_half(cur[i].x, a.x, a.y);
+        codes_to_half(cur[i].y, a.z, a.w);
+        codes_to_half(cur[i].z, b.x, b.y);
+        codes_to_half(cur[i].w, b.z, b.w);
+        *reinterpret_cast<uint4*>(tile + off_a + i * STEP * 128) = a;
+        *reinterpret_cast<uint4*>(tile + off_b + i * STEP * 128) = b;
       }
       fence_proxy_async_smem();
       mbar_arrive(&kv_full[slot]);
@@ -305,7 +284,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
     int round = next_item(0);
     if (round >= 0) {
       const Item first = get_item(p, item_at(round));
-      fetch(first, first.j0, 0, nxt, ks);
+      fetch(first.seq, first.hk, first.j0, 0);
     }
     while (round >= 0) {
       const Item it = get_item(p, item_at(round));
@@ -315,13 +294,14 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
       {
         uint32_t mx = 0;
         const __nv_bfloat16* src[2];
-#pragma unroll
+#pragma unroll 1
         for (int t = 0; t < 2; ++t) {
           const int tl = tid / group, g = tid - tl * group, tok = it.t0 + t * p.tok_per_tile + tl;
           const bool ok = tl < p.tok_per_tile && tok < it.q_len && g < it.n_heads;
           src[t] = ok ? p.q + (it.q_beg + tok) * p.q_tok + (it.h0 + g) * D : nullptr;
           if (!ok) continue;
           uint32_t m = 0;
+#pragma unroll 4
           for (int i = 0; i < D / 8; ++i) {
             const uint4 v = __ldg(reinterpret_cast<const uint4*>(src[t]) + i);
             const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -340,9 +320,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         cq = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + 8 - shift) << 23);   // 2^8: fp16 keys are code / 2^8
         mbar_wait(&q_empty, (n_item & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
         ++n_item;
-#pragma unroll
+#pragma unroll 1
         for (int t = 0; t < 2; ++t) {
           uint8_t* dst = s_q + t * TILE + tid * 128;
+#pragma unroll 4
           for (int i = 0; i < D / 8; ++i) {
             const uint4 v = src[t] != nullptr ? __ldg(reinterpret_cast<const uint4*>(src[t]) + i) : make_uint4(0, 0, 0, 0);
             uint4 h;   // channels in the order of the codes: (0, 2), (1, 3) of every four
@@ -357,34 +338,34 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         mbar_arrive(&q_full);
       }
       round = next_item(round + 1);
-      for (int j = 0; j < it.n; ++j) {
+#pragma unroll 1
+      for (int i = 0; i < 2 * it.n; ++i) {           // K and V of every page; the next tile is fetched while this one is converted
 #pragma unroll
-        for (int i = 0; i < ITER; ++i) cur[i] = nxt[i];
-        const float k_scale = ks;
-        fetch(it, it.j0 + j, 1, nxt, vs);            // V while K is converted
-        store(cur);
-        const uint32_t s = n_sc % SRING;
-        mbar_wait(&sc_empty[s], ((n_sc / SRING) & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
-        float* sc = s_scale + s * 3 * KV8_PAGE + tid;
-        const float v = vs < 1.2e-38f ? 1.2e-38f : vs;
-        sc[0] = k_scale * cq;
-        sc[KV8_PAGE] = __log2f(v);
-        sc[2 * KV8_PAGE] = 1.0f / v;
-        mbar_arrive(&sc_full[s]);
-        ++n_sc;
-#pragma unroll
-        for (int i = 0; i < ITER; ++i) cur[i] = nxt[i];
-        if (j + 1 < it.n) fetch(it, it.j0 + j + 1, 0, nxt, ks);
+        for (int k = 0; k < ITER; ++k) cur[k] = nxt[k];
+        const float scale = next_scale;
+        if (i + 1 < 2 * it.n) fetch(it.seq, it.hk, it.j0 + (i + 1) / 2, (i + 1) & 1);
         else if (round >= 0) {
           const Item after = get_item(p, item_at(round));
-          fetch(after, after.j0, 0, nxt, ks);
+          fetch(after.seq, after.hk, after.j0, 0);
         }
-        store(cur);
+        store();
+        // scale vectors of the page: the first goes with K, the others with V
+        const uint32_t s = n_sc % SRING;
+        float* sc = s_scale + s * 3 * KV8_PAGE + tid;
+        if ((i & 1) == 0) {
+          mbar_wait(&sc_empty[s], ((n_sc / SRING) & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
+          sc[0] = scale * cq;
+        } else {
+          const float v = scale < 1.2e-38f ? 1.2e-38f : scale;
+          sc[KV8_PAGE] = __log2f(v);
+          sc[2 * KV8_PAGE] = 1.0f / v;
+          mbar_arrive(&sc_full[s]);
+          ++n_sc;
+        }
       }
     }
   } else {
     // ---------------------------------- softmax -----------------------------------
-    regs_inc<REGS_SOFTMAX>();
     const int t = warp >> 2, r = (warp & 3) * 32 + lane;         // tile, row == TMEM lane
     const int tl = r / p.G, g = r - tl * p.G;                    // token in tile, head within group
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -405,89 +386,96 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         mbar_wait(&sc_full[s], (n_step / SRING) & 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
         mbar_wait(&s_full[t], n_step & 1, abortp, p.err, CS_ERR_TIMEOUT_MMA);
         tc_fence_after();
-        uint32_t x[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, x[c]);
-        tmem_wait_ld();
-        // t = s + log2 vs, in place
         const float* sc = s_scale + s * 3 * KV8_PAGE;
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
+        const int nvalid = lim - (it.j0 + j) * KV8_PAGE;       // visible keys of the page (may be negative or beyond 128)
+        // first pass: the largest s + log2 vs of the row
+        float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < KV8_PAGE; c += 32) {
+          uint32_t x[32];
+          tmem_ld32(tS + c, x);
+          tmem_wait_ld();
+          float y[32];
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
-            const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(sc + c * 32 + i);
-            const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(sc + KV8_PAGE + c * 32 + i);
-            float y0, y1;
-            unpack2(fma2(pack2(__uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1])), a.x, b.x), y0, y1);
-            x[c][i] = __float_as_uint(y0);
-            x[c][i + 1] = __float_as_uint(y1);
-            unpack2(fma2(pack2(__uint_as_float(x[c][i + 2]), __uint_as_float(x[c][i + 3])), a.y, b.y), y0, y1);
-            x[c][i + 2] = __float_as_uint(y0);
-            x[c][i + 3] = __float_as_uint(y1);
+            const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(sc + c + i);
+            const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(sc + KV8_PAGE + c + i);
+            unpack2(fma2(pack2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), a.x, b.x), y[i], y[i + 1]);
+            unpack2(fma2(pack2(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])), a.y, b.y), y[i + 2], y[i + 3]);
           }
-        const int nvalid = lim - (it.j0 + j) * KV8_PAGE;
-        if (nvalid < KV8_PAGE) {                     // hidden keys: whatever their scales were
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
+          if (nvalid < c + 32) {                     // hidden keys: whatever their scales were
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (c * 32 + i >= nvalid) x[c][i] = 0xff800000u;
-        }
-        float mx[4];
+              if (c + i >= nvalid) y[i] = -INFINITY;
+          }
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          mx[c] = __uint_as_float(x[c][0]);
-#pragma unroll
-          for (int i = 1; i < 32; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(x[c][i]));
+          for (int i = 0; i < 32; i += 4) {
+            mx0 = fmaxf(fmaxf(mx0, y[i]), y[i + 1]);
+            mx1 = fmaxf(fmaxf(mx1, y[i + 2]), y[i + 3]);
+          }
         }
-        const float mx_all = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        const float mx_all = fmaxf(mx0, mx1);
         // The reference m - 6 moves only when a weight would pass 2^14
         const float m_new = mx_all > m + 8.f ? mx_all : m;
-        const float alpha = ex2(m - m_new);
         if (__any_sync(0xffffffffu, m_new != m)) {   // tcgen05.ld / st are warp-wide: the warp decides together
+          const float alpha = ex2(m - m_new);
           float lo, hi;
           unpack2(l2, lo, hi);
           l2 = pack2(lo * alpha, hi * alpha);
           if (j > 0) {                               // PV of the last page is complete: S of this one was issued behind it
-#pragma unroll
-            for (int c = 0; c < D / 16; ++c) {
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
               uint32_t o[16];
-              tmem_ld16(tO + c * 16, o);
+              tmem_ld16(tO + c, o);
               tmem_wait_ld();
 #pragma unroll
               for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-              tmem_st16(tO + c * 16, o);
+              tmem_st16(tO + c, o);
             }
           }
         }
         m = m_new;
+        // second pass: weights, normaliser; the weights of 32 keys take 16 columns and stay behind the scores still to be read
         const uint64_t ref = pack2(6.f - m, 6.f - m);
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {       // 64 keys at a time: their weights go straight to TMEM
-          uint32_t pk[32];
-#pragma unroll
-          for (int cc = 0; cc < 2; ++cc)
+#pragma unroll 1
+        for (int c = 0; c < KV8_PAGE; c += 32) {
+          uint32_t x[32];
+          tmem_ld32(tS + c, x);
+          tmem_wait_ld();
+          uint32_t pk[16];
+          if (nvalid >= c + 32) {
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
-              const int c = half * 2 + cc, k = c * 32 + i;
-              ulonglong2 iv = *reinterpret_cast<const ulonglong2*>(sc + 2 * KV8_PAGE + k);
+              const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(sc + c + i);
+              const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(sc + KV8_PAGE + c + i);
+              const ulonglong2 iv = *reinterpret_cast<const ulonglong2*>(sc + 2 * KV8_PAGE + c + i);
               float e0, e1, e2, e3;
-              unpack2(add2(pack2(__uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1])), ref), e0, e1);
-              unpack2(add2(pack2(__uint_as_float(x[c][i + 2]), __uint_as_float(x[c][i + 3])), ref), e2, e3);
+              unpack2(fma2(pack2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), a.x, add2(b.x, ref)), e0, e1);
+              unpack2(fma2(pack2(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])), a.y, add2(b.y, ref)), e2, e3);
               e0 = ex2(e0); e1 = ex2(e1); e2 = ex2(e2); e3 = ex2(e3);
-              if (nvalid < KV8_PAGE) {               // 0 / vs of a hidden key may not be 0
-                float i0, i1, i2, i3;
-                unpack2(iv.x, i0, i1);
-                unpack2(iv.y, i2, i3);
-                iv.x = pack2(k < nvalid ? i0 : 0.f, k + 1 < nvalid ? i1 : 0.f);
-                iv.y = pack2(k + 2 < nvalid ? i2 : 0.f, k + 3 < nvalid ? i3 : 0.f);
-              }
               l2 = fma2(pack2(e0, e1), iv.x, l2);
               l2 = fma2(pack2(e2, e3), iv.y, l2);
-              pk[cc * 16 + (i >> 1)] = half2_bits(e0, e1);
-              pk[cc * 16 + (i >> 1) + 1] = half2_bits(e2, e3);
+              pk[i >> 1] = half2_bits(e0, e1);
+              pk[(i >> 1) + 1] = half2_bits(e2, e3);
             }
-          tmem_st32(tS + half * 32, pk);
+          } else {                                   // the row ends in (or before) these keys
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              float e[2];
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const float* f = sc + c + i + k;
+                e[k] = 0.f;
+                if (c + i + k < nvalid) {
+                  e[k] = ex2(__uint_as_float(x[i + k]) * f[0] + (f[KV8_PAGE] + (6.f - m)));
+                  l2 = fma2(pack2(e[k], 0.f), pack2(f[2 * KV8_PAGE], 0.f), l2);
+                }
+              }
+              pk[i >> 1] = half2_bits(e[0], e[1]);
+            }
+          }
+          __syncwarp();
+          tmem_st16(tS + (c >> 1), pk);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&sc_empty[s]);
@@ -512,7 +500,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
       const float inv = p.splits > 1 ? 256.f : (l == 0.f ? 0.f : 256.f / l);          // 2^8: fp16 values are code / 2^8
       __nv_bfloat16* dst = p.o + static_cast<long long>(it.q_beg + tok) * p.o_tok + (it.h0 + g) * p.o_head;
       float* part = p.splits > 1 ? p.ws_o + (row * p.splits + it.split) * D : nullptr;
-#pragma unroll
+#pragma unroll 1
       for (int c = 0; c < D / 16; ++c) {
         uint32_t o[16];
         if (it.n > 0) {
@@ -589,10 +577,6 @@ int launch_prefill(const PrefillParams& p, int grid, long long rows, cudaStream_
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -10;
   if (!ready[dev]) {
-    // the register split after setmaxnreg must fit what the block is launched with
-    cudaFuncAttributes a{};
-    if (cudaFuncGetAttributes(&a, attention_prefill_fp8_kernel<D>) != cudaSuccess) return -10;
-    if (a.numRegs * THREADS < 256 * REGS_SOFTMAX + 128 * REGS_PREP + 128 * REGS_MMA) return -6;
     if (cudaFuncSetAttribute(attention_prefill_fp8_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::SMEM) != cudaSuccess)
       return -10;
     ready[dev] = true;
