@@ -1,26 +1,28 @@
 // Attention of packed prompts (or chunks of them) over the 8-bit paged key-value cache (layout in kv_fp8.cuh):
 //
-//   o_i = sum_j w_ij vc_j / sum_j w_ij / vs_j,   w_ij = 2^(s_ij + log2 vs_j - M_i),   s_ij = scale * log2(e) * ks_j * (q_i . kc_j)
+//   o_i = sum_j w_ij V_j / sum_j w_ij 2^-F_j,   w_ij = 2^(s_ij + F_j - M_i),   s_ij = scale * log2(e) * 2^E_j * (q_i . K_j)
 //
-// over the keys j that query i sees (all, or those up to its own position), with the e4m3 codes kc, vc and the scales
-// ks, vs of the cache.  Codes are exact in fp16, so both products run as fp16 tcgen05.mma on the codes themselves; the
-// scales enter in fp32, as one fused multiply-add per score on the way into the exponential and one into the normaliser.
-// M_i follows the largest weight (not the largest score), so weights fit fp16 whatever the value scales are.  Queries
-// become fp16 too, scaled by a power of two that is common to a tile pair (exact for every element within 2^-38 of the
-// pair's largest).
+// over the keys j that query i sees (all, or those up to its own position).  K_j = kc_j ks_j 2^-E and V_j = vc_j vs_j 2^-F
+// are the cached rows (e4m3 codes times the fp32 scale of the row) in fp16, with one power of two per page that brings the
+// page's largest scale to the top of fp16's range: code times scale is rounded once, to 11 bits, and the page's factors
+// enter in fp32 as scalars.  (Scales could stay exact as a vector over the keys that the softmax applies, but every row's
+// thread would have to read it from shared memory: 3 x 128 values per row and page made that the slowest part, at 8400
+// cycles a page and tile pair.)  M_i follows the largest weight, not the largest score, so weights fit fp16 whatever the
+// value scales are.  Queries become fp16 too, scaled by a power of two common to a tile pair (exact for every element
+// within 2^-38 of the pair's largest).
 //
 // One CTA works on 2 x 128 query rows of one sequence and one key head (rows = tokens x the query heads that share the
 // key head) against pages of 128 keys:
 //   warps 0-3, 4-7 : softmax of tile 0 / tile 1, one thread per row; scores come from TMEM, weights go back to TMEM over
 //                    them and are the A operand of the second product there
-//   warps 8-11     : operand preparation: e4m3 codes from global memory through registers to fp16 tiles in shared memory
-//                    (128-byte swizzle), the scale vectors of a page, the queries of an item
+//   warps 8-11     : operand preparation: codes and scales from global memory through registers to fp16 tiles in shared
+//                    memory (128-byte swizzle), the queries of an item
 //   warp 12        : issues tcgen05.mma: S_t = Q_t K^T (t = 0, 1) and O_t += P_t V.  While one tile's softmax runs, the
 //                    tensor cores work for the other.
 // The codes are converted once per 256 query rows.  They are not staged in shared memory as bytes: its bandwidth is what
-// this kernel has least of (192 KB of operands per page and tile pair for the products alone), so the preparation warps
-// load them straight into registers, a tile ahead.  Few items (short chunks over a long cache) split the pages of an item
-// over several CTAs and a second kernel joins the parts.
+// the products need most of (192 KB of operands per page and tile pair), so the preparation warps load them straight into
+// registers, a tile ahead.  Few items (short chunks over a long cache) split the pages of an item over several CTAs and a
+// second kernel joins the parts.
 #include <math.h>
 
 #include "kv_fp8.cuh"
@@ -29,7 +31,7 @@ namespace {
 
 constexpr int ATOM = 128 * 128;            // 128 rows x 64 fp16, 128-byte swizzle
 constexpr int RING = 4;                    // fp16 tiles (K0 V0 K1 V1 ...)
-constexpr int SRING = 4;                   // scale vectors of a page
+constexpr int SRING = 4;                   // the two scalars of a page
 constexpr int THREADS = 13 * 32;
 constexpr float M_NONE = -3.0e38f;         // running maximum before the first key (finite: differences stay defined)
 
@@ -131,12 +133,12 @@ __device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& r02, uint32_
   r02 = (e & 0x80008000u) | ((e >> 1) & 0x3f803f80u);
 }
 
-// Shared memory: queries (two tiles), ring of fp16 tiles, scale vectors.
+// Shared memory: queries (two tiles), ring of fp16 tiles.
 template <int D>
 struct Shape {
   static constexpr int ATOMS = D / 64, TILE = ATOMS * ATOM;
-  static constexpr int Q = 2 * TILE, SCALES = SRING * 3 * KV8_PAGE * 4;
-  static constexpr int SMEM = 1024 + Q + RING * TILE + SCALES;
+  static constexpr int Q = 2 * TILE;
+  static constexpr int SMEM = 1024 + Q + RING * TILE;
 };
 
 template <int D>
@@ -146,11 +148,11 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* s_q = smem;
   uint8_t* s_kv = smem + Shape<D>::Q;
-  float* s_scale = reinterpret_cast<float*>(s_kv + RING * TILE);      // [SRING][a, log2 vs, 1 / vs][128]
   __shared__ uint64_t q_full, q_empty, kv_full[RING], kv_empty[RING], sc_full[SRING], sc_empty[SRING], s_full[2], p_full[2], o_full[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   __shared__ uint32_t s_max[4];
+  __shared__ float2 s_scale[SRING];     // of a page: factor from S to base-2 exponents, F
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -158,7 +160,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
     mbar_init(&q_full, 128);
     mbar_init(&q_empty, 1);
     for (int i = 0; i < RING; ++i) { mbar_init(&kv_full[i], 128); mbar_init(&kv_empty[i], 1); }
-    for (int i = 0; i < SRING; ++i) { mbar_init(&sc_full[i], 128); mbar_init(&sc_empty[i], 8); }
+    for (int i = 0; i < SRING; ++i) { mbar_init(&sc_full[i], 1); mbar_init(&sc_empty[i], 8); }
     for (int t = 0; t < 2; ++t) { mbar_init(&s_full[t], 1); mbar_init(&p_full[t], 128); mbar_init(&o_full[t], 1); }
     mbar_fence_init();
   }
@@ -243,32 +245,84 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
     const int off_a = (c0 >> 2) * ATOM + row0 * 128 + ((((c0 & 3) * 2) ^ (row0 & 7)) << 4), off_b = off_a ^ 16;   // STEP is a multiple of 8
     uint32_t n_kv = 0, n_sc = 0, n_item = 0;
     uint4 cur[ITER], nxt[ITER];                    // codes: tile in hand, next tile
-    float next_scale = 0.f;                        // scale of key `tid` of the next tile
-    // codes of the keys (kv = 0) or values (kv = 1) of page j of a sequence
-    auto fetch = [&](int seq, int hk, int j, int kv) {
-      int page = p.block_table[seq * p.bt_stride + j];
+    float row_s[ITER];                             // next tile: scales of this thread's rows
+    float4 all_s, val_s;                           // next tile: scales of keys 4 lane .. + 3; with keys those of the values too
+    const float* val_src = nullptr;
+    int rows = 0;                                  // next tile: rows that are keys of the sequence (may exceed 128)
+    // codes and scales of the keys (kv = 0) or values (kv = 1) of page j of a sequence
+    auto fetch = [&](const Item& it, int j, int kv) {
+      int page = p.block_table[it.seq * p.bt_stride + j];
       if (page < 0 || page >= p.num_pages) {
         if (tid == 0) cs_set_error(p.err, CS_ERR_BAD_ARG);
         page = 0;
       }
-      const uint8_t* src = p.cache + ((static_cast<long long>(page) * 2 + kv) * p.Hkv + hk) * kv8_block_bytes(D);
+      const uint8_t* src = p.cache + ((static_cast<long long>(page) * 2 + kv) * p.Hkv + it.hk) * kv8_block_bytes(D);
+      const float* scales = reinterpret_cast<const float*>(src + KV8_PAGE * D);
 #pragma unroll
       for (int i = 0; i < ITER; ++i) nxt[i] = __ldg(reinterpret_cast<const uint4*>(src + row0 * D + c0 * 16 + i * STEP * D));
-      next_scale = __ldg(reinterpret_cast<const float*>(src + KV8_PAGE * D) + tid);
+#pragma unroll
+      for (int i = 0; i < ITER; ++i) row_s[i] = __ldg(scales + row0 + i * STEP);
+      all_s = __ldg(reinterpret_cast<const float4*>(scales) + lane);
+      rows = it.k_len - j * KV8_PAGE;
+      if (kv == 0) {
+        val_src = reinterpret_cast<const float*>(src + p.Hkv * kv8_block_bytes(D) + KV8_PAGE * D);
+        val_s = __ldg(reinterpret_cast<const float4*>(val_src) + lane);
+      }
     };
-    auto store = [&]() {
+    auto finite_bits = [](float f) { const uint32_t b = __float_as_uint(f) & 0x7fffffffu; return b < 0x7f800000u ? b : 0u; };
+    auto is_finite = [](float f) { return (__float_as_uint(f) & 0x7fffffffu) < 0x7f800000u; };
+    // Multipliers of this thread's rows as fp16 pairs (upper and lower part), and the exponent E (or F) of the page.  Rows
+    // behind the sequence's keys become 0, whatever is there.  A key row or value row with a scale that is no number makes
+    // the key a NaN, so that queries that see it, and only those, become NaN; in V such a row is 0 (0 * NaN is not 0).
+    auto multipliers = [&](int kv, uint32_t (&hi)[ITER], uint32_t (&lo)[ITER]) {
+      const float a4[4] = {all_s.x, all_s.y, all_s.z, all_s.w};
+      uint32_t mx = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) mx = max(mx, lane * 4 + k < rows ? finite_bits(a4[k]) : 0u);
+      mx = __reduce_max_sync(0xffffffffu, mx);
+      const int e = min(max(static_cast<int>(mx >> 23) - 127 - 13, -110), 120);     // the largest scale into [2^13, 2^14)
+      const float f = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+      bool bad = false;
+      if (kv == 0) {
+        const float v4[4] = {val_s.x, val_s.y, val_s.z, val_s.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) bad |= lane * 4 + k < rows && !is_finite(v4[k]);
+        bad = __any_sync(0xffffffffu, bad);
+      }
+#pragma unroll
+      for (int i = 0; i < ITER; ++i) {
+        const int row = row0 + i * STEP;
+        float v = row_s[i] * f;
+        if (kv == 1 && !is_finite(row_s[i])) v = 0.f;
+        if (bad && row < rows && !is_finite(__ldg(val_src + row))) v = __uint_as_float(0x7fffffffu);
+        if (row >= rows) v = 0.f;
+        const __half h = __float2half_rn(v), r = __float2half_rn(v - __half2float(h));
+        hi[i] = __half_as_ushort(h) * 0x10001u;
+        lo[i] = __half_as_ushort(r) * 0x10001u;
+      }
+      return e;
+    };
+    auto scaled = [](uint32_t c, uint32_t hi, uint32_t lo) {      // c * (hi + lo), rounded once
+      const __half2 x = *reinterpret_cast<const __half2*>(&c), h = *reinterpret_cast<const __half2*>(&hi), l = *reinterpret_cast<const __half2*>(&lo);
+      const __half2 y = __hfma2(x, h, __hmul2(x, l));
+      return *reinterpret_cast<const uint32_t*>(&y);
+    };
+    auto store = [&](const uint32_t (&hi)[ITER], const uint32_t (&lo)[ITER]) {
       const uint32_t slot = n_kv % RING;
       mbar_wait(&kv_empty[slot], ((n_kv / RING) & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
       uint8_t* tile = s_kv + slot * TILE;
 #pragma unroll
       for (int i = 0; i < ITER; ++i) {
-        uint4 a, b;
-        codes_to_half(cur[i].x, a.x, a.y);
-        codes_to_half(cur[i].y, a.z, a.w);
-        codes_to_half(cur[i].z, b.x, b.y);
-        codes_to_half(cur[i].w, b.z, b.w);
-        *reinterpret_cast<uint4*>(tile + off_a + i * STEP * 128) = a;
-        *reinterpret_cast<uint4*>(tile + off_b + i * STEP * 128) = b;
+        const uint32_t w[4] = {cur[i].x, cur[i].y, cur[i].z, cur[i].w};
+        uint32_t h[8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          codes_to_half(w[k], h[2 * k], h[2 * k + 1]);
+          h[2 * k] = scaled(h[2 * k], hi[i], lo[i]);
+          h[2 * k + 1] = scaled(h[2 * k + 1], hi[i], lo[i]);
+        }
+        *reinterpret_cast<uint4*>(tile + off_a + i * STEP * 128) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(tile + off_b + i * STEP * 128) = make_uint4(h[4], h[5], h[6], h[7]);
       }
       fence_proxy_async_smem();
       mbar_arrive(&kv_full[slot]);
@@ -284,7 +338,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
     int round = next_item(0);
     if (round >= 0) {
       const Item first = get_item(p, item_at(round));
-      fetch(first.seq, first.hk, first.j0, 0);
+      fetch(first, first.j0, 0);
     }
     while (round >= 0) {
       const Item it = get_item(p, item_at(round));
@@ -316,8 +370,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         mx = max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3]));
         asm volatile("bar.sync 1, 128;" ::: "memory");
         const int shift = min(max(127 + 14 - static_cast<int>(mx >> 7), -110), 110);   // the largest element into [2^14, 2^15)
-        const float up = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
-        cq = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + 8 - shift) << 23);   // 2^8: fp16 keys are code / 2^8
+        // a negative scale turns the queries around, so that the largest score is the largest S
+        const float up = copysignf(__uint_as_float(static_cast<uint32_t>(127 + shift) << 23), p.scale_log2);
+        cq = fabsf(p.scale_log2) * __uint_as_float(static_cast<uint32_t>(127 + 8 - shift) << 23);   // 2^8: codes_to_half gives code / 2^8
         mbar_wait(&q_empty, (n_item & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
         ++n_item;
 #pragma unroll 1
@@ -338,27 +393,26 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         mbar_arrive(&q_full);
       }
       round = next_item(round + 1);
+      int e_k = 0;
 #pragma unroll 1
       for (int i = 0; i < 2 * it.n; ++i) {           // K and V of every page; the next tile is fetched while this one is converted
 #pragma unroll
         for (int k = 0; k < ITER; ++k) cur[k] = nxt[k];
-        const float scale = next_scale;
-        if (i + 1 < 2 * it.n) fetch(it.seq, it.hk, it.j0 + (i + 1) / 2, (i + 1) & 1);
+        uint32_t hi[ITER], lo[ITER];
+        const int e = multipliers(i & 1, hi, lo);
+        if (i + 1 < 2 * it.n) fetch(it, it.j0 + (i + 1) / 2, (i + 1) & 1);
         else if (round >= 0) {
           const Item after = get_item(p, item_at(round));
-          fetch(after.seq, after.hk, after.j0, 0);
+          fetch(after, after.j0, 0);
         }
-        store();
-        // scale vectors of the page: the first goes with K, the others with V
-        const uint32_t s = n_sc % SRING;
-        float* sc = s_scale + s * 3 * KV8_PAGE + tid;
+        store(hi, lo);
         if ((i & 1) == 0) {
+          e_k = e;
+        } else if (tid == 0) {
+          const uint32_t s = n_sc % SRING;
           mbar_wait(&sc_empty[s], ((n_sc / SRING) & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
-          sc[0] = scale * cq;
-        } else {
-          const float v = scale < 1.2e-38f ? 1.2e-38f : scale;
-          sc[KV8_PAGE] = __log2f(v);
-          sc[2 * KV8_PAGE] = 1.0f / v;
+          // (not 0, also for a scale of 0: a hidden key's -inf times the factor has to stay -inf)
+          s_scale[s] = make_float2(fmaxf(cq * __uint_as_float(static_cast<uint32_t>(127 + e_k) << 23), 1e-37f), static_cast<float>(e));
           mbar_arrive(&sc_full[s]);
           ++n_sc;
         }
@@ -380,48 +434,40 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
       const bool row_ok = tl < p.tok_per_tile && tok < it.q_len && g < it.n_heads;
       const int lim = p.causal ? min(it.k_len, tok + it.shift + 1) : it.k_len;     // keys [0, lim) are visible
       float m = M_NONE;
-      uint64_t l2 = pack2(0.f, 0.f);
+      float l = 0.f;
       for (int j = 0; j < it.n; ++j, ++n_step) {
         const uint32_t s = n_step % SRING;
         mbar_wait(&sc_full[s], (n_step / SRING) & 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
         mbar_wait(&s_full[t], n_step & 1, abortp, p.err, CS_ERR_TIMEOUT_MMA);
         tc_fence_after();
-        const float* sc = s_scale + s * 3 * KV8_PAGE;
+        const float2 sc = s_scale[s];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sc_empty[s]);
         const int nvalid = lim - (it.j0 + j) * KV8_PAGE;       // visible keys of the page (may be negative or beyond 128)
-        // first pass: the largest s + log2 vs of the row
+        // first pass: the largest S of the row
         float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll 1
         for (int c = 0; c < KV8_PAGE; c += 32) {
           uint32_t x[32];
           tmem_ld32(tS + c, x);
           tmem_wait_ld();
-          float y[32];
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(sc + c + i);
-            const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(sc + KV8_PAGE + c + i);
-            unpack2(fma2(pack2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), a.x, b.x), y[i], y[i + 1]);
-            unpack2(fma2(pack2(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])), a.y, b.y), y[i + 2], y[i + 3]);
-          }
-          if (nvalid < c + 32) {                     // hidden keys: whatever their scales were
+          if (nvalid < c + 32) {                     // hidden keys: whatever is there
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (c + i >= nvalid) y[i] = -INFINITY;
+              if (c + i >= nvalid) x[i] = 0xff800000u;
           }
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
-            mx0 = fmaxf(fmaxf(mx0, y[i]), y[i + 1]);
-            mx1 = fmaxf(fmaxf(mx1, y[i + 2]), y[i + 3]);
+            mx0 = fmaxf(fmaxf(mx0, __uint_as_float(x[i])), __uint_as_float(x[i + 1]));
+            mx1 = fmaxf(fmaxf(mx1, __uint_as_float(x[i + 2])), __uint_as_float(x[i + 3]));
           }
         }
-        const float mx_all = fmaxf(mx0, mx1);
+        const float mx = fmaxf(mx0, mx1) * sc.x + sc.y;
         // The reference m - 6 moves only when a weight would pass 2^14
-        const float m_new = mx_all > m + 8.f ? mx_all : m;
+        const float m_new = mx > m + 8.f ? mx : m;
         if (__any_sync(0xffffffffu, m_new != m)) {   // tcgen05.ld / st are warp-wide: the warp decides together
           const float alpha = ex2(m - m_new);
-          float lo, hi;
-          unpack2(l2, lo, hi);
-          l2 = pack2(lo * alpha, hi * alpha);
+          l *= alpha;
           if (j > 0) {                               // PV of the last page is complete: S of this one was issued behind it
 #pragma unroll 1
             for (int c = 0; c < D; c += 16) {
@@ -435,50 +481,40 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
           }
         }
         m = m_new;
-        // second pass: weights, normaliser; the weights of 32 keys take 16 columns and stay behind the scores still to be read
-        const uint64_t ref = pack2(6.f - m, 6.f - m);
+        // second pass: weights and their sum; the weights of 32 keys take 16 columns and stay behind the scores still to be read
+        const float add = sc.y + (6.f - m);
+        const uint64_t mul2 = pack2(sc.x, sc.x), ref2 = pack2(add, add);
+        uint64_t sum_a = pack2(0.f, 0.f), sum_b = sum_a;
 #pragma unroll 1
         for (int c = 0; c < KV8_PAGE; c += 32) {
           uint32_t x[32];
           tmem_ld32(tS + c, x);
           tmem_wait_ld();
+          if (nvalid < c + 32) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (c + i >= nvalid) x[i] = 0xff800000u;
+          }
           uint32_t pk[16];
-          if (nvalid >= c + 32) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(sc + c + i);
-              const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(sc + KV8_PAGE + c + i);
-              const ulonglong2 iv = *reinterpret_cast<const ulonglong2*>(sc + 2 * KV8_PAGE + c + i);
-              float e0, e1, e2, e3;
-              unpack2(fma2(pack2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), a.x, add2(b.x, ref)), e0, e1);
-              unpack2(fma2(pack2(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])), a.y, add2(b.y, ref)), e2, e3);
-              e0 = ex2(e0); e1 = ex2(e1); e2 = ex2(e2); e3 = ex2(e3);
-              l2 = fma2(pack2(e0, e1), iv.x, l2);
-              l2 = fma2(pack2(e2, e3), iv.y, l2);
-              pk[i >> 1] = half2_bits(e0, e1);
-              pk[(i >> 1) + 1] = half2_bits(e2, e3);
-            }
-          } else {                                   // the row ends in (or before) these keys
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              float e[2];
-#pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                const float* f = sc + c + i + k;
-                e[k] = 0.f;
-                if (c + i + k < nvalid) {
-                  e[k] = ex2(__uint_as_float(x[i + k]) * f[0] + (f[KV8_PAGE] + (6.f - m)));
-                  l2 = fma2(pack2(e[k], 0.f), pack2(f[2 * KV8_PAGE], 0.f), l2);
-                }
-              }
-              pk[i >> 1] = half2_bits(e[0], e[1]);
-            }
+          for (int i = 0; i < 32; i += 4) {
+            float e0, e1, e2, e3;
+            unpack2(fma2(pack2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), mul2, ref2), e0, e1);
+            unpack2(fma2(pack2(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])), mul2, ref2), e2, e3);
+            e0 = ex2(e0); e1 = ex2(e1); e2 = ex2(e2); e3 = ex2(e3);
+            sum_a = add2(sum_a, pack2(e0, e1));
+            sum_b = add2(sum_b, pack2(e2, e3));
+            pk[i >> 1] = half2_bits(e0, e1);
+            pk[(i >> 1) + 1] = half2_bits(e2, e3);
           }
           __syncwarp();
           tmem_st16(tS + (c >> 1), pk);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sc_empty[s]);
+        {
+          float s0, s1;
+          unpack2(add2(sum_a, sum_b), s0, s1);
+          l += (s0 + s1) * ex2(-sc.y);
+        }
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&p_full[t]);
@@ -489,15 +525,12 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         ++n_item;
         tc_fence_after();
       }
-      float l_lo, l_hi;
-      unpack2(l2, l_lo, l_hi);
-      const float l = l_lo + l_hi;
       const long long row = static_cast<long long>(it.q_beg + tok) * p.Hq + it.h0 + g;
       if (p.splits > 1 && row_ok) {
         p.ws_ml[(row * p.splits + it.split) * 2] = m;
         p.ws_ml[(row * p.splits + it.split) * 2 + 1] = l;
       }
-      const float inv = p.splits > 1 ? 256.f : (l == 0.f ? 0.f : 256.f / l);          // 2^8: fp16 values are code / 2^8
+      const float inv = p.splits > 1 ? 256.f : (l == 0.f ? 0.f : 256.f / l);          // 2^8: codes_to_half gives code / 2^8
       __nv_bfloat16* dst = p.o + static_cast<long long>(it.q_beg + tok) * p.o_tok + (it.h0 + g) * p.o_head;
       float* part = p.splits > 1 ? p.ws_o + (row * p.splits + it.split) * D : nullptr;
 #pragma unroll 1

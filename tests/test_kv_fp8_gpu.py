@@ -3,7 +3,10 @@
 Tolerances.  A stored code is off by at most half a step of e4m3: 2^-4 of the value, 2^-10 among the subnormal codes.  A
 bf16 output is off by 2^-8 of its value.  Inside the attention a key's weight (probability times value scale) may be rounded
 to fp16: off by 2^-11 of it, or by half a step of the subnormals, 2^-25, where the largest weight is at least 2^6; so by
-2^-31 of the largest, for every code of the row.  Scores are fp32 sums whose error is at most (d + 4) * 2^-24 times the sum of the magnitudes of
+2^-31 of the largest, for every code of the row.  With more than one query per sequence the keys and values themselves
+(code times scale) are rounded to fp16 once: off by 2^-11 of them, or by half a step of the subnormals, which is 2^-30 of
+the largest scale of their page (a power of two brings that scale to at least 2^13 when a code stands for code / 2^8).
+Scores are fp32 sums whose error is at most (d + 4) * 2^-24 times the sum of the magnitudes of
 their products, and an error e of a score changes its probability, and at most as much the normaliser, by e.
 """
 
@@ -192,10 +195,22 @@ def _check(out, q, cache, table, lens, new, causal=True, scale=None):
         p = torch.softmax(s.masked_fill(~vis, float("-inf")), -1).masked_fill(dead[:, None], 0.0)
         want = torch.einsum("hqk,khd->qhd", p, v)
         size = torch.einsum("hqk,khd->qhd", p, v.abs())
-        es = (mag.masked_fill(~vis, 0.0).amax(-1) * (d + 4) * 2.0 ** -24).transpose(0, 1)[..., None] if L else 0.0
+        prompt = max(new) > 1
+        es = mag * ((d + 4) * 2.0 ** -24 + (2.0 ** -11 if prompt else 0.0))
+        tiny_v = 0.0
+        if prompt and L:
+            ks_top, vs_top = (scales[ids, j].nan_to_num(0.0, 0.0, 0.0).double().masked_fill(
+                torch.arange(ids.numel() * 128, device=DEV).view(-1, 1, 128) >= L, 0.0).amax(-1).repeat_interleave(128, dim=0)[:L]
+                .repeat_interleave(group, dim=1) for j in (0, 1))                       # [keys, Hq]
+            es = es + torch.einsum("qh,kh->hqk", qq.abs().sum(-1), ks_top) * abs(scale) * 2.0 ** -30
+            tiny_v = torch.einsum("hqk,kh->qh", p, vs_top)[..., None] * 2.0 ** -30
+            # here a key's weight is its probability times a power of two within a factor of two of its page's largest value
+            # scale (up to a constant), so the step of the smallest weights is at most 2^-30 of the largest such product
+            vs = vs_top.clamp_min(1e-30)
+        es = es.masked_fill(~vis, 0.0).amax(-1).transpose(0, 1)[..., None] if L else 0.0
         top = (p * vs.t()[:, None, :]).amax(-1).transpose(0, 1)[..., None] if L else 0.0     # the largest weight of a row
         code_sum = torch.einsum("qk,khd->qhd", vis.double(), (v / vs[..., None]).abs()) if L else 0.0
-        tol = want.abs() * 2.0 ** -8 + size * (2.0 ** -11 + 2 * es + 2.0 ** -18) + top * code_sum * 2.0 ** -31
+        tol = want.abs() * 2.0 ** -8 + size * (2.0 ** -11 + (2.0 ** -11 if prompt else 0.0) + 2 * es + 2.0 ** -18) + top * code_sum * 2.0 ** (-30 if prompt else -31) + tiny_v
         assert not got[dead].any()
         err = (got - want).abs()
         assert (err <= tol).all(), f"sequence {i}: {n} of {L} keys, error {err.max().item():.3g} beyond tolerance by {(err - tol).max().item():.3g}"
