@@ -15,13 +15,13 @@
 // key head) against pages of 128 keys:
 //   warps 0-3, 4-7 : softmax of tile 0 / tile 1, one thread per row; scores come from TMEM, weights go back to TMEM over
 //                    them and are the A operand of the second product there
-//   warps 8-11     : operand preparation: codes and scales from global memory through registers to fp16 tiles in shared
-//                    memory (128-byte swizzle), the queries of an item
-//   warp 12        : issues tcgen05.mma: S_t = Q_t K^T (t = 0, 1) and O_t += P_t V.  While one tile's softmax runs, the
+//   warps 8-11, 12-15 : operand preparation, K tiles (and the queries of an item) / V tiles: codes and scales from global
+//                    memory through registers to fp16 tiles in shared memory (128-byte swizzle)
+//   warp 16        : issues tcgen05.mma: S_t = Q_t K^T (t = 0, 1) and O_t += P_t V.  While one tile's softmax runs, the
 //                    tensor cores work for the other.
 // The codes are converted once per 256 query rows.  They are not staged in shared memory as bytes: its bandwidth is what
 // the products need most of (192 KB of operands per page and tile pair), so the preparation warps load them straight into
-// registers, a tile ahead.  Few items (short chunks over a long cache) split the pages of an item over several CTAs and a
+// registers.  Few items (short chunks over a long cache) split the pages of an item over several CTAs and a
 // second kernel joins the parts.
 #include <math.h>
 
@@ -30,9 +30,9 @@
 namespace {
 
 constexpr int ATOM = 128 * 128;            // 128 rows x 64 fp16, 128-byte swizzle
-constexpr int RING = 4;                    // fp16 tiles (K0 V0 K1 V1 ...)
+constexpr int RING = 2;                    // fp16 tiles of K and of V
 constexpr int SRING = 4;                   // the two scalars of a page
-constexpr int THREADS = 13 * 32;
+constexpr int THREADS = 17 * 32;
 constexpr float M_NONE = -3.0e38f;         // running maximum before the first key (finite: differences stay defined)
 
 struct PrefillParams {
@@ -138,7 +138,7 @@ template <int D>
 struct Shape {
   static constexpr int ATOMS = D / 64, TILE = ATOMS * ATOM;
   static constexpr int Q = 2 * TILE;
-  static constexpr int SMEM = 1024 + Q + RING * TILE;
+  static constexpr int SMEM = 1024 + Q + 2 * RING * TILE;
 };
 
 template <int D>
@@ -147,8 +147,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* s_q = smem;
-  uint8_t* s_kv = smem + Shape<D>::Q;
-  __shared__ uint64_t q_full, q_empty, kv_full[RING], kv_empty[RING], sc_full[SRING], sc_empty[SRING], s_full[2], p_full[2], o_full[2];
+  uint8_t* s_kv = smem + Shape<D>::Q;    // K tiles, V tiles
+  __shared__ uint64_t q_full, q_empty, kv_full[2][RING], kv_empty[2][RING], sc_full[SRING], sc_empty[SRING], s_full[2], p_full[2], o_full[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   __shared__ uint32_t s_max[4];
@@ -159,12 +159,12 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
     abort_flag = 0;
     mbar_init(&q_full, 128);
     mbar_init(&q_empty, 1);
-    for (int i = 0; i < RING; ++i) { mbar_init(&kv_full[i], 128); mbar_init(&kv_empty[i], 1); }
-    for (int i = 0; i < SRING; ++i) { mbar_init(&sc_full[i], 1); mbar_init(&sc_empty[i], 8); }
+    for (int i = 0; i < 2 * RING; ++i) { mbar_init(&kv_full[i / RING][i % RING], 128); mbar_init(&kv_empty[i / RING][i % RING], 1); }
+    for (int i = 0; i < SRING; ++i) { mbar_init(&sc_full[i], 2); mbar_init(&sc_empty[i], 8); }
     for (int t = 0; t < 2; ++t) { mbar_init(&s_full[t], 1); mbar_init(&p_full[t], 128); mbar_init(&o_full[t], 1); }
     mbar_fence_init();
   }
-  if (warp == 12) { tmem_alloc(&tmem_slot, 512); tmem_relinquish(); }
+  if (warp == 16) { tmem_alloc(&tmem_slot, 512); tmem_relinquish(); }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -174,13 +174,13 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
   volatile int* abortp = &abort_flag;
 
   // No role leaves its loops early when a wait gives up: later waits return at once, and all keep their barriers company.
-  if (warp >= 12) {
-    if (warp == 12 && elect_one()) {
+  if (warp == 16) {
+    if (elect_one()) {
       // -------------------------------- MMA issuer --------------------------------
       const uint32_t q_addr = smem_u32(s_q), kv_addr = smem_u32(s_kv);
-      uint32_t n_item = 0, n_kv = 0, n_p = 0;     // running counts: items, fp16 tiles consumed, softmax steps
-      auto wait_kv = [&](uint32_t n) {
-        mbar_wait(&kv_full[n % RING], (n / RING) & 1, abortp, p.err, CS_ERR_TIMEOUT_TMA);
+      uint32_t n_item = 0, n_p = 0;     // running counts: items, pages (steps of the softmax)
+      auto wait_kv = [&](int kv, uint32_t n) {
+        mbar_wait(&kv_full[kv][n % RING], (n / RING) & 1, abortp, p.err, CS_ERR_TIMEOUT_TMA);
         tc_fence_after();
       };
       // (short loops: three roles run through their code in turn, and what does not stay in the instruction cache costs
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         umma_commit(&s_full[t]);
       };
       auto issue_pv = [&](int t, uint32_t n, bool first) {
-        uint64_t b = umma_smem_desc(kv_addr + (n % RING) * TILE, ATOM, 1024);
+        uint64_t b = umma_smem_desc(kv_addr + (RING + n % RING) * TILE, ATOM, 1024);
         uint32_t a = tmem + t * 128;
 #pragma unroll 1
         for (int k4 = 0; k4 < 2; ++k4, a += 32, b += 4 * 128)
@@ -208,25 +208,25 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         if (it.n == 0) continue;
         mbar_wait(&q_full, n_item & 1, abortp, p.err, CS_ERR_TIMEOUT_TMA);
         ++n_item;
-        wait_kv(n_kv);
-        issue_s(0, n_kv);
-        issue_s(1, n_kv);
-        umma_commit(&kv_empty[n_kv % RING]);
+        wait_kv(0, n_p);
+        issue_s(0, n_p);
+        issue_s(1, n_p);
+        umma_commit(&kv_empty[0][n_p % RING]);
         if (it.n == 1) umma_commit(&q_empty);
-        for (int j = 0; j < it.n; ++j, ++n_p, n_kv += 2) {
+        for (int j = 0; j < it.n; ++j, ++n_p) {
           const bool more = j + 1 < it.n;
-          wait_kv(n_kv + 1);                       // V of this page
-          if (more) wait_kv(n_kv + 2);             // K of the next
+          wait_kv(1, n_p);
+          if (more) wait_kv(0, n_p + 1);
 #pragma unroll 1
           for (int t = 0; t < 2; ++t) {
             mbar_wait(&p_full[t], n_p & 1, abortp, p.err, CS_ERR_TIMEOUT_EPI);
             tc_fence_after();
-            issue_pv(t, n_kv + 1, j == 0);
-            if (t == 1) umma_commit(&kv_empty[(n_kv + 1) % RING]);
-            if (more) issue_s(t, n_kv + 2); else umma_commit(&o_full[t]);
+            issue_pv(t, n_p, j == 0);
+            if (t == 1) umma_commit(&kv_empty[1][n_p % RING]);
+            if (more) issue_s(t, n_p + 1); else umma_commit(&o_full[t]);
           }
           if (more) {
-            umma_commit(&kv_empty[(n_kv + 2) % RING]);
+            umma_commit(&kv_empty[0][(n_p + 1) % RING]);
             if (j + 2 == it.n) umma_commit(&q_empty);
           }
         }
@@ -236,33 +236,33 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
     // ------------------------------ operand preparation ------------------------------
     constexpr int CHUNKS = D / 16;                 // 16-byte chunks of codes per row
     constexpr int ITER = CHUNKS;                   // chunks per thread and tile (128 rows, 128 threads)
-    const int tid = threadIdx.x - 256;
+    const int kv = (warp - 8) >> 2, tid = threadIdx.x - 256 - kv * 128;     // 0: keys, 1: values
     // This thread's chunks are chunk c0 of rows row0, row0 + STEP, ...  The eight threads of a shared-memory phase write
     // two rows of different parity, so that the swizzle sends their stores to different banks.
     constexpr int STEP = 128 / CHUNKS;
     const int row0 = D == 128 ? (tid >> 5) * 4 + ((tid >> 4) & 1) * 2 + ((tid >> 2) & 1) : tid >> 2;
     const int c0 = D == 128 ? ((tid >> 3) & 1) * 4 + (tid & 3) : tid & 3;
     const int off_a = (c0 >> 2) * ATOM + row0 * 128 + ((((c0 & 3) * 2) ^ (row0 & 7)) << 4), off_b = off_a ^ 16;   // STEP is a multiple of 8
-    uint32_t n_kv = 0, n_sc = 0, n_item = 0;
-    uint4 cur[ITER], nxt[ITER];                    // codes: tile in hand, next tile
-    float row_s[ITER];                             // next tile: scales of this thread's rows
-    float4 all_s, val_s;                           // next tile: scales of keys 4 lane .. + 3; with keys those of the values too
+    uint32_t n = 0, n_item = 0;                    // running counts: pages, items
+    uint4 code[ITER];                              // a tile: codes,
+    float row_s[ITER];                             // scales of this thread's rows,
+    float4 all_s, val_s;                           // scales of keys 4 lane .. + 3; with keys those of the values too
     const float* val_src = nullptr;
-    int rows = 0;                                  // next tile: rows that are keys of the sequence (may exceed 128)
-    // codes and scales of the keys (kv = 0) or values (kv = 1) of page j of a sequence
-    auto fetch = [&](const Item& it, int j, int kv) {
-      int page = p.block_table[it.seq * p.bt_stride + j];
+    int rows = 0;                                  // rows that are keys of the sequence (may exceed 128)
+    auto page_of = [&](const Item& it, int j) { return j < it.j0 + it.n ? p.block_table[it.seq * p.bt_stride + j] : 0; };
+    // codes and scales of the keys or values of a page, the j-th of its sequence
+    auto fetch = [&](const Item& it, int page, int j) {
       if (page < 0 || page >= p.num_pages) {
         if (tid == 0) cs_set_error(p.err, CS_ERR_BAD_ARG);
         page = 0;
       }
       const uint8_t* src = p.cache + ((static_cast<long long>(page) * 2 + kv) * p.Hkv + it.hk) * kv8_block_bytes(D);
       const float* scales = reinterpret_cast<const float*>(src + KV8_PAGE * D);
-#pragma unroll
-      for (int i = 0; i < ITER; ++i) nxt[i] = __ldg(reinterpret_cast<const uint4*>(src + row0 * D + c0 * 16 + i * STEP * D));
+      all_s = __ldg(reinterpret_cast<const float4*>(scales) + lane);
 #pragma unroll
       for (int i = 0; i < ITER; ++i) row_s[i] = __ldg(scales + row0 + i * STEP);
-      all_s = __ldg(reinterpret_cast<const float4*>(scales) + lane);
+#pragma unroll
+      for (int i = 0; i < ITER; ++i) code[i] = __ldg(reinterpret_cast<const uint4*>(src + row0 * D + c0 * 16 + i * STEP * D));
       rows = it.k_len - j * KV8_PAGE;
       if (kv == 0) {
         val_src = reinterpret_cast<const float*>(src + p.Hkv * kv8_block_bytes(D) + KV8_PAGE * D);
@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
     // Multipliers of this thread's rows as fp16 pairs (upper and lower part), and the exponent E (or F) of the page.  Rows
     // behind the sequence's keys become 0, whatever is there.  A key row or value row with a scale that is no number makes
     // the key a NaN, so that queries that see it, and only those, become NaN; in V such a row is 0 (0 * NaN is not 0).
-    auto multipliers = [&](int kv, uint32_t (&hi)[ITER], uint32_t (&lo)[ITER]) {
+    auto multipliers = [&](uint32_t (&hi)[ITER], uint32_t (&lo)[ITER]) {
       const float a4[4] = {all_s.x, all_s.y, all_s.z, all_s.w};
       uint32_t mx = 0;
 #pragma unroll
@@ -308,12 +308,12 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
       return *reinterpret_cast<const uint32_t*>(&y);
     };
     auto store = [&](const uint32_t (&hi)[ITER], const uint32_t (&lo)[ITER]) {
-      const uint32_t slot = n_kv % RING;
-      mbar_wait(&kv_empty[slot], ((n_kv / RING) & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
-      uint8_t* tile = s_kv + slot * TILE;
+      const uint32_t slot = n % RING;
+      mbar_wait(&kv_empty[kv][slot], ((n / RING) & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
+      uint8_t* tile = s_kv + (kv * RING + slot) * TILE;
 #pragma unroll
       for (int i = 0; i < ITER; ++i) {
-        const uint32_t w[4] = {cur[i].x, cur[i].y, cur[i].z, cur[i].w};
+        const uint32_t w[4] = {code[i].x, code[i].y, code[i].z, code[i].w};
         uint32_t h[8];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -325,8 +325,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         *reinterpret_cast<uint4*>(tile + off_b + i * STEP * 128) = make_uint4(h[4], h[5], h[6], h[7]);
       }
       fence_proxy_async_smem();
-      mbar_arrive(&kv_full[slot]);
-      ++n_kv;
+      mbar_arrive(&kv_full[kv][slot]);
     };
     auto next_item = [&](int round) {              // the next round that gives an item with pages, or -1
       for (; round * static_cast<int>(gridDim.x) < p.total_items; ++round) {
@@ -335,17 +334,15 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
       }
       return -1;
     };
-    int round = next_item(0);
-    if (round >= 0) {
-      const Item first = get_item(p, item_at(round));
-      fetch(first, first.j0, 0);
-    }
-    while (round >= 0) {
+    for (int round = next_item(0); round >= 0; round = next_item(round + 1)) {
       const Item it = get_item(p, item_at(round));
+      int page = page_of(it, it.j0);
+      fetch(it, page, it.j0);
+      page = page_of(it, it.j0 + 1);
       // queries of both tiles: thread = row; largest magnitude of the finite rows first, then fp16 with a common scale
-      const int group = p.G;
-      float cq;
-      {
+      float cq = 0.f;
+      if (kv == 0) {
+        const int group = p.G;
         uint32_t mx = 0;
         const __nv_bfloat16* src[2];
 #pragma unroll 1
@@ -392,29 +389,22 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         fence_proxy_async_smem();
         mbar_arrive(&q_full);
       }
-      round = next_item(round + 1);
-      int e_k = 0;
 #pragma unroll 1
-      for (int i = 0; i < 2 * it.n; ++i) {           // K and V of every page; the next tile is fetched while this one is converted
-#pragma unroll
-        for (int k = 0; k < ITER; ++k) cur[k] = nxt[k];
+      for (int j = it.j0; j < it.j0 + it.n; ++j, ++n) {
         uint32_t hi[ITER], lo[ITER];
-        const int e = multipliers(i & 1, hi, lo);
-        if (i + 1 < 2 * it.n) fetch(it, it.j0 + (i + 1) / 2, (i + 1) & 1);
-        else if (round >= 0) {
-          const Item after = get_item(p, item_at(round));
-          fetch(after, after.j0, 0);
-        }
+        const int e = multipliers(hi, lo);
         store(hi, lo);
-        if ((i & 1) == 0) {
-          e_k = e;
-        } else if (tid == 0) {
-          const uint32_t s = n_sc % SRING;
-          mbar_wait(&sc_empty[s], ((n_sc / SRING) & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
+        if (j + 1 < it.j0 + it.n) {
+          fetch(it, page, j + 1);
+          page = page_of(it, j + 2);
+        }
+        if (tid == 0) {
+          const uint32_t s = n % SRING;
+          mbar_wait(&sc_empty[s], ((n / SRING) & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
           // (not 0, also for a scale of 0: a hidden key's -inf times the factor has to stay -inf)
-          s_scale[s] = make_float2(fmaxf(cq * __uint_as_float(static_cast<uint32_t>(127 + e_k) << 23), 1e-37f), static_cast<float>(e));
+          if (kv == 0) s_scale[s].x = fmaxf(cq * __uint_as_float(static_cast<uint32_t>(127 + e) << 23), 1e-37f);
+          else s_scale[s].y = static_cast<float>(e);
           mbar_arrive(&sc_full[s]);
-          ++n_sc;
         }
       }
     }
@@ -568,7 +558,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 12) { tc_fence_after(); tmem_dealloc(tmem, 512); }
+  if (warp == 16) { tc_fence_after(); tmem_dealloc(tmem, 512); }
 }
 
 // Joins the parts of the rows of an item that was split: one warp per (token, head) row, parts in order.
