@@ -243,63 +243,53 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
     const int row0 = D == 128 ? (tid >> 5) * 4 + ((tid >> 4) & 1) * 2 + ((tid >> 2) & 1) : tid >> 2;
     const int c0 = D == 128 ? ((tid >> 3) & 1) * 4 + (tid & 3) : tid & 3;
     const int off_a = (c0 >> 2) * ATOM + row0 * 128 + ((((c0 & 3) * 2) ^ (row0 & 7)) << 4), off_b = off_a ^ 16;   // STEP is a multiple of 8
+    // Lane L looks after the scale of one of the 32 rows of its warp (rows row0 + i * STEP over the warp's threads).
+    constexpr int RPW = 32 / ITER;
+    const int my_row = (warp & 3) * RPW + lane % RPW + STEP * (lane / RPW);
     uint32_t n = 0, n_item = 0;                    // running counts: pages, items
-    uint4 code[ITER];                              // a tile: codes,
-    float row_s[ITER];                             // scales of this thread's rows,
-    float4 all_s, val_s;                           // scales of keys 4 lane .. + 3; with keys those of the values too
-    const float* val_src = nullptr;
+    // A tile in registers: codes, the scale of row `my_row` (with keys that of the value row too), the scales of keys 4 lane .. + 3
+    uint4 code[ITER];
+    float row_s, row_vs = 0.f;
+    float4 all_s;
     int rows = 0;                                  // rows that are keys of the sequence (may exceed 128)
     auto page_of = [&](const Item& it, int j) { return j < it.j0 + it.n ? p.block_table[it.seq * p.bt_stride + j] : 0; };
-    // codes and scales of the keys or values of a page, the j-th of its sequence
-    auto fetch = [&](const Item& it, int page, int j) {
-      if (page < 0 || page >= p.num_pages) {
+    const long long page_bytes = 2 * p.Hkv * kv8_block_bytes(D);
+    auto block_of = [&](const uint8_t* head, int page) {
+      if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_pages)) {
         if (tid == 0) cs_set_error(p.err, CS_ERR_BAD_ARG);
         page = 0;
       }
-      const uint8_t* src = p.cache + ((static_cast<long long>(page) * 2 + kv) * p.Hkv + it.hk) * kv8_block_bytes(D);
-      const float* scales = reinterpret_cast<const float*>(src + KV8_PAGE * D);
+      return head + page * page_bytes;
+    };
+    auto fetch_scales = [&](const uint8_t* block) {
+      const float* scales = reinterpret_cast<const float*>(block + KV8_PAGE * D);
+      row_s = __ldg(scales + my_row);
       all_s = __ldg(reinterpret_cast<const float4*>(scales) + lane);
-#pragma unroll
-      for (int i = 0; i < ITER; ++i) row_s[i] = __ldg(scales + row0 + i * STEP);
-#pragma unroll
-      for (int i = 0; i < ITER; ++i) code[i] = __ldg(reinterpret_cast<const uint4*>(src + row0 * D + c0 * 16 + i * STEP * D));
-      rows = it.k_len - j * KV8_PAGE;
       if (kv == 0) {
-        val_src = reinterpret_cast<const float*>(src + p.Hkv * kv8_block_bytes(D) + KV8_PAGE * D);
-        val_s = __ldg(reinterpret_cast<const float4*>(val_src) + lane);
+        const float* values = reinterpret_cast<const float*>(block + p.Hkv * kv8_block_bytes(D) + KV8_PAGE * D);
+        row_vs = __ldg(values + my_row);
       }
+    };
+    auto fetch_codes = [&](const uint8_t* block, int i) {
+      code[i] = __ldg(reinterpret_cast<const uint4*>(block + row0 * D + c0 * 16 + i * STEP * D));
     };
     auto finite_bits = [](float f) { const uint32_t b = __float_as_uint(f) & 0x7fffffffu; return b < 0x7f800000u ? b : 0u; };
     auto is_finite = [](float f) { return (__float_as_uint(f) & 0x7fffffffu) < 0x7f800000u; };
-    // Multipliers of this thread's rows as fp16 pairs (upper and lower part), and the exponent E (or F) of the page.  Rows
-    // behind the sequence's keys become 0, whatever is there.  A key row or value row with a scale that is no number makes
-    // the key a NaN, so that queries that see it, and only those, become NaN; in V such a row is 0 (0 * NaN is not 0).
-    auto multipliers = [&](uint32_t (&hi)[ITER], uint32_t (&lo)[ITER]) {
+    // The multiplier of row `my_row` as two fp16 parts, and the exponent E (or F) of the page.  Rows behind the sequence's
+    // keys become 0, whatever is there.  A key row or value row with a scale that is no number makes the key a NaN, so that
+    // queries that see it, and only those, become NaN; in V such a row is 0 (0 * NaN is not 0).
+    auto multiplier = [&](uint32_t& parts) {
       const float a4[4] = {all_s.x, all_s.y, all_s.z, all_s.w};
       uint32_t mx = 0;
 #pragma unroll
       for (int k = 0; k < 4; ++k) mx = max(mx, lane * 4 + k < rows ? finite_bits(a4[k]) : 0u);
       mx = __reduce_max_sync(0xffffffffu, mx);
       const int e = min(max(static_cast<int>(mx >> 23) - 127 - 13, -110), 120);     // the largest scale into [2^13, 2^14)
-      const float f = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-      bool bad = false;
-      if (kv == 0) {
-        const float v4[4] = {val_s.x, val_s.y, val_s.z, val_s.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) bad |= lane * 4 + k < rows && !is_finite(v4[k]);
-        bad = __any_sync(0xffffffffu, bad);
-      }
-#pragma unroll
-      for (int i = 0; i < ITER; ++i) {
-        const int row = row0 + i * STEP;
-        float v = row_s[i] * f;
-        if (kv == 1 && !is_finite(row_s[i])) v = 0.f;
-        if (bad && row < rows && !is_finite(__ldg(val_src + row))) v = __uint_as_float(0x7fffffffu);
-        if (row >= rows) v = 0.f;
-        const __half h = __float2half_rn(v), r = __float2half_rn(v - __half2float(h));
-        hi[i] = __half_as_ushort(h) * 0x10001u;
-        lo[i] = __half_as_ushort(r) * 0x10001u;
-      }
+      float v = row_s * __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+      if (!is_finite(row_s) || !is_finite(row_vs)) v = kv == 0 ? __uint_as_float(0x7fffffffu) : 0.f;
+      if (my_row >= rows) v = 0.f;
+      const __half h = __float2half_rn(v), r = __float2half_rn(v - __half2float(h));
+      parts = __half_as_ushort(h) | static_cast<uint32_t>(__half_as_ushort(r)) << 16;
       return e;
     };
     auto scaled = [](uint32_t c, uint32_t hi, uint32_t lo) {      // c * (hi + lo), rounded once
@@ -307,19 +297,23 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
       const __half2 y = __hfma2(x, h, __hmul2(x, l));
       return *reinterpret_cast<const uint32_t*>(&y);
     };
-    auto store = [&](const uint32_t (&hi)[ITER], const uint32_t (&lo)[ITER]) {
+    // Convert the tile in hand and, chunk by chunk, fetch the next one into the registers that become free.
+    auto convert = [&](uint32_t parts, const uint8_t* next) {
       const uint32_t slot = n % RING;
       mbar_wait(&kv_empty[kv][slot], ((n / RING) & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
       uint8_t* tile = s_kv + (kv * RING + slot) * TILE;
 #pragma unroll
       for (int i = 0; i < ITER; ++i) {
+        const uint32_t f = __shfl_sync(0xffffffffu, parts, i * RPW + row0 % RPW);
+        const uint32_t hi = __byte_perm(f, 0, 0x1010), lo = __byte_perm(f, 0, 0x3232);
         const uint32_t w[4] = {code[i].x, code[i].y, code[i].z, code[i].w};
+        fetch_codes(next, i);
         uint32_t h[8];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           codes_to_half(w[k], h[2 * k], h[2 * k + 1]);
-          h[2 * k] = scaled(h[2 * k], hi[i], lo[i]);
-          h[2 * k + 1] = scaled(h[2 * k + 1], hi[i], lo[i]);
+          h[2 * k] = scaled(h[2 * k], hi, lo);
+          h[2 * k + 1] = scaled(h[2 * k + 1], hi, lo);
         }
         *reinterpret_cast<uint4*>(tile + off_a + i * STEP * 128) = make_uint4(h[0], h[1], h[2], h[3]);
         *reinterpret_cast<uint4*>(tile + off_b + i * STEP * 128) = make_uint4(h[4], h[5], h[6], h[7]);
@@ -336,29 +330,45 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
     };
     for (int round = next_item(0); round >= 0; round = next_item(round + 1)) {
       const Item it = get_item(p, item_at(round));
-      int page = page_of(it, it.j0);
-      fetch(it, page, it.j0);
-      page = page_of(it, it.j0 + 1);
-      // queries of both tiles: thread = row; largest magnitude of the finite rows first, then fp16 with a common scale
+      const uint8_t* head = p.cache + (static_cast<long long>(kv) * p.Hkv + it.hk) * kv8_block_bytes(D);
+      const uint8_t* block = block_of(head, page_of(it, it.j0));
+      fetch_scales(block);
+#pragma unroll
+      for (int i = 0; i < ITER; ++i) fetch_codes(block, i);
+      int page = page_of(it, it.j0 + 1);
       float cq = 0.f;
       if (kv == 0) {
-        const int group = p.G;
-        uint32_t mx = 0;
-        const __nv_bfloat16* src[2];
-#pragma unroll 1
-        for (int t = 0; t < 2; ++t) {
-          const int tl = tid / group, g = tid - tl * group, tok = it.t0 + t * p.tok_per_tile + tl;
+        // Queries of both tiles, D / 8 lanes per row: copied as they are to the place where their fp16 form will be, all in
+        // flight at once; then the largest magnitude of the finite rows, and fp16 with a common scale in place.
+        // (row * inv_g >> 16 is row / G for row < 128.)
+        constexpr int LANES = D / 8, PER = 32 / LANES, PASSES = 32 / PER;   // lanes per row, rows per warp and pass, passes per tile
+        const int ch = lane % LANES, row_w = (warp & 3) * PER + lane / LANES;
+        const uint32_t inv_g = (65536u + p.G - 1) / p.G, q_sm = smem_u32(s_q);
+        auto place = [&](int i) {                                 // 16-byte chunk of this thread in pass i
+          const int row = (i % PASSES) * 4 * PER + row_w;
+          return static_cast<uint32_t>((i / PASSES) * TILE + (ch >> 3) * ATOM + row * 128 + (((ch & 7) ^ (row & 7)) << 4));
+        };
+        mbar_wait(&q_empty, (n_item & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
+        ++n_item;
+#pragma unroll 2
+        for (int i = 0; i < 2 * PASSES; ++i) {
+          const int row = (i % PASSES) * 4 * PER + row_w;
+          const int tl = static_cast<int>(row * inv_g >> 16), g = row - tl * p.G, tok = it.t0 + (i / PASSES) * p.tok_per_tile + tl;
           const bool ok = tl < p.tok_per_tile && tok < it.q_len && g < it.n_heads;
-          src[t] = ok ? p.q + (it.q_beg + tok) * p.q_tok + (it.h0 + g) * D : nullptr;
-          if (!ok) continue;
-          uint32_t m = 0;
+          const __nv_bfloat16* src = p.q + (it.q_beg + (ok ? tok : 0)) * p.q_tok + (it.h0 + (ok ? g : 0)) * D + ch * 8;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(q_sm + place(i)), "l"(src), "r"(ok ? 16 : 0) : "memory");
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        uint32_t mx = 0;
 #pragma unroll 4
-          for (int i = 0; i < D / 8; ++i) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4*>(src[t]) + i);
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        for (int i = 0; i < 2 * PASSES; ++i) {
+          const uint4 v = *reinterpret_cast<const uint4*>(s_q + place(i));
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+          uint32_t m = 0;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) m = max(m, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
-          }
+          for (int k = 0; k < 4; ++k) m = max(m, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
+#pragma unroll
+          for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
           if (m < 0x7f80u) mx = max(mx, m);
         }
         mx = __reduce_max_sync(0xffffffffu, mx);
@@ -370,34 +380,29 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         // a negative scale turns the queries around, so that the largest score is the largest S
         const float up = copysignf(__uint_as_float(static_cast<uint32_t>(127 + shift) << 23), p.scale_log2);
         cq = fabsf(p.scale_log2) * __uint_as_float(static_cast<uint32_t>(127 + 8 - shift) << 23);   // 2^8: codes_to_half gives code / 2^8
-        mbar_wait(&q_empty, (n_item & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
-        ++n_item;
-#pragma unroll 1
-        for (int t = 0; t < 2; ++t) {
-          uint8_t* dst = s_q + t * TILE + tid * 128;
 #pragma unroll 4
-          for (int i = 0; i < D / 8; ++i) {
-            const uint4 v = src[t] != nullptr ? __ldg(reinterpret_cast<const uint4*>(src[t]) + i) : make_uint4(0, 0, 0, 0);
-            uint4 h;   // channels in the order of the codes: (0, 2), (1, 3) of every four
-            h.x = half2_bits(bf16lo(v.x) * up, bf16lo(v.y) * up);
-            h.y = half2_bits(bf16hi(v.x) * up, bf16hi(v.y) * up);
-            h.z = half2_bits(bf16lo(v.z) * up, bf16lo(v.w) * up);
-            h.w = half2_bits(bf16hi(v.z) * up, bf16hi(v.w) * up);
-            *reinterpret_cast<uint4*>(dst + (i >> 3) * ATOM + (((i & 7) ^ (tid & 7)) << 4)) = h;
-          }
+        for (int i = 0; i < 2 * PASSES; ++i) {
+          uint4* at = reinterpret_cast<uint4*>(s_q + place(i));
+          const uint4 v = *at;
+          uint4 h;   // channels in the order of the codes: (0, 2), (1, 3) of every four
+          h.x = half2_bits(bf16lo(v.x) * up, bf16lo(v.y) * up);
+          h.y = half2_bits(bf16hi(v.x) * up, bf16hi(v.y) * up);
+          h.z = half2_bits(bf16lo(v.z) * up, bf16lo(v.w) * up);
+          h.w = half2_bits(bf16hi(v.z) * up, bf16hi(v.w) * up);
+          *at = h;
         }
         fence_proxy_async_smem();
         mbar_arrive(&q_full);
       }
 #pragma unroll 1
       for (int j = it.j0; j < it.j0 + it.n; ++j, ++n) {
-        uint32_t hi[ITER], lo[ITER];
-        const int e = multipliers(hi, lo);
-        store(hi, lo);
-        if (j + 1 < it.j0 + it.n) {
-          fetch(it, page, j + 1);
-          page = page_of(it, j + 2);
-        }
+        uint32_t parts;
+        rows = it.k_len - j * KV8_PAGE;
+        const int e = multiplier(parts);
+        if (j + 1 < it.j0 + it.n) block = block_of(head, page);   // (behind the last page the same one is read again)
+        fetch_scales(block);
+        page = page_of(it, j + 2);
+        convert(parts, block);
         if (tid == 0) {
           const uint32_t s = n % SRING;
           mbar_wait(&sc_empty[s], ((n / SRING) & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
