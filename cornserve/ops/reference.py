@@ -188,9 +188,13 @@ KV_FP8_AMAX_FLOOR = 2.0 ** -40
 
 
 def kv_cache_fp8_views(cache):
-    d = cache.shape[-1] // KV_FP8_PAGE - 4
-    codes = cache[..., : KV_FP8_PAGE * d].view(torch.float8_e4m3fn).unflatten(-1, (KV_FP8_PAGE, d))
-    return codes, cache[..., KV_FP8_PAGE * d:].view(torch.float32)
+    pages, _, heads, block = cache.shape
+    d = block // KV_FP8_PAGE - 4
+    at = cache.storage_offset()
+    codes = cache.view(torch.float8_e4m3fn).as_strided((pages, 2, heads, KV_FP8_PAGE, d), (2 * heads * block, heads * block, block, d, 1), at)
+    b4 = block // 4
+    scales = cache.view(torch.float32).as_strided((pages, 2, heads, KV_FP8_PAGE), (2 * heads * b4, heads * b4, b4, 1), at // 4 + KV_FP8_PAGE * d // 4)
+    return codes, scales
 
 
 def quantize_kv_rows(x):
