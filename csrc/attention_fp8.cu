@@ -31,9 +31,11 @@ namespace {
 
 constexpr int ATOM = 128 * 128;            // 128 rows x 64 fp16, 128-byte swizzle
 constexpr int RING = 2;                    // fp16 tiles of K and of V
-constexpr int SRING = 4;                   // the two scalars of a page
+constexpr int SRING = 4;                   // the two scalars of a page; at least RING + 2
 constexpr int THREADS = 17 * 32;
 constexpr float M_NONE = -3.0e38f;         // running maximum before the first key (finite: differences stay defined)
+
+static_assert(SRING >= RING + 2, "scalars outlive their tile by a page");
 
 struct PrefillParams {
   const __nv_bfloat16* q; long long q_tok;              // heads follow each other; every token on a 16-byte boundary
@@ -148,23 +150,24 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* s_q = smem;
   uint8_t* s_kv = smem + Shape<D>::Q;    // K tiles, V tiles
-  __shared__ uint64_t q_full, q_empty, kv_full[2][RING], kv_empty[2][RING], sc_full[SRING], sc_empty[SRING], s_full[2], p_full[2], o_full[2];
+  __shared__ uint64_t q_full, q_empty, kv_full[2][RING], kv_empty[2][RING], sc_full[SRING], s_full[2], p_full[2], o_full[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
-  __shared__ uint32_t s_max[4];
+  __shared__ uint32_t s_max[8], s_row[128];   // s_row: token in tile | head << 16 of a tile row
   __shared__ float2 s_scale[SRING];     // of a page: factor from S to base-2 exponents, F
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     abort_flag = 0;
-    mbar_init(&q_full, 128);
+    mbar_init(&q_full, 256);
     mbar_init(&q_empty, 1);
     for (int i = 0; i < 2 * RING; ++i) { mbar_init(&kv_full[i / RING][i % RING], 128); mbar_init(&kv_empty[i / RING][i % RING], 1); }
-    for (int i = 0; i < SRING; ++i) { mbar_init(&sc_full[i], 2); mbar_init(&sc_empty[i], 8); }
+    for (int i = 0; i < SRING; ++i) mbar_init(&sc_full[i], 2);
     for (int t = 0; t < 2; ++t) { mbar_init(&s_full[t], 1); mbar_init(&p_full[t], 128); mbar_init(&o_full[t], 1); }
     mbar_fence_init();
   }
   if (warp == 16) { tmem_alloc(&tmem_slot, 512); tmem_relinquish(); }
+  if (threadIdx.x < 128) s_row[threadIdx.x] = threadIdx.x / p.G | (threadIdx.x % p.G) << 16;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -298,9 +301,18 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
       return *reinterpret_cast<const uint32_t*>(&y);
     };
     // Convert the tile in hand and, chunk by chunk, fetch the next one into the registers that become free.
-    auto convert = [&](uint32_t parts, const uint8_t* next) {
+    auto convert = [&](uint32_t parts, const uint8_t* next, int e, float cq) {
       const uint32_t slot = n % RING;
       mbar_wait(&kv_empty[kv][slot], ((n / RING) & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
+      if (tid == 0) {
+        // The page's scalars.  Their place was that of page n - SRING, which both softmax groups are done with: the tile of
+        // page n - RING is free only behind products that waited for the weights of page n - RING - 1 or a later one.
+        // (The factor is not 0, also for a scale of 0: a hidden key's -inf times the factor has to stay -inf.)
+        const uint32_t s = n % SRING;
+        if (kv == 0) s_scale[s].x = fmaxf(cq * __uint_as_float(static_cast<uint32_t>(127 + e) << 23), 1e-37f);
+        else s_scale[s].y = static_cast<float>(e);
+        mbar_arrive(&sc_full[s]);
+      }
       uint8_t* tile = s_kv + (kv * RING + slot) * TILE;
 #pragma unroll
       for (int i = 0; i < ITER; ++i) {
@@ -321,79 +333,85 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
       fence_proxy_async_smem();
       mbar_arrive(&kv_full[kv][slot]);
     };
-    auto next_item = [&](int round) {              // the next round that gives an item with pages, or -1
+    Item it;
+    auto next_item = [&](int round) {              // the next round that gives an item with pages (in `it`), or -1
       for (; round * static_cast<int>(gridDim.x) < p.total_items; ++round) {
         const int w = item_at(round);
-        if (w < p.total_items && get_item(p, w).n > 0) return round;
+        if (w >= p.total_items) continue;
+        it = get_item(p, w);
+        if (it.n > 0) return round;
       }
       return -1;
     };
     for (int round = next_item(0); round >= 0; round = next_item(round + 1)) {
-      const Item it = get_item(p, item_at(round));
       const uint8_t* head = p.cache + (static_cast<long long>(kv) * p.Hkv + it.hk) * kv8_block_bytes(D);
       const uint8_t* block = block_of(head, page_of(it, it.j0));
       fetch_scales(block);
 #pragma unroll
       for (int i = 0; i < ITER; ++i) fetch_codes(block, i);
       int page = page_of(it, it.j0 + 1);
-      float cq = 0.f;
-      if (kv == 0) {
-        // Queries of both tiles, D / 8 lanes per row: copied as they are to the place where their fp16 form will be, all in
-        // flight at once; then the largest magnitude of the finite rows, and fp16 with a common scale in place.
-        // (row * inv_g >> 16 is row / G for row < 128.)
-        constexpr int LANES = D / 8, PER = 32 / LANES, PASSES = 32 / PER;   // lanes per row, rows per warp and pass, passes per tile
-        const int ch = lane % LANES, row_w = (warp & 3) * PER + lane / LANES;
-        const uint32_t inv_g = (65536u + p.G - 1) / p.G, q_sm = smem_u32(s_q);
-        auto place = [&](int i) {                                 // 16-byte chunk of this thread in pass i
-          const int row = (i % PASSES) * 4 * PER + row_w;
-          return static_cast<uint32_t>((i / PASSES) * TILE + (ch >> 3) * ATOM + row * 128 + (((ch & 7) ^ (row & 7)) << 4));
-        };
-        mbar_wait(&q_empty, (n_item & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
-        ++n_item;
-#pragma unroll 2
-        for (int i = 0; i < 2 * PASSES; ++i) {
-          const int row = (i % PASSES) * 4 * PER + row_w;
-          const int tl = static_cast<int>(row * inv_g >> 16), g = row - tl * p.G, tok = it.t0 + (i / PASSES) * p.tok_per_tile + tl;
-          const bool ok = tl < p.tok_per_tile && tok < it.q_len && g < it.n_heads;
-          const __nv_bfloat16* src = p.q + (it.q_beg + (ok ? tok : 0)) * p.q_tok + (it.h0 + (ok ? g : 0)) * D + ch * 8;
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(q_sm + place(i)), "l"(src), "r"(ok ? 16 : 0) : "memory");
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        uint32_t mx = 0;
+      // Queries, one tile per group, D / 8 lanes per row: copied as they are to the place where their fp16 form will be, all
+      // in flight at once; then the largest finite magnitude of both tiles, and fp16 with a common scale in place.
+      constexpr int LANES = D / 8, PER = 32 / LANES, PASSES = 32 / PER;     // lanes per row, rows per warp and pass, passes
+      const int ch = lane % LANES, row_w = (warp & 3) * PER + lane / LANES;
+      // row i * 4 * PER + row_w: its swizzle is the same in all passes (4 * PER is a multiple of 8)
+      uint8_t* q_at = s_q + kv * TILE + (ch >> 3) * ATOM + row_w * 128 + (((ch & 7) ^ (row_w & 7)) << 4);
+      mbar_wait(&q_empty, (n_item & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
+      ++n_item;
+      {
+        const int t0 = it.t0 + kv * p.tok_per_tile, n_tok = min(p.tok_per_tile, it.q_len - t0);
+        const __nv_bfloat16* src0 = p.q + (it.q_beg + (n_tok > 0 ? t0 : 0)) * p.q_tok + it.h0 * D + ch * 8;
+        const uint32_t q_sm = smem_u32(q_at);
 #pragma unroll 4
-        for (int i = 0; i < 2 * PASSES; ++i) {
-          const uint4 v = *reinterpret_cast<const uint4*>(s_q + place(i));
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-          uint32_t m = 0;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) m = max(m, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
-#pragma unroll
-          for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-          if (m < 0x7f80u) mx = max(mx, m);
+        for (int i = 0; i < PASSES; ++i) {
+          const uint32_t rc = s_row[i * 4 * PER + row_w];                   // token in tile | head << 16
+          const int tl = rc & 0xffff, g = rc >> 16;
+          const bool ok = tl < n_tok && g < it.n_heads;
+          const __nv_bfloat16* src = ok ? src0 + tl * p.q_tok + g * D : src0;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(q_sm + i * 4 * PER * 128), "l"(src), "r"(ok ? 16 : 0) : "memory");
         }
-        mx = __reduce_max_sync(0xffffffffu, mx);
-        if (lane == 0) s_max[warp - 8] = mx;
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        mx = max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3]));
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        const int shift = min(max(127 + 14 - static_cast<int>(mx >> 7), -110), 110);   // the largest element into [2^14, 2^15)
-        // a negative scale turns the queries around, so that the largest score is the largest S
-        const float up = copysignf(__uint_as_float(static_cast<uint32_t>(127 + shift) << 23), p.scale_log2);
-        cq = fabsf(p.scale_log2) * __uint_as_float(static_cast<uint32_t>(127 + 8 - shift) << 23);   // 2^8: codes_to_half gives code / 2^8
-#pragma unroll 4
-        for (int i = 0; i < 2 * PASSES; ++i) {
-          uint4* at = reinterpret_cast<uint4*>(s_q + place(i));
-          const uint4 v = *at;
-          uint4 h;   // channels in the order of the codes: (0, 2), (1, 3) of every four
-          h.x = half2_bits(bf16lo(v.x) * up, bf16lo(v.y) * up);
-          h.y = half2_bits(bf16hi(v.x) * up, bf16hi(v.y) * up);
-          h.z = half2_bits(bf16lo(v.z) * up, bf16lo(v.w) * up);
-          h.w = half2_bits(bf16hi(v.z) * up, bf16hi(v.w) * up);
-          *at = h;
-        }
-        fence_proxy_async_smem();
-        mbar_arrive(&q_full);
       }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      auto largest = [&](bool finite_only) {
+        uint32_t m2 = 0;                           // two 16-bit maxima
+#pragma unroll 8
+        for (int i = 0; i < PASSES; ++i) {
+          const uint4 v = *reinterpret_cast<const uint4*>(q_at + i * 4 * PER * 128);
+          uint32_t w[4] = {v.x & 0x7fff7fffu, v.y & 0x7fff7fffu, v.z & 0x7fff7fffu, v.w & 0x7fff7fffu};
+          if (finite_only) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[k] = ((w[k] & 0xffffu) < 0x7f80u ? w[k] & 0xffffu : 0u) | ((w[k] >> 16) < 0x7f80u ? w[k] & 0xffff0000u : 0u);
+          }
+          m2 = __vmaxu2(m2, __vmaxu2(__vmaxu2(w[0], w[1]), __vmaxu2(w[2], w[3])));
+        }
+        const uint32_t mx = __reduce_max_sync(0xffffffffu, max(m2 & 0xffffu, m2 >> 16));
+        if (lane == 0) s_max[warp - 8] = mx;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        uint32_t all = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) all = max(all, s_max[i]);
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        return all;
+      };
+      uint32_t mx = largest(false);
+      if (mx >= 0x7f80u) mx = largest(true);       // (an infinity or NaN makes its own row NaN and nothing else)
+      const int shift = min(max(127 + 14 - static_cast<int>(mx >> 7), -110), 110);   // the largest element into [2^14, 2^15)
+      // a negative scale turns the queries around, so that the largest score is the largest S
+      const float up = copysignf(__uint_as_float(static_cast<uint32_t>(127 + shift) << 23), p.scale_log2);
+      const float cq = fabsf(p.scale_log2) * __uint_as_float(static_cast<uint32_t>(127 + 8 - shift) << 23);   // 2^8: codes_to_half gives code / 2^8
+#pragma unroll 4
+      for (int i = 0; i < PASSES; ++i) {
+        uint4* at = reinterpret_cast<uint4*>(q_at + i * 4 * PER * 128);
+        const uint4 v = *at;
+        uint4 h;   // channels in the order of the codes: (0, 2), (1, 3) of every four
+        h.x = half2_bits(bf16lo(v.x) * up, bf16lo(v.y) * up);
+        h.y = half2_bits(bf16hi(v.x) * up, bf16hi(v.y) * up);
+        h.z = half2_bits(bf16lo(v.z) * up, bf16lo(v.w) * up);
+        h.w = half2_bits(bf16hi(v.z) * up, bf16hi(v.w) * up);
+        *at = h;
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&q_full);
 #pragma unroll 1
       for (int j = it.j0; j < it.j0 + it.n; ++j, ++n) {
         uint32_t parts;
@@ -402,15 +420,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         if (j + 1 < it.j0 + it.n) block = block_of(head, page);   // (behind the last page the same one is read again)
         fetch_scales(block);
         page = page_of(it, j + 2);
-        convert(parts, block);
-        if (tid == 0) {
-          const uint32_t s = n % SRING;
-          mbar_wait(&sc_empty[s], ((n / SRING) & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
-          // (not 0, also for a scale of 0: a hidden key's -inf times the factor has to stay -inf)
-          if (kv == 0) s_scale[s].x = fmaxf(cq * __uint_as_float(static_cast<uint32_t>(127 + e) << 23), 1e-37f);
-          else s_scale[s].y = static_cast<float>(e);
-          mbar_arrive(&sc_full[s]);
-        }
+        convert(parts, block, e, cq);
       }
     }
   } else {
@@ -436,16 +446,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         mbar_wait(&s_full[t], n_step & 1, abortp, p.err, CS_ERR_TIMEOUT_MMA);
         tc_fence_after();
         const float2 sc = s_scale[s];
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sc_empty[s]);
         const int nvalid = lim - (it.j0 + j) * KV8_PAGE;       // visible keys of the page (may be negative or beyond 128)
         // first pass: the largest S of the row
         float mx0 = -INFINITY, mx1 = -INFINITY;
-#pragma unroll 1
-        for (int c = 0; c < KV8_PAGE; c += 32) {
-          uint32_t x[32];
-          tmem_ld32(tS + c, x);
-          tmem_wait_ld();
+        auto largest = [&](uint32_t (&x)[32], int c) {
           if (nvalid < c + 32) {                     // hidden keys: whatever is there
 #pragma unroll
             for (int i = 0; i < 32; ++i)
@@ -456,6 +460,15 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
             mx0 = fmaxf(fmaxf(mx0, __uint_as_float(x[i])), __uint_as_float(x[i + 1]));
             mx1 = fmaxf(fmaxf(mx1, __uint_as_float(x[i + 2])), __uint_as_float(x[i + 3]));
           }
+        };
+#pragma unroll 1
+        for (int c = 0; c < KV8_PAGE; c += 64) {
+          uint32_t x[32], y[32];
+          tmem_ld32(tS + c, x);
+          tmem_ld32(tS + c + 32, y);
+          tmem_wait_ld();
+          largest(x, c);
+          largest(y, c + 32);
         }
         const float mx = fmaxf(mx0, mx1) * sc.x + sc.y;
         // The reference m - 6 moves only when a weight would pass 2^14
@@ -480,19 +493,15 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         const float add = sc.y + (6.f - m);
         const uint64_t mul2 = pack2(sc.x, sc.x), ref2 = pack2(add, add);
         uint64_t sum_a = pack2(0.f, 0.f), sum_b = sum_a;
-#pragma unroll 1
-        for (int c = 0; c < KV8_PAGE; c += 32) {
-          uint32_t x[32];
-          tmem_ld32(tS + c, x);
-          tmem_wait_ld();
-          if (nvalid < c + 32) {
+        auto weigh = [&](uint32_t (&x)[16], int c) {
+          if (nvalid < c + 16) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
+            for (int i = 0; i < 16; ++i)
               if (c + i >= nvalid) x[i] = 0xff800000u;
           }
-          uint32_t pk[16];
+          uint32_t pk[8];
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
+          for (int i = 0; i < 16; i += 4) {
             float e0, e1, e2, e3;
             unpack2(fma2(pack2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), mul2, ref2), e0, e1);
             unpack2(fma2(pack2(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])), mul2, ref2), e2, e3);
@@ -503,7 +512,18 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
             pk[(i >> 1) + 1] = half2_bits(e2, e3);
           }
           __syncwarp();
-          tmem_st16(tS + (c >> 1), pk);
+          tmem_st8(tS + (c >> 1), pk);
+        };
+        uint32_t x[16], y[16];                       // the next 16 scores are on their way while 16 become weights
+        tmem_ld16(tS, x);
+#pragma unroll 1
+        for (int c = 0; c < KV8_PAGE; c += 32) {
+          tmem_wait_ld();
+          tmem_ld16(tS + c + 16, y);
+          weigh(x, c);
+          tmem_wait_ld();
+          if (c + 32 < KV8_PAGE) tmem_ld16(tS + c + 32, x);
+          weigh(y, c + 16);
         }
         {
           float s0, s1;
