@@ -493,15 +493,15 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         const float add = sc.y + (6.f - m);
         const uint64_t mul2 = pack2(sc.x, sc.x), ref2 = pack2(add, add);
         uint64_t sum_a = pack2(0.f, 0.f), sum_b = sum_a;
-        auto weigh = [&](uint32_t (&x)[16], int c) {
-          if (nvalid < c + 16) {
+        auto weigh = [&](uint32_t (&x)[32], int c) {
+          if (nvalid < c + 32) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
+            for (int i = 0; i < 32; ++i)
               if (c + i >= nvalid) x[i] = 0xff800000u;
           }
-          uint32_t pk[8];
+          uint32_t pk[16];
 #pragma unroll
-          for (int i = 0; i < 16; i += 4) {
+          for (int i = 0; i < 32; i += 4) {
             float e0, e1, e2, e3;
             unpack2(fma2(pack2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), mul2, ref2), e0, e1);
             unpack2(fma2(pack2(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])), mul2, ref2), e2, e3);
@@ -512,18 +512,14 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
             pk[(i >> 1) + 1] = half2_bits(e2, e3);
           }
           __syncwarp();
-          tmem_st8(tS + (c >> 1), pk);
+          tmem_st16(tS + (c >> 1), pk);
         };
-        uint32_t x[16], y[16];                       // the next 16 scores are on their way while 16 become weights
-        tmem_ld16(tS, x);
 #pragma unroll 1
         for (int c = 0; c < KV8_PAGE; c += 32) {
+          uint32_t x[32];
+          tmem_ld32(tS + c, x);
           tmem_wait_ld();
-          tmem_ld16(tS + c + 16, y);
           weigh(x, c);
-          tmem_wait_ld();
-          if (c + 32 < KV8_PAGE) tmem_ld16(tS + c + 32, x);
-          weigh(y, c + 16);
         }
         {
           float s0, s1;
