@@ -126,15 +126,6 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
       : "memory");
 }
 
-// Four codes as fp16 numbers times 2^-8, in the order (0, 2), (1, 3): the sign stays on top and the seven magnitude bits
-// move one place down, where e4m3's exponent is fp16's exponent minus 8 (subnormal codes become subnormal halves).  On
-// the integer pipe: the conversion instruction shares its pipe with the exponentials of the softmax.
-__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& r02, uint32_t& r13) {
-  const uint32_t e = w << 8;
-  r13 = (w & 0x80008000u) | ((w >> 1) & 0x3f803f80u);
-  r02 = (e & 0x80008000u) | ((e >> 1) & 0x3f803f80u);
-}
-
 // Shared memory: queries (two tiles), ring of fp16 tiles.
 template <int D>
 struct Shape {
@@ -154,7 +145,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   __shared__ uint32_t s_max[8], s_row[128];   // s_row: token in tile | head << 16 of a tile row
-  __shared__ float2 s_scale[SRING];     // of a page: factor from S to base-2 exponents, F
+  __shared__ float4 s_scale[SRING];     // of a page: factor from S to base-2 exponents, F, 2^-F
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -287,7 +278,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
 #pragma unroll
       for (int k = 0; k < 4; ++k) mx = max(mx, lane * 4 + k < rows ? finite_bits(a4[k]) : 0u);
       mx = __reduce_max_sync(0xffffffffu, mx);
-      const int e = min(max(static_cast<int>(mx >> 23) - 127 - 13, -110), 120);     // the largest scale into [2^13, 2^14)
+      const int e = min(max(static_cast<int>(mx >> 23) - 127 - 6, -110), 120);      // the largest scale into [2^6, 2^7): codes reach 448
       float v = row_s * __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
       if (!is_finite(row_s) || !is_finite(row_vs)) v = kv == 0 ? __uint_as_float(0x7fffffffu) : 0.f;
       if (my_row >= rows) v = 0.f;
@@ -310,10 +301,18 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         // (The factor is not 0, also for a scale of 0: a hidden key's -inf times the factor has to stay -inf.)
         const uint32_t s = n % SRING;
         if (kv == 0) s_scale[s].x = fmaxf(cq * __uint_as_float(static_cast<uint32_t>(127 + e) << 23), 1e-37f);
-        else s_scale[s].y = static_cast<float>(e);
+        else {
+          s_scale[s].y = static_cast<float>(e);
+          s_scale[s].z = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+        }
         mbar_arrive(&sc_full[s]);
       }
       uint8_t* tile = s_kv + (kv * RING + slot) * TILE;
+      if (rows < KV8_PAGE) {                       // what lies behind the keys may be anything
+#pragma unroll
+        for (int i = 0; i < ITER; ++i)
+          if (row0 + i * STEP >= rows) code[i] = make_uint4(0, 0, 0, 0);
+      }
 #pragma unroll
       for (int i = 0; i < ITER; ++i) {
         const uint32_t f = __shfl_sync(0xffffffffu, parts, i * RPW + row0 % RPW);
@@ -322,11 +321,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         fetch_codes(next, i);
         uint32_t h[8];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          codes_to_half(w[k], h[2 * k], h[2 * k + 1]);
-          h[2 * k] = scaled(h[2 * k], hi, lo);
-          h[2 * k + 1] = scaled(h[2 * k + 1], hi, lo);
-        }
+        for (int k = 0; k < 4; ++k) e4m3x4_to_half2x2(w[k], h[2 * k], h[2 * k + 1]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) h[k] = scaled(h[k], hi, lo);
         *reinterpret_cast<uint4*>(tile + off_a + i * STEP * 128) = make_uint4(h[0], h[1], h[2], h[3]);
         *reinterpret_cast<uint4*>(tile + off_b + i * STEP * 128) = make_uint4(h[4], h[5], h[6], h[7]);
       }
@@ -398,17 +395,13 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
       const int shift = min(max(127 + 14 - static_cast<int>(mx >> 7), -110), 110);   // the largest element into [2^14, 2^15)
       // a negative scale turns the queries around, so that the largest score is the largest S
       const float up = copysignf(__uint_as_float(static_cast<uint32_t>(127 + shift) << 23), p.scale_log2);
-      const float cq = fabsf(p.scale_log2) * __uint_as_float(static_cast<uint32_t>(127 + 8 - shift) << 23);   // 2^8: codes_to_half gives code / 2^8
+      const float cq = fabsf(p.scale_log2) * __uint_as_float(static_cast<uint32_t>(127 - shift) << 23);
 #pragma unroll 4
       for (int i = 0; i < PASSES; ++i) {
         uint4* at = reinterpret_cast<uint4*>(q_at + i * 4 * PER * 128);
         const uint4 v = *at;
-        uint4 h;   // channels in the order of the codes: (0, 2), (1, 3) of every four
-        h.x = half2_bits(bf16lo(v.x) * up, bf16lo(v.y) * up);
-        h.y = half2_bits(bf16hi(v.x) * up, bf16hi(v.y) * up);
-        h.z = half2_bits(bf16lo(v.z) * up, bf16lo(v.w) * up);
-        h.w = half2_bits(bf16hi(v.z) * up, bf16hi(v.w) * up);
-        *at = h;
+        *at = make_uint4(half2_bits(bf16lo(v.x) * up, bf16hi(v.x) * up), half2_bits(bf16lo(v.y) * up, bf16hi(v.y) * up),
+                         half2_bits(bf16lo(v.z) * up, bf16hi(v.z) * up), half2_bits(bf16lo(v.w) * up, bf16hi(v.w) * up));
       }
       fence_proxy_async_smem();
       mbar_arrive(&q_full);
@@ -445,7 +438,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         mbar_wait(&sc_full[s], (n_step / SRING) & 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
         mbar_wait(&s_full[t], n_step & 1, abortp, p.err, CS_ERR_TIMEOUT_MMA);
         tc_fence_after();
-        const float2 sc = s_scale[s];
+        const float4 sc = s_scale[s];
         const int nvalid = lim - (it.j0 + j) * KV8_PAGE;       // visible keys of the page (may be negative or beyond 128)
         // first pass: the largest S of the row
         float mx0 = -INFINITY, mx1 = -INFINITY;
@@ -524,7 +517,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         {
           float s0, s1;
           unpack2(add2(sum_a, sum_b), s0, s1);
-          l += (s0 + s1) * ex2(-sc.y);
+          l += (s0 + s1) * sc.z;
         }
         tmem_wait_st();
         tc_fence_before();
@@ -541,7 +534,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         p.ws_ml[(row * p.splits + it.split) * 2] = m;
         p.ws_ml[(row * p.splits + it.split) * 2 + 1] = l;
       }
-      const float inv = p.splits > 1 ? 256.f : (l == 0.f ? 0.f : 256.f / l);          // 2^8: codes_to_half gives code / 2^8
+      const float inv = p.splits > 1 ? 1.f : (l == 0.f ? 0.f : 1.f / l);
       __nv_bfloat16* dst = p.o + static_cast<long long>(it.q_beg + tok) * p.o_tok + (it.h0 + g) * p.o_head;
       float* part = p.splits > 1 ? p.ws_o + (row * p.splits + it.split) * D : nullptr;
 #pragma unroll 1
@@ -555,9 +548,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
           for (int i = 0; i < 16; ++i) o[i] = 0u;
         }
         if (!row_ok) continue;
-        float f[16];   // back from (0, 2), (1, 3)
+        float f[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(o[(i & ~3) + ((i & 1) << 1) + ((i >> 1) & 1)]) * inv;
+        for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(o[i]) * inv;
         if (p.splits > 1) {
 #pragma unroll
           for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(part + c * 16 + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);

@@ -4,8 +4,8 @@ Tolerances.  A stored code is off by at most half a step of e4m3: 2^-4 of the va
 bf16 output is off by 2^-8 of its value.  Inside the attention a key's weight (probability times value scale) may be rounded
 to fp16: off by 2^-11 of it, or by half a step of the subnormals, 2^-25, where the largest weight is at least 2^6; so by
 2^-31 of the largest, for every code of the row.  With more than one query per sequence the keys and values themselves
-(code times scale) are rounded to fp16 once: off by 2^-11 of them, or by half a step of the subnormals, which is 2^-30 of
-the largest scale of their page (a power of two brings that scale to at least 2^13 when a code stands for code / 2^8).
+(code times scale) are rounded to fp16 once: off by 2^-11 of them, or by half a step of the subnormals, which is at most
+2^-30 of the largest scale of their page (a power of two brings that scale to at least 2^6).
 Scores are fp32 sums whose error is at most (d + 4) * 2^-24 times the sum of the magnitudes of
 their products, and an error e of a score changes its probability, and at most as much the normaliser, by e.
 """
