@@ -447,7 +447,6 @@ def attention_paged(q, cache, block_table, kv_len, cu_q, max_q_len: int, scale: 
 # --------------------------------------------------------------------------------------------
 KV_FP8_PAGE = reference.KV_FP8_PAGE
 KV_FP8_HEAD_DIMS = (64, 128)     # head widths the CUDA kernels are built for
-KV_FP8_MAX_SPLITS = 16           # parts the pages of one prompt tile are cut into when there are few tiles
 
 
 def kv_cache_fp8(num_pages: int, kv_heads: int, d: int, device: torch.device | str | None = None) -> torch.Tensor:
@@ -546,7 +545,7 @@ def attention_paged_fp8(q: torch.Tensor, cache: torch.Tensor, block_table: torch
 
     With one query per sequence (``max_q_len`` 1 and as many rows as sequences) keys and values take part exactly as they
     are cached; with more they are rounded to fp16 once (code times scale, 11 bits).  The lengths are read on the device:
-    a captured call follows them from replay to replay, within the table's width and ``max_q_len``.
+    a captured call follows them from replay to replay, within the table's width and the number of queries.
 
     Keys beyond the table or pages outside the cache raise on the CPU; on a GPU they are not read (the result of that
     sequence is then meaningless) and :func:`check_error` reports them."""
@@ -579,7 +578,7 @@ def attention_paged_fp8(q: torch.Tensor, cache: torch.Tensor, block_table: torch
     if Tq == 0 or B == 0 or max_q_len == 0:
         return out
     lib = _lib.load()
-    width, group = block_table.shape[1], Hq // Hkv
+    width = block_table.shape[1]
     # scratch belongs to the call: calls on several streams, and captured graphs, never share it
     if max_q_len == 1 and Tq == B:
         nbytes = lib.cs_attention_decode_fp8_ws_bytes(Hq, Hkv, d)
@@ -589,20 +588,13 @@ def attention_paged_fp8(q: torch.Tensor, cache: torch.Tensor, block_table: torch
                                          Hkv, d, scale, ws.data_ptr(), nbytes, _stream()), "cs_attention_decode_fp8")
         _count(2)
         return out
-    # few items (a pair of 128-row tiles of one sequence and key head each): their pages are spread over idle SMs
-    items = B * Hkv * -(-max_q_len // (2 * (128 // min(group, 128)))) * -(-group // 128)
-    splits = 1
-    if 2 * items <= 148 and width > 3:
-        splits = max(1, min(lib.cs_sm_count() // items, width // 2, KV_FP8_MAX_SPLITS))
-    ws, nbytes = None, 0
-    if splits > 1:
-        nbytes = Tq * Hq * splits * (d + 2) * 4
-        ws = cache.new_empty(nbytes)
+    nbytes = lib.cs_attention_prefill_fp8_ws_bytes(Tq, B, Hq, Hkv, d, width)
+    ws = cache.new_empty(nbytes)
     _chk(lib.cs_attention_prefill_fp8(q.data_ptr(), q.stride(0), cache.data_ptr(), cache.shape[0], out.data_ptr(), out.stride(0),
                                       out.stride(1), cu_q.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(), block_table.stride(0),
-                                      width, B, Tq, max_q_len, Hq, Hkv, d, scale, 1 if causal else 0, splits, _ptr(ws), nbytes,
-                                      _stream()), "cs_attention_prefill_fp8")
-    _count(2 if splits > 1 else 1)
+                                      width, B, Tq, Hq, Hkv, d, scale, 1 if causal else 0, ws.data_ptr(), nbytes, _stream()),
+         "cs_attention_prefill_fp8")
+    _count(2)
     return out
 
 

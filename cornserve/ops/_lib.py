@@ -63,7 +63,8 @@ _SIGNATURES = {
     "cs_quant_fp8_rows": ([P, L, I, I, P, L, P, L, P], I),
     "cs_kv_copy_pages": ([P, P, L, L, L, I, I, I, I, P, P, P], I),
     "cs_rope_kv_write_fp8": ([P, L, I, I, I, I, P, P, P, F, P, P, P, L, P], I),
-    "cs_attention_prefill_fp8": ([P, L, P, L, P, L, L, P, P, P, L, I, I, I, I, I, I, I, F, I, I, P, L, P], I),
+    "cs_attention_prefill_fp8": ([P, L, P, L, P, L, L, P, P, P, L, I, I, I, I, I, I, F, I, P, L, P], I),
+    "cs_attention_prefill_fp8_ws_bytes": ([L, L, I, I, I, L], L),
     "cs_attention_decode_fp8": ([P, L, P, L, P, L, L, P, P, L, I, I, I, I, I, F, P, L, P], I),
     "cs_attention_decode_fp8_ws_bytes": ([I, I, I], L),
     "cs_enable_peer_access": ([I], I),

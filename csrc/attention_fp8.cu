@@ -21,8 +21,12 @@
 //                    tensor cores work for the other.
 // The codes are converted once per 256 query rows.  They are not staged in shared memory as bytes: its bandwidth is what
 // the products need most of (192 KB of operands per page and tile pair), so the preparation warps load them straight into
-// registers.  Few items (short chunks over a long cache) split the pages of an item over several CTAs and a
-// second kernel joins the parts.
+// registers.
+//
+// Work: the items (a tile pair of one sequence and key head, and all its pages) form one list; the CTAs cut it, on the
+// device from the lengths, into runs of equal cost (visible keys, plus a constant per item).  An item that a cut goes
+// through is worked on by two or more CTAs, which leave partial sums that a second kernel joins.  So prompts of any mix of
+// lengths load all SMs alike, and a short chunk over a long cache is spread over the whole GPU.
 #include <math.h>
 
 #include "kv_fp8.cuh"
@@ -37,59 +41,138 @@ constexpr float M_NONE = -3.0e38f;         // running maximum before the first k
 
 static_assert(SRING >= RING + 2, "scalars outlive their tile by a page");
 
+constexpr int ITEM_COST = 3 * KV8_PAGE;     // what an item costs beside its keys, in keys
+constexpr int MIN_RUN = 4 * KV8_PAGE;       // no CTA for less
+constexpr int PAIR_ROWS = 256;
+
 struct PrefillParams {
   const __nv_bfloat16* q; long long q_tok;              // heads follow each other; every token on a 16-byte boundary
   __nv_bfloat16* o; long long o_tok, o_head; int o_vec; // o_vec: 16-byte stores are aligned
   const uint8_t* cache; int num_pages;
   const int* block_table; long long bt_stride; int bt_width;
   const int* kv_len; const int* cu_q;
-  int B, Hq, Hkv, G, head_blocks, causal;               // G query heads of a key head per tile row block
-  int tok_per_tile, max_pairs, total_items, splits;
+  int B, Tq, Hq, Hkv, G, blocks, causal;                // G query heads of a key head per tile row block; blocks = Hkv * row blocks
+  int tok_per_tile;
   float scale_log2;
-  float* ws_o;     // [Tq * Hq, splits, D] sums of the parts
-  float* ws_ml;    // [Tq * Hq, splits, 2] their maximum and normaliser
+  float* ws_o;     // [ctas, 2, 256, D] partial sums: slot 0 = the first item of a CTA, begun by another, slot 1 = its last
+  float* ws_ml;    // [ctas, 2, 256, 2] their maximum and normaliser
+  int4* ws_item;   // [ctas, 2] the items (sequence, row block, pair), sequence -1 = none
   uint32_t idesc_s, idesc_pv;
   int* err;
 };
 
-// One work item: a pair of query tiles of one sequence and key head (block), and a range of its pages.
-struct Item {
-  int seq, hk, h0, n_heads, q_beg, q_len, t0, k_len, shift, j0, n, split;
-  bool valid;
+// Lengths of a sequence, brought into the bounds of q and of the table.
+struct Seq {
+  int q_beg, q_len, k_len, shift;           // causal: query i sees keys j <= i + shift
 };
-
-__device__ __forceinline__ Item get_item(const PrefillParams& p, int w) {
-  Item it;
-  it.split = w % p.splits;
-  w /= p.splits;
-  const int blocks = p.Hkv * p.head_blocks, hb = w % blocks;
-  w /= blocks;
-  it.seq = w % p.B;
-  const int back = w / p.B;                 // the last pairs of every sequence, which see the most keys, come first
-  it.hk = hb / p.head_blocks;
-  const int first = (hb - it.hk * p.head_blocks) * p.G, group = p.Hq / p.Hkv;
-  it.h0 = it.hk * group + first;
-  it.n_heads = min(p.G, group - first);
-  it.q_beg = p.cu_q[it.seq];
-  it.q_len = p.cu_q[it.seq + 1] - it.q_beg;
-  const int pair_tok = 2 * p.tok_per_tile, pairs = (it.q_len + pair_tok - 1) / pair_tok;
-  it.valid = back < pairs;
-  it.t0 = (pairs - 1 - back) * pair_tok;
-  const int len = p.kv_len[it.seq];
+__device__ __forceinline__ Seq get_seq(const PrefillParams& p, int s) {
+  const int a = min(max(p.cu_q[s], 0), p.Tq), b = min(p.cu_q[s + 1], p.Tq), len = p.kv_len[s];
   const long long cap = static_cast<long long>(p.bt_width) * KV8_PAGE;
-  it.k_len = len < 0 ? 0 : (len > cap ? static_cast<int>(cap) : len);
-  it.shift = len - it.q_len;                // causal: token i sees keys j <= i + shift
-  const int end = p.causal ? min(it.k_len, min(it.q_len, it.t0 + pair_tok) + it.shift) : it.k_len;
-  const int pages = it.valid && end > 0 ? (end + KV8_PAGE - 1) / KV8_PAGE : 0;
-  it.j0 = static_cast<int>(static_cast<long long>(it.split) * pages / p.splits);
-  it.n = static_cast<int>(static_cast<long long>(it.split + 1) * pages / p.splits) - it.j0;
-  return it;
+  Seq q;
+  q.q_beg = a;
+  q.q_len = max(b - a, 0);
+  q.k_len = len < 0 ? 0 : (len > cap ? static_cast<int>(cap) : len);
+  q.shift = len - q.q_len;
+  return q;
+}
+__device__ __forceinline__ int pairs_of(const PrefillParams& p, const Seq& q) { return (q.q_len + 2 * p.tok_per_tile - 1) / (2 * p.tok_per_tile); }
+// Pages that pair k of a sequence looks at.
+__device__ __forceinline__ int pages_of(const PrefillParams& p, const Seq& q, int k) {
+  const int end = p.causal ? min(q.k_len, min(q.q_len, (k + 1) * 2 * p.tok_per_tile) + q.shift) : q.k_len;
+  return end > 0 ? (end + KV8_PAGE - 1) / KV8_PAGE : 0;
+}
+// a / b for a >= 0 and b > 0; costs fit 32 bits but for huge batches
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
+}
+// Cost of the first n pairs of a sequence (one row block): a sum over an arithmetic progression.
+__device__ __forceinline__ long long cost_of(const PrefillParams& p, const Seq& q, int n) {
+  if (!p.causal) return static_cast<long long>(n) * (q.k_len + ITEM_COST);
+  const int step = 2 * p.tok_per_tile;
+  const int k0 = q.shift >= 0 ? 0 : min(n, (-q.shift) / step);       // pairs that end before the first key
+  const long long m = n - k0;
+  return m * q.shift + step * (m * (k0 + 1) + m * (m - 1) / 2) + static_cast<long long>(n) * ITEM_COST;
 }
 
-// CTA b walks the items in a snake (0 .. g-1, then g-1 .. 0, ...): with items in falling order of size this evens out.
-__device__ __forceinline__ int item_at(int round) {
-  const int g = gridDim.x, b = blockIdx.x;
-  return round * g + ((round & 1) ? g - 1 - b : b);
+// A place in the list: page `page` of pair `pair` of row block `blk` of a sequence.
+struct Pos { int seq, blk, pair, page; };
+
+// The place at distance r (cost units) into the row blocks of sequence `seq`.  Cuts that would leave less than two pages of
+// an item on one side move to its edge.
+__device__ __forceinline__ Pos place_at(const PrefillParams& p, int seq, long long r) {
+  const Seq q = get_seq(p, seq);
+  const int pairs = pairs_of(p, q);
+  const long long per_blk = cost_of(p, q, pairs);
+  Pos at{seq, static_cast<int>(quotient(r, per_blk)), 0, 0};
+  r -= at.blk * per_blk;
+  int lo = 0, hi = pairs;                   // the pair with cost_of(lo) <= r < cost_of(lo + 1)
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (cost_of(p, q, mid) <= r) lo = mid; else hi = mid;
+  }
+  at.pair = lo;
+  const int pages = pages_of(p, q, lo), cut = static_cast<int>(max(0ll, r - cost_of(p, q, lo) - ITEM_COST + KV8_PAGE / 2) / KV8_PAGE);
+  if (cut < 2) return at;
+  if (pages - cut >= 2) { at.page = cut; return at; }
+  if (++at.pair == pairs) {                 // on to the next item
+    at.pair = 0;
+    if (++at.blk == p.blocks) { at.blk = 0; ++at.seq; }
+  }
+  return at;
+}
+
+// One visit of a CTA to an item: pages [j0, j0 + n) of a pair of query tiles of one sequence and key head (row block).
+struct Item {
+  int seq, hk, h0, n_heads, q_beg, q_len, t0, k_len, shift, j0, n;
+  bool whole;                               // all pages of the item
+};
+struct Walk { Pos at, end; };               // of one warp, in shared memory
+
+__device__ __forceinline__ void make_item(const PrefillParams& p, const Seq& q, int seq, int blk, int pair, Item& it) {
+  const int group = p.Hq / p.Hkv, per = p.blocks / p.Hkv;
+  it.seq = seq;
+  it.hk = blk / per;
+  const int first = (blk - it.hk * per) * p.G;
+  it.h0 = it.hk * group + first;
+  it.n_heads = min(p.G, group - first);
+  it.q_beg = q.q_beg; it.q_len = q.q_len; it.k_len = q.k_len; it.shift = q.shift;
+  it.t0 = pair * 2 * p.tok_per_tile;
+}
+
+// The next visit of this warp's walk (all lanes), or false.
+__device__ __forceinline__ bool next_visit(const PrefillParams& p, Walk* w, Item* out) {
+  Pos at = w->at;
+  const Pos end = w->end;
+  bool found = false;
+  Item it;
+  while (!found && at.seq < p.B) {
+    const Seq q = get_seq(p, at.seq);
+    const int pairs = pairs_of(p, q);
+    if (at.pair >= pairs) { at = Pos{at.seq + 1, 0, 0, 0}; continue; }     // no queries
+    const bool last = at.seq == end.seq && at.blk == end.blk && at.pair == end.pair;
+    if (at.seq > end.seq || (last && (end.page == 0 || at.page >= end.page))) break;
+    const int pages = pages_of(p, q, at.pair), stop = last ? min(end.page, pages) : pages;
+    make_item(p, q, at.seq, at.blk, at.pair, it);
+    it.j0 = at.page;
+    it.n = stop - at.page;
+    it.whole = at.page == 0 && stop == pages;
+    found = it.n > 0 || pages == 0;
+    if (last) {
+      at.page = max(end.page, 1);           // behind the end
+    } else {
+      at.page = 0;
+      if (++at.pair == pairs) {
+        at.pair = 0;
+        if (++at.blk == p.blocks) { at.blk = 0; ++at.seq; }
+      }
+    }
+  }
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) w->at = at;
+  __syncwarp();
+  if (found) *out = it;
+  return found;
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -144,6 +227,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
   __shared__ uint64_t q_full, q_empty, kv_full[2][RING], kv_empty[2][RING], sc_full[SRING], s_full[2], p_full[2], o_full[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
+  __shared__ Walk s_walk[THREADS / 32];
+  __shared__ Pos s_pos[2];
+  __shared__ long long s_sum[THREADS / 32], s_cut[2];
+  __shared__ int s_cut_seq[2];
   __shared__ uint32_t s_max[8], s_row[128];   // s_row: token in tile | head << 16 of a tile row
   __shared__ float4 s_scale[SRING];     // of a page: factor from S to base-2 exponents, F, 2^-F
 
@@ -164,12 +251,59 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
   tc_fence_after();
   pdl_wait();
   pdl_launch_dependents();
+  if (threadIdx.x < 2) p.ws_item[blockIdx.x * 2 + threadIdx.x] = make_int4(-1, 0, 0, 0);
+
+  // ------------------------------- this CTA's run of the list -------------------------------
+  // Thread i adds up the cost of `per` consecutive sequences (one, unless the batch is huge); a scan over the threads gives
+  // the total and who owns the two cuts.
+  {
+    const int per = (p.B + THREADS - 1) / THREADS, b0 = min(static_cast<int>(threadIdx.x) * per, p.B), b1 = min(b0 + per, p.B);
+    auto seq_cost = [&](int b) { const Seq q = get_seq(p, b); return cost_of(p, q, pairs_of(p, q)) * p.blocks; };
+    long long mine = 0;
+    for (int b = b0; b < b1; ++b) mine += seq_cost(b);
+    long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (lane == 31) s_sum[warp] = incl;
+    if (threadIdx.x < 2) { s_cut_seq[threadIdx.x] = p.B; s_cut[threadIdx.x] = 0; }
+    __syncthreads();
+    long long total = 0;
+    for (int w = 0; w < THREADS / 32; ++w) {
+      if (w == warp) incl += total;
+      total += s_sum[w];
+    }
+    const long long active = max(1ll, min(static_cast<long long>(gridDim.x), total / MIN_RUN)), quota = quotient(total, active), extra = total - quota * active;
+    for (int e = 0; e < 2; ++e) {
+      const long long c = blockIdx.x + e, r = c >= active ? total : quota * c + min(c, extra);
+      if (r >= incl - mine && r < incl) {
+        long long at = incl - mine;
+        int b = b0;
+        for (; b + 1 < b1; ++b) {
+          const long long x = seq_cost(b);
+          if (r < at + x) break;
+          at += x;
+        }
+        s_cut_seq[e] = b;
+        s_cut[e] = r - at;
+      }
+    }
+    __syncthreads();
+    if (warp < 2 && lane == 0) s_pos[warp] = s_cut_seq[warp] < p.B ? place_at(p, s_cut_seq[warp], s_cut[warp]) : Pos{p.B, 0, 0, 0};
+    __syncthreads();
+    if (lane == 0) s_walk[warp] = Walk{s_pos[0], s_pos[1]};
+    __syncwarp();
+  }
+  Walk* walk = &s_walk[warp];
   const uint32_t tmem = tmem_slot;      // S_0, S_1 at columns 0, 128 (P_t over the first half of S_t), O_0, O_1 at 256, 384
   volatile int* abortp = &abort_flag;
 
   // No role leaves its loops early when a wait gives up: later waits return at once, and all keep their barriers company.
   if (warp == 16) {
-    if (elect_one()) {
+    const bool leader = elect_one();
+    {
       // -------------------------------- MMA issuer --------------------------------
       const uint32_t q_addr = smem_u32(s_q), kv_addr = smem_u32(s_kv);
       uint32_t n_item = 0, n_p = 0;     // running counts: items, pages (steps of the softmax)
@@ -195,11 +329,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) umma_f16_ts(tmem + 256 + t * 128, a + kk * 8, b + kk * 128, p.idesc_pv, !(first && (k4 | kk) == 0));
       };
-      for (int round = 0; round * static_cast<int>(gridDim.x) < p.total_items; ++round) {
-        const int w = item_at(round);
-        if (w >= p.total_items) continue;
-        const Item it = get_item(p, w);
-        if (it.n == 0) continue;
+      Item visit;      // (copied: what has its address taken lives in memory)
+      while (next_visit(p, walk, &visit)) {
+        const Item it = visit;
+        if (it.n == 0 || !leader) continue;
         mbar_wait(&q_full, n_item & 1, abortp, p.err, CS_ERR_TIMEOUT_TMA);
         ++n_item;
         wait_kv(0, n_p);
@@ -330,17 +463,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
       fence_proxy_async_smem();
       mbar_arrive(&kv_full[kv][slot]);
     };
-    Item it;
-    auto next_item = [&](int round) {              // the next round that gives an item with pages (in `it`), or -1
-      for (; round * static_cast<int>(gridDim.x) < p.total_items; ++round) {
-        const int w = item_at(round);
-        if (w >= p.total_items) continue;
-        it = get_item(p, w);
-        if (it.n > 0) return round;
-      }
-      return -1;
-    };
-    for (int round = next_item(0); round >= 0; round = next_item(round + 1)) {
+    Item visit;
+    while (next_visit(p, walk, &visit)) {
+      const Item it = visit;
+      if (it.n == 0) continue;
       const uint8_t* head = p.cache + (static_cast<long long>(kv) * p.Hkv + it.hk) * kv8_block_bytes(D);
       const uint8_t* block = block_of(head, page_of(it, it.j0));
       fetch_scales(block);
@@ -423,11 +549,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + t * 128 + lane_off, tO = tmem + 256 + t * 128 + lane_off;
     uint32_t n_step = 0, n_item = 0;
-    for (int round = 0; round * static_cast<int>(gridDim.x) < p.total_items; ++round) {
-      const int w = item_at(round);
-      if (w >= p.total_items) continue;
-      const Item it = get_item(p, w);
-      if (!it.valid) continue;
+    Item visit;
+    while (next_visit(p, walk, &visit)) {
+      const Item it = visit;
       const int tok = it.t0 + t * p.tok_per_tile + tl;
       const bool row_ok = tl < p.tok_per_tile && tok < it.q_len && g < it.n_heads;
       const int lim = p.causal ? min(it.k_len, tok + it.shift + 1) : it.k_len;     // keys [0, lim) are visible
@@ -529,14 +653,16 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         ++n_item;
         tc_fence_after();
       }
-      const long long row = static_cast<long long>(it.q_beg + tok) * p.Hq + it.h0 + g;
-      if (p.splits > 1 && row_ok) {
-        p.ws_ml[(row * p.splits + it.split) * 2] = m;
-        p.ws_ml[(row * p.splits + it.split) * 2 + 1] = l;
+      // a partial sum goes to slot 0 when another CTA began the item, to slot 1 when this one did
+      const int slot = blockIdx.x * 2 + (it.j0 == 0 ? 1 : 0);
+      const long long row = static_cast<long long>(slot) * PAIR_ROWS + t * 128 + r;
+      if (!it.whole) {
+        if (row_ok) { p.ws_ml[row * 2] = m; p.ws_ml[row * 2 + 1] = l; }
+        if (threadIdx.x == 0) p.ws_item[slot] = make_int4(it.seq, it.h0, it.t0, 0);
       }
-      const float inv = p.splits > 1 ? 1.f : (l == 0.f ? 0.f : 1.f / l);
+      const float inv = !it.whole ? 1.f : (l == 0.f ? 0.f : 1.f / l);
       __nv_bfloat16* dst = p.o + static_cast<long long>(it.q_beg + tok) * p.o_tok + (it.h0 + g) * p.o_head;
-      float* part = p.splits > 1 ? p.ws_o + (row * p.splits + it.split) * D : nullptr;
+      float* part = p.ws_o + row * D;
 #pragma unroll 1
       for (int c = 0; c < D / 16; ++c) {
         uint32_t o[16];
@@ -551,7 +677,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         float f[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(o[i]) * inv;
-        if (p.splits > 1) {
+        if (!it.whole) {
 #pragma unroll
           for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(part + c * 16 + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
         } else if (p.o_vec) {
@@ -566,39 +692,47 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
       }
       tc_fence_before();
     }
-    // lengths that do not fit the table are reported
+    // lengths that do not fit the table or the queries are reported
     for (int b = blockIdx.x * 256 + threadIdx.x; b < p.B; b += gridDim.x * 256)
-      if (p.kv_len[b] > static_cast<long long>(p.bt_width) * KV8_PAGE) cs_set_error(p.err, CS_ERR_BAD_ARG);
+      if (p.kv_len[b] > static_cast<long long>(p.bt_width) * KV8_PAGE || p.cu_q[b] < 0 || p.cu_q[b + 1] < p.cu_q[b] || p.cu_q[b + 1] > p.Tq)
+        cs_set_error(p.err, CS_ERR_BAD_ARG);
   }
   tc_fence_before();
   __syncthreads();
   if (warp == 16) { tc_fence_after(); tmem_dealloc(tmem, 512); }
 }
 
-// Joins the parts of the rows of an item that was split: one warp per (token, head) row, parts in order.
+// Joins the items that several CTAs worked on: blocks (c, y) take rows 8 y .. + 7 of the item whose first part is the last of
+// CTA c, one warp per row.  The parts are slot 1 of CTA c and slot 0 of the CTAs behind it, read in order.
 template <int D>
-__global__ void __launch_bounds__(256) attention_prefill_fp8_join_kernel(const PrefillParams p) {
+__global__ void __launch_bounds__(256) attention_prefill_fp8_join_kernel(const PrefillParams p, int ctas) {
   pdl_wait();
   pdl_launch_dependents();
-  const long long row = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (row >= static_cast<long long>(p.cu_q[p.B]) * p.Hq || row < static_cast<long long>(p.cu_q[0]) * p.Hq) return;
-  float mx = M_NONE, l = 0.f;
-  for (int s = 0; s < p.splits; ++s) mx = fmaxf(mx, p.ws_ml[(row * p.splits + s) * 2]);
+  const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int4 item = p.ws_item[c * 2 + 1];
+  if (item.x < 0) return;
+  const int r = blockIdx.y * 8 + warp, rr = r & 127;
+  const int tl = rr / p.G, g = rr - tl * p.G;
+  const Seq q = get_seq(p, item.x);
+  const int group = p.Hq / p.Hkv, tok = item.z + (r >> 7) * p.tok_per_tile + tl;
+  if (tl >= p.tok_per_tile || tok >= q.q_len || item.y % group + g >= group) return;
+  auto same = [&](int4 o) { return o.x == item.x && o.y == item.y && o.z == item.z; };
+  auto row_of = [&](int i) { return (static_cast<long long>(c + i) * 2 + (i == 0 ? 1 : 0)) * PAIR_ROWS + r; };
+  float m = M_NONE, l = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int s = 0; s < p.splits; ++s) {
-    const long long at = row * p.splits + s;
-    const float e = ex2(p.ws_ml[at * 2] - mx);
-    l += p.ws_ml[at * 2 + 1] * e;
-    if (lane * 4 < D) {
-      const float4 v = *reinterpret_cast<const float4*>(p.ws_o + at * D + lane * 4);
-      acc.x += v.x * e; acc.y += v.y * e; acc.z += v.z * e; acc.w += v.w * e;
-    }
+  for (int i = 0; c + i < ctas; ++i) {
+    if (i > 0 && !same(p.ws_item[(c + i) * 2])) break;
+    const long long row = row_of(i);
+    const float mi = p.ws_ml[row * 2], li = p.ws_ml[row * 2 + 1];
+    const float4 v = lane * 4 < D ? *reinterpret_cast<const float4*>(p.ws_o + row * D + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+    const float mx = fmaxf(m, mi), a = ex2(m - mx), b = ex2(mi - mx);
+    m = mx;
+    l = l * a + li * b;
+    acc.x = acc.x * a + v.x * b; acc.y = acc.y * a + v.y * b; acc.z = acc.z * a + v.z * b; acc.w = acc.w * a + v.w * b;
   }
   if (lane * 4 >= D) return;
   const float inv = l == 0.f ? 0.f : 1.0f / l;
-  __nv_bfloat16* dst = p.o + row / p.Hq * p.o_tok + row % p.Hq * p.o_head + lane * 4;
+  __nv_bfloat16* dst = p.o + static_cast<long long>(q.q_beg + tok) * p.o_tok + (item.y + g) * p.o_head + lane * 4;
   const float f[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
   if (p.o_vec) {
     *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
@@ -609,7 +743,7 @@ __global__ void __launch_bounds__(256) attention_prefill_fp8_join_kernel(const P
 }
 
 template <int D>
-int launch_prefill(const PrefillParams& p, int grid, long long rows, cudaStream_t stream) {
+int launch_prefill(const PrefillParams& p, int grid, cudaStream_t stream) {
   static bool ready[64] = {false};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -10;
@@ -619,23 +753,39 @@ int launch_prefill(const PrefillParams& p, int grid, long long rows, cudaStream_
     ready[dev] = true;
   }
   if (cs_launch_pdl(attention_prefill_fp8_kernel<D>, dim3(grid), dim3(THREADS), Shape<D>::SMEM, stream, p) != cudaSuccess) return -10;
-  if (p.splits == 1) return 0;
-  return cs_launch_pdl(attention_prefill_fp8_join_kernel<D>, dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256), 0, stream, p) == cudaSuccess
-             ? 0 : -10;
+  if (grid == 1) return 0;
+  return cs_launch_pdl(attention_prefill_fp8_join_kernel<D>, dim3(grid, PAIR_ROWS / 8), dim3(256), 0, stream, p, grid) == cudaSuccess ? 0 : -10;
+}
+
+// CTAs of a call: no more than runs of the least length that the queries and tables could make up.
+int prefill_ctas(long long Tq, long long B, int Hq, int Hkv, long long bt_width) {
+  const int group = Hq / Hkv, G = group < 128 ? group : 128, pair = 2 * (128 / G);
+  const long long items = (Tq / pair + B) * Hkv * ((group + G - 1) / G);
+  const long long most = (items * (bt_width * KV8_PAGE + pair + ITEM_COST)) / MIN_RUN;
+  const int sms = cs_num_sms();
+  return most >= sms ? sms : (most < 1 ? 1 : static_cast<int>(most));
 }
 
 }  // namespace
 
+// Scratch of a call.
+CS_API long long cs_attention_prefill_fp8_ws_bytes(long long Tq, long long B, int Hq, int Hkv, int d, long long bt_width) {
+  if (Hkv <= 0 || Hq <= 0) return 0;
+  return prefill_ctas(Tq, B, Hq, Hkv, bt_width) * 2LL * (PAIR_ROWS * (d + 2LL) * 4 + 16);
+}
+
 // q: [Tq, Hq, d] with contiguous heads, tokens q_tok elements apart and on 16-byte boundaries; o: [Tq, Hq, d] with token and
-// head strides in elements; d is 64 or 128.  No sequence has more than max_q_len queries.  splits > 1 cuts the pages of
-// every item into that many parts; ws then holds Tq * Hq * splits * (d + 2) floats that no call on another stream uses.
+// head strides in elements; d is 64 or 128.  ws: cs_attention_prefill_fp8_ws_bytes of scratch that no call on another stream
+// uses.
 CS_API int cs_attention_prefill_fp8(const void* q, long long q_tok, const void* cache, long long num_pages, void* o, long long o_tok,
                                     long long o_head, const void* cu_q, const void* kv_len, const void* block_table, long long bt_stride,
-                                    int bt_width, int B, int Tq, int max_q_len, int Hq, int Hkv, int d, float scale, int causal, int splits,
-                                    void* ws, long long ws_bytes, void* stream) {
-  if (B <= 0 || Tq <= 0 || max_q_len <= 0) return 0;
+                                    int bt_width, int B, int Tq, int Hq, int Hkv, int d, float scale, int causal, void* ws,
+                                    long long ws_bytes, void* stream) {
+  if (B <= 0 || Tq <= 0) return 0;
   if ((d != 64 && d != 128) || Hkv <= 0 || Hq <= 0 || Hq % Hkv != 0 || num_pages <= 0 || num_pages > 0x7fffffffLL) return -1;
   if ((reinterpret_cast<uintptr_t>(q) & 15) || (q_tok & 7)) return -1;
+  if (ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 15) || ws_bytes < cs_attention_prefill_fp8_ws_bytes(Tq, B, Hq, Hkv, d, bt_width))
+    return -5;
   PrefillParams p{};
   p.q = (const __nv_bfloat16*)q; p.q_tok = q_tok;
   p.o = (__nv_bfloat16*)o; p.o_tok = o_tok; p.o_head = o_head;
@@ -644,25 +794,17 @@ CS_API int cs_attention_prefill_fp8(const void* q, long long q_tok, const void* 
   p.block_table = (const int*)block_table; p.bt_stride = bt_stride; p.bt_width = bt_width;
   p.kv_len = (const int*)kv_len; p.cu_q = (const int*)cu_q;
   const int group = Hq / Hkv;
-  p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.G = group < 128 ? group : 128; p.causal = causal;
-  p.head_blocks = (group + p.G - 1) / p.G;
+  p.B = B; p.Tq = Tq; p.Hq = Hq; p.Hkv = Hkv; p.G = group < 128 ? group : 128; p.causal = causal;
+  p.blocks = Hkv * ((group + p.G - 1) / p.G);
   p.tok_per_tile = 128 / p.G;
-  p.max_pairs = (max_q_len + 2 * p.tok_per_tile - 1) / (2 * p.tok_per_tile);
   p.scale_log2 = scale * 1.4426950408889634f;
   p.err = cs_error_word();
   p.idesc_s = umma_idesc_f16(128, 128, 0, 0);
   p.idesc_pv = umma_idesc_f16(128, d, 0, 1);
-  p.splits = splits < 1 ? 1 : splits;
-  const long long rows = static_cast<long long>(Tq) * Hq;
-  if (p.splits > 1) {
-    if (ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 15) || rows * p.splits * (d + 2) * 4 > ws_bytes) return -5;
-    p.ws_o = reinterpret_cast<float*>(ws);
-    p.ws_ml = p.ws_o + rows * p.splits * d;
-  }
-  const long long total = static_cast<long long>(p.max_pairs) * B * Hkv * p.head_blocks * p.splits;
-  if (total > 0x3fffffffLL || (rows + 7) / 8 > 0x7fffffffLL) return -1;
-  p.total_items = static_cast<int>(total);
-  const int grid = p.total_items < cs_num_sms() ? p.total_items : cs_num_sms();
+  const int ctas = prefill_ctas(Tq, B, Hq, Hkv, bt_width);
+  p.ws_item = reinterpret_cast<int4*>(ws);
+  p.ws_o = reinterpret_cast<float*>(p.ws_item + ctas * 2);
+  p.ws_ml = p.ws_o + ctas * 2LL * PAIR_ROWS * d;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return d == 128 ? launch_prefill<128>(p, grid, rows, st) : launch_prefill<64>(p, grid, rows, st);
+  return d == 128 ? launch_prefill<128>(p, ctas, st) : launch_prefill<64>(p, ctas, st);
 }

@@ -321,7 +321,6 @@ def test_a_nan_row_spreads_only_to_the_queries_that_see_it(n):
 def test_tables_and_lengths_that_do_not_fit_are_reported(new):
     lens = [300, 64, 10, 129, 500, 40]
     q, cache, table, kv_len, cu = _setup(lens, new, 8, 2, 64, seed=13, poison=False)
-    good = ops.attention_paged_fp8(q, cache, table, kv_len, cu, max(new))
     bad_table = table.clone()
     bad_table[0, 1] = cache.shape[0]
     bad_table[4, 2] = -1
@@ -336,7 +335,9 @@ def test_tables_and_lengths_that_do_not_fit_are_reported(new):
     with pytest.raises(RuntimeError, match="bad argument"):
         ops.check_error("length")
     a, b = sum(new[:1]), sum(new[:2])
-    assert torch.equal(out[:a], good[:a]) and torch.equal(out[b:], good[b:])     # the others are unharmed
+    # the others are right (their sums may be cut elsewhere than with the good length, so not the same to the last bit)
+    _check(out[:a], q[:a], cache, table[:1], lens[:1], new[:1])
+    _check(out[b:], q[b:], cache, table[2:], lens[2:], new[2:])
 
 
 def test_results_do_not_depend_on_the_run_or_the_batch_order():
