@@ -41,7 +41,7 @@ constexpr float M_NONE = -3.0e38f;         // running maximum before the first k
 
 static_assert(SRING >= RING + 2, "scalars outlive their tile by a page");
 
-constexpr int ITEM_COST = 3 * KV8_PAGE;     // what an item costs beside its keys, in keys
+constexpr int ITEM_COST = 7 * KV8_PAGE / 2; // what an item costs beside its keys, in keys
 constexpr int MIN_RUN = 4 * KV8_PAGE;       // no CTA for less
 constexpr int PAIR_ROWS = 256;
 
@@ -424,22 +424,26 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
       const __half2 y = __hfma2(x, h, __hmul2(x, l));
       return *reinterpret_cast<const uint32_t*>(&y);
     };
+    // The scalars of page n, once its tile's place was free.  Their own place was that of page n - SRING, which both softmax
+    // groups are done with: the tile of page n - RING is free only behind products that waited for the weights of page
+    // n - RING - 1 or a later one.  (The factor is not 0, also for a scale of 0: a hidden key's -inf times the factor has to
+    // stay -inf.)
+    auto publish = [&](int e, float cq) {
+      if (tid != 0) return;
+      const uint32_t s = n % SRING;
+      if (kv == 0) {
+        s_scale[s].x = fmaxf(cq * __uint_as_float(static_cast<uint32_t>(127 + e) << 23), 1e-37f);
+      } else {
+        s_scale[s].y = static_cast<float>(e);
+        s_scale[s].z = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+      }
+      mbar_arrive(&sc_full[s]);
+    };
     // Convert the tile in hand and, chunk by chunk, fetch the next one into the registers that become free.
-    auto convert = [&](uint32_t parts, const uint8_t* next, int e, float cq) {
+    auto convert = [&](uint32_t parts, const uint8_t* next, int e, float cq, bool pub) {
       const uint32_t slot = n % RING;
       mbar_wait(&kv_empty[kv][slot], ((n / RING) & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
-      if (tid == 0) {
-        // The page's scalars.  Their place was that of page n - SRING, which both softmax groups are done with: the tile of
-        // page n - RING is free only behind products that waited for the weights of page n - RING - 1 or a later one.
-        // (The factor is not 0, also for a scale of 0: a hidden key's -inf times the factor has to stay -inf.)
-        const uint32_t s = n % SRING;
-        if (kv == 0) s_scale[s].x = fmaxf(cq * __uint_as_float(static_cast<uint32_t>(127 + e) << 23), 1e-37f);
-        else {
-          s_scale[s].y = static_cast<float>(e);
-          s_scale[s].z = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-        }
-        mbar_arrive(&sc_full[s]);
-      }
+      if (pub) publish(e, cq);
       uint8_t* tile = s_kv + (kv * RING + slot) * TILE;
       if (rows < KV8_PAGE) {                       // what lies behind the keys may be anything
 #pragma unroll
@@ -473,73 +477,82 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
 #pragma unroll
       for (int i = 0; i < ITER; ++i) fetch_codes(block, i);
       int page = page_of(it, it.j0 + 1);
-      // Queries, one tile per group, D / 8 lanes per row: copied as they are to the place where their fp16 form will be, all
-      // in flight at once; then the largest finite magnitude of both tiles, and fp16 with a common scale in place.
-      constexpr int LANES = D / 8, PER = 32 / LANES, PASSES = 32 / PER;     // lanes per row, rows per warp and pass, passes
-      const int ch = lane % LANES, row_w = (warp & 3) * PER + lane / LANES;
-      // row i * 4 * PER + row_w: its swizzle is the same in all passes (4 * PER is a multiple of 8)
-      uint8_t* q_at = s_q + kv * TILE + (ch >> 3) * ATOM + row_w * 128 + (((ch & 7) ^ (row_w & 7)) << 4);
-      mbar_wait(&q_empty, (n_item & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
-      ++n_item;
-      {
-        const int t0 = it.t0 + kv * p.tok_per_tile, n_tok = min(p.tok_per_tile, it.q_len - t0);
-        const __nv_bfloat16* src0 = p.q + (it.q_beg + (n_tok > 0 ? t0 : 0)) * p.q_tok + it.h0 * D + ch * 8;
-        const uint32_t q_sm = smem_u32(q_at);
-#pragma unroll 4
-        for (int i = 0; i < PASSES; ++i) {
-          const uint32_t rc = s_row[i * 4 * PER + row_w];                   // token in tile | head << 16
-          const int tl = rc & 0xffff, g = rc >> 16;
-          const bool ok = tl < n_tok && g < it.n_heads;
-          const __nv_bfloat16* src = ok ? src0 + tl * p.q_tok + g * D : src0;
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(q_sm + i * 4 * PER * 128), "l"(src), "r"(ok ? 16 : 0) : "memory");
-        }
-      }
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      auto largest = [&](bool finite_only) {
-        uint32_t m2 = 0;                           // two 16-bit maxima
-#pragma unroll 8
-        for (int i = 0; i < PASSES; ++i) {
-          const uint4 v = *reinterpret_cast<const uint4*>(q_at + i * 4 * PER * 128);
-          uint32_t w[4] = {v.x & 0x7fff7fffu, v.y & 0x7fff7fffu, v.z & 0x7fff7fffu, v.w & 0x7fff7fffu};
-          if (finite_only) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) w[k] = ((w[k] & 0xffffu) < 0x7f80u ? w[k] & 0xffffu : 0u) | ((w[k] >> 16) < 0x7f80u ? w[k] & 0xffff0000u : 0u);
-          }
-          m2 = __vmaxu2(m2, __vmaxu2(__vmaxu2(w[0], w[1]), __vmaxu2(w[2], w[3])));
-        }
-        const uint32_t mx = __reduce_max_sync(0xffffffffu, max(m2 & 0xffffu, m2 >> 16));
-        if (lane == 0) s_max[warp - 8] = mx;
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        uint32_t all = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) all = max(all, s_max[i]);
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        return all;
-      };
-      uint32_t mx = largest(false);
-      if (mx >= 0x7f80u) mx = largest(true);       // (an infinity or NaN makes its own row NaN and nothing else)
-      const int shift = min(max(127 + 14 - static_cast<int>(mx >> 7), -110), 110);   // the largest element into [2^14, 2^15)
-      // a negative scale turns the queries around, so that the largest score is the largest S
-      const float up = copysignf(__uint_as_float(static_cast<uint32_t>(127 + shift) << 23), p.scale_log2);
-      const float cq = fabsf(p.scale_log2) * __uint_as_float(static_cast<uint32_t>(127 - shift) << 23);
-#pragma unroll 4
-      for (int i = 0; i < PASSES; ++i) {
-        uint4* at = reinterpret_cast<uint4*>(q_at + i * 4 * PER * 128);
-        const uint4 v = *at;
-        *at = make_uint4(half2_bits(bf16lo(v.x) * up, bf16hi(v.x) * up), half2_bits(bf16lo(v.y) * up, bf16hi(v.y) * up),
-                         half2_bits(bf16lo(v.z) * up, bf16hi(v.z) * up), half2_bits(bf16lo(v.w) * up, bf16hi(v.w) * up));
-      }
-      fence_proxy_async_smem();
-      mbar_arrive(&q_full);
+      float cq = 0.f;
 #pragma unroll 1
       for (int j = it.j0; j < it.j0 + it.n; ++j, ++n) {
+        // the tile of a page, and the next page's scales and codes on their way
         uint32_t parts;
         rows = it.k_len - j * KV8_PAGE;
         const int e = multiplier(parts);
         if (j + 1 < it.j0 + it.n) block = block_of(head, page);   // (behind the last page the same one is read again)
         fetch_scales(block);
         page = page_of(it, j + 2);
-        convert(parts, block, e, cq);
+        convert(parts, block, e, cq, j > it.j0);
+        if (j > it.j0) continue;
+        // The queries come behind the first tile, which does not need them: the item before is still at work on its own.
+        // Queries, one tile per group, D / 8 lanes per row: copied as they are to the place where their fp16 form will be, all
+        // in flight at once; then the largest finite magnitude of both tiles, and fp16 with a common scale in place.
+        constexpr int LANES = D / 8, PER = 32 / LANES, PASSES = 32 / PER;     // lanes per row, rows per warp and pass, passes
+        const int ch = lane % LANES, row_w = (warp & 3) * PER + lane / LANES;
+        // row i * 4 * PER + row_w: its swizzle is the same in all passes (4 * PER is a multiple of 8)
+        uint8_t* q_at = s_q + kv * TILE + (ch >> 3) * ATOM + row_w * 128 + (((ch & 7) ^ (row_w & 7)) << 4);
+        mbar_wait(&q_empty, (n_item & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
+        ++n_item;
+        {
+          const int t0 = it.t0 + kv * p.tok_per_tile, n_tok = min(p.tok_per_tile, it.q_len - t0);
+          const __nv_bfloat16* src0 = p.q + (it.q_beg + (n_tok > 0 ? t0 : 0)) * p.q_tok + it.h0 * D + ch * 8;
+          const uint32_t q_sm = smem_u32(q_at);
+#pragma unroll 8
+          for (int i = 0; i < PASSES; ++i) {
+            const uint32_t rc = s_row[i * 4 * PER + row_w];                   // token in tile | head << 16
+            const int tl = rc & 0xffff, g = rc >> 16;
+            const bool ok = tl < n_tok && g < it.n_heads;
+            const __nv_bfloat16* src = ok ? src0 + tl * p.q_tok + g * D : src0;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(q_sm + i * 4 * PER * 128), "l"(src), "r"(ok ? 16 : 0) : "memory");
+          }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        auto largest = [&](bool finite_only) {
+          uint32_t m2 = 0;                           // two 16-bit maxima
+#pragma unroll 8
+          for (int i = 0; i < PASSES; ++i) {
+            const uint4 v = *reinterpret_cast<const uint4*>(q_at + i * 4 * PER * 128);
+            uint32_t w[4] = {v.x & 0x7fff7fffu, v.y & 0x7fff7fffu, v.z & 0x7fff7fffu, v.w & 0x7fff7fffu};
+            if (finite_only) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) w[k] = ((w[k] & 0xffffu) < 0x7f80u ? w[k] & 0xffffu : 0u) | ((w[k] >> 16) < 0x7f80u ? w[k] & 0xffff0000u : 0u);
+            }
+            m2 = __vmaxu2(m2, __vmaxu2(__vmaxu2(w[0], w[1]), __vmaxu2(w[2], w[3])));
+          }
+          const uint32_t mx = __reduce_max_sync(0xffffffffu, max(m2 & 0xffffu, m2 >> 16));
+          if (lane == 0) s_max[warp - 8] = mx;
+          asm volatile("bar.sync 1, 256;" ::: "memory");
+          uint32_t all = 0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) all = max(all, s_max[i]);
+          asm volatile("bar.sync 1, 256;" ::: "memory");
+          return all;
+        };
+        uint32_t mx = largest(false);
+        if (mx >= 0x7f80u) mx = largest(true);       // (an infinity or NaN makes its own row NaN and nothing else)
+        const int shift = min(max(127 + 14 - static_cast<int>(mx >> 7), -110), 110);   // the largest element into [2^14, 2^15)
+        // a negative scale turns the queries around, so that the largest score is the largest S
+        const float up = copysignf(__uint_as_float(static_cast<uint32_t>(127 + shift) << 23), p.scale_log2);
+        cq = fabsf(p.scale_log2) * __uint_as_float(static_cast<uint32_t>(127 - shift) << 23);
+#pragma unroll 1
+        for (int i0 = 0; i0 < PASSES; i0 += 4) {
+          uint4 v[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint4*>(q_at + (i0 + i) * 4 * PER * 128);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<uint4*>(q_at + (i0 + i) * 4 * PER * 128) =
+                make_uint4(half2_bits(bf16lo(v[i].x) * up, bf16hi(v[i].x) * up), half2_bits(bf16lo(v[i].y) * up, bf16hi(v[i].y) * up),
+                           half2_bits(bf16lo(v[i].z) * up, bf16hi(v[i].z) * up), half2_bits(bf16lo(v[i].w) * up, bf16hi(v[i].w) * up));
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(&q_full);
+        publish(e, cq);
       }
     }
   } else {
