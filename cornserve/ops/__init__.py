@@ -461,16 +461,19 @@ def kv_cache_fp8(num_pages: int, kv_heads: int, d: int, device: torch.device | s
 def kv_cache_fp8_views(cache: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """``(codes [pages, 2, kv_heads, 128, d] float8_e4m3fn, scales [pages, 2, kv_heads, 128] fp32)``, views of ``cache``:
     row ``r`` of a page stands for ``codes[..., r, :] * scales[..., r]``."""
-    _kv_fp8_dim(cache)
-    return reference.kv_cache_fp8_views(cache)
+    pages, heads, d = _kv_fp8_shape(cache)
+    return reference.kv_cache_fp8_views(cache, pages, heads, d)
 
 
-def _kv_fp8_dim(cache: torch.Tensor) -> int:
-    if cache.dtype is not torch.uint8 or cache.dim() != 4 or cache.shape[1] != 2 or cache.shape[3] % KV_FP8_PAGE or \
-            cache.shape[3] <= 4 * KV_FP8_PAGE or not cache.is_contiguous():
-        raise ValueError("an 8-bit KV cache is a contiguous uint8 tensor [pages, 2, kv_heads, 128 * (d + 4)] "
-                         f"(see kv_cache_fp8); got {cache.dtype} {list(cache.shape)}")
-    return cache.shape[3] // KV_FP8_PAGE - 4
+def _kv_fp8_shape(cache: torch.Tensor) -> tuple[int, int, int]:
+    """Pages, key heads and head width of an 8-bit cache."""
+    shape = cache.shape
+    if len(shape) == 4 and cache.dtype is torch.uint8 and cache.is_contiguous():
+        pages, two, heads, block = shape
+        if two == 2 and block % KV_FP8_PAGE == 0 and block > 4 * KV_FP8_PAGE:
+            return pages, heads, block // KV_FP8_PAGE - 4
+    raise ValueError("an 8-bit KV cache is a contiguous uint8 tensor [pages, 2, kv_heads, 128 * (d + 4)] "
+                     f"(see kv_cache_fp8); got {cache.dtype} {list(shape)}")
 
 
 # The checks below sit in front of kernels of a few microseconds: plain comparisons, messages made only when one fails.
@@ -502,7 +505,8 @@ def rope_kv_write_fp8_(qkv: torch.Tensor, Hq: int, Hkv: int, d: int, cs: torch.T
 
     A slot beyond the cache raises on the CPU; on a GPU its token is skipped and :func:`check_error` reports it."""
     T, dev = qkv.shape[0], qkv.device
-    if _kv_fp8_dim(cache) != d or cache.shape[2] != Hkv or cache.device != dev:
+    pages, heads, width = _kv_fp8_shape(cache)
+    if width != d or heads != Hkv or cache.device != dev:
         raise ValueError(f"cache {list(cache.shape)} on {cache.device} does not hold {Hkv} heads of width {d} on {dev}")
     if Hq <= 0 or qkv.dim() != 2 or qkv.shape[1] != (Hq + 2 * Hkv) * d:
         raise ValueError(f"qkv must be [T, ({Hq} + 2 * {Hkv}) * {d}], got {list(qkv.shape)}")
@@ -529,7 +533,7 @@ def rope_kv_write_fp8_(qkv: torch.Tensor, Hq: int, Hkv: int, d: int, cs: torch.T
         cs = cs.clone()
     lib = _lib.load()
     _chk(lib.cs_rope_kv_write_fp8(qkv.data_ptr(), qkv.stride(0), T, Hq, Hkv, d, cs.data_ptr(), _ptr(q_norm), _ptr(k_norm), eps,
-                                  slot.data_ptr(), q.data_ptr(), cache.data_ptr(), cache.shape[0], _stream()), "cs_rope_kv_write_fp8")
+                                  slot.data_ptr(), q.data_ptr(), cache.data_ptr(), pages, _stream()), "cs_rope_kv_write_fp8")
     _count()
     return q
 
@@ -549,11 +553,11 @@ def attention_paged_fp8(q: torch.Tensor, cache: torch.Tensor, block_table: torch
 
     Keys beyond the table or pages outside the cache raise on the CPU; on a GPU they are not read (the result of that
     sequence is then meaningless) and :func:`check_error` reports them."""
-    d, dev = _kv_fp8_dim(cache), q.device
+    (pages, Hkv, d), dev = _kv_fp8_shape(cache), q.device
     if q.dim() != 3 or q.shape[2] != d or cache.device != dev:
         raise ValueError(f"q must be [Tq, Hq, {d}] on {cache.device}, got {list(q.shape)} on {dev}")
     Tq, Hq, _ = q.shape
-    Hkv, B = cache.shape[2], kv_len.numel()
+    B = kv_len.numel()
     if Hq <= 0 or Hkv <= 0 or Hq % Hkv:
         raise ValueError(f"{Hq} query heads cannot share {Hkv} key heads")
     _check_i32("kv_len", kv_len, B, dev)
@@ -583,14 +587,14 @@ def attention_paged_fp8(q: torch.Tensor, cache: torch.Tensor, block_table: torch
     if max_q_len == 1 and Tq == B:
         nbytes = lib.cs_attention_decode_fp8_ws_bytes(Hq, Hkv, d)
         ws = cache.new_empty(nbytes)
-        _chk(lib.cs_attention_decode_fp8(q.data_ptr(), q.stride(0), cache.data_ptr(), cache.shape[0], out.data_ptr(), out.stride(0),
+        _chk(lib.cs_attention_decode_fp8(q.data_ptr(), q.stride(0), cache.data_ptr(), pages, out.data_ptr(), out.stride(0),
                                          out.stride(1), kv_len.data_ptr(), block_table.data_ptr(), block_table.stride(0), width, B, Hq,
                                          Hkv, d, scale, ws.data_ptr(), nbytes, _stream()), "cs_attention_decode_fp8")
         _count(2)
         return out
     nbytes = lib.cs_attention_prefill_fp8_ws_bytes(Tq, B, Hq, Hkv, d, width)
     ws = cache.new_empty(nbytes)
-    _chk(lib.cs_attention_prefill_fp8(q.data_ptr(), q.stride(0), cache.data_ptr(), cache.shape[0], out.data_ptr(), out.stride(0),
+    _chk(lib.cs_attention_prefill_fp8(q.data_ptr(), q.stride(0), cache.data_ptr(), pages, out.data_ptr(), out.stride(0),
                                       out.stride(1), cu_q.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(), block_table.stride(0),
                                       width, B, Tq, Hq, Hkv, d, scale, 1 if causal else 0, ws.data_ptr(), nbytes, _stream()),
          "cs_attention_prefill_fp8")

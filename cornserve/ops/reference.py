@@ -187,10 +187,8 @@ KV_FP8_MAX = 448.0
 KV_FP8_AMAX_FLOOR = 2.0 ** -40
 
 
-def kv_cache_fp8_views(cache):
-    pages, _, heads, block = cache.shape
-    d = block // KV_FP8_PAGE - 4
-    at = cache.storage_offset()
+def kv_cache_fp8_views(cache, pages, heads, d):
+    block, at = KV_FP8_PAGE * (d + 4), cache.storage_offset()
     codes = cache.view(torch.float8_e4m3fn).as_strided((pages, 2, heads, KV_FP8_PAGE, d), (2 * heads * block, heads * block, block, d, 1), at)
     b4 = block // 4
     scales = cache.view(torch.float32).as_strided((pages, 2, heads, KV_FP8_PAGE), (2 * heads * b4, heads * b4, b4, 1), at // 4 + KV_FP8_PAGE * d // 4)
@@ -216,7 +214,7 @@ def rope_kv_write_fp8(qkv, Hq, Hkv, d, cs, cache, slot, q_norm=None, k_norm=None
         w = torch.cat([q_norm.float().expand(Hq, d), k_norm.float().expand(Hkv, d)])
         qk = qk * torch.rsqrt(qk.pow(2).mean(-1, keepdim=True) + eps) * w
     qk = rope(qk, cs)
-    codes, scales = kv_cache_fp8_views(cache)
+    codes, scales = kv_cache_fp8_views(cache, cache.shape[0], Hkv, d)
     raw = codes.view(torch.uint8)      # indexed stores move bytes
     ok = slot >= 0
     at = slot[ok].long()
@@ -232,7 +230,7 @@ def rope_kv_write_fp8(qkv, Hq, Hkv, d, cs, cache, slot, q_norm=None, k_norm=None
 
 def gather_kv_fp8(cache, block_table, kv_len, seq):
     """Keys and values ``[kv_len, Hkv, d]`` (fp32) of sequence ``seq``."""
-    codes, scales = kv_cache_fp8_views(cache)
+    codes, scales = kv_cache_fp8_views(cache, cache.shape[0], cache.shape[2], cache.shape[3] // KV_FP8_PAGE - 4)
     n = int(kv_len[seq])
     ids = block_table[seq, : -(-n // KV_FP8_PAGE)].long()
     if n > block_table.shape[1] * KV_FP8_PAGE or bool(((ids < 0) | (ids >= cache.shape[0])).any()):

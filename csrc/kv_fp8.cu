@@ -13,7 +13,7 @@
 
 namespace {
 
-constexpr int APPEND_THREADS = 256;
+constexpr int APPEND_THREADS = 128;
 
 struct AppendParams {
   const __nv_bfloat16* qkv; long long ld;
@@ -22,7 +22,7 @@ struct AppendParams {
   const int* slot;                        // [T]
   __nv_bfloat16* q_out;                   // [T, Hq, d]
   uint8_t* cache;
-  long long rows;                         // T * (Hq + 2 Hkv)
+  unsigned rows;                          // T * (Hq + 2 Hkv)
   long long num_slots;                    // pages * 128
   int Hq, Hkv;
   float eps;
@@ -32,17 +32,17 @@ struct AppendParams {
 // A team of D/16 lanes owns one head row: lane c holds channels [8c, 8c+8) of the lower and of the upper half, so that
 // both members of every rotated pair are in one thread and all accesses are 8 or 16 bytes wide.
 template <int D>
-__global__ void __launch_bounds__(APPEND_THREADS) rope_kv_write_fp8_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(APPEND_THREADS, 12) rope_kv_write_fp8_kernel(const AppendParams p) {
   constexpr int LANES = D / 16, HALF = D / 2;
   pdl_wait();
   pdl_launch_dependents();
-  const long long row = (static_cast<long long>(blockIdx.x) * APPEND_THREADS + threadIdx.x) / LANES;
+  const unsigned row = blockIdx.x * (APPEND_THREADS / LANES) + threadIdx.x / LANES;
   const int c = threadIdx.x % LANES;
   const unsigned team = (LANES == 8 ? 0xffu : 0xfu) << ((threadIdx.x & 31) / LANES * LANES);
   if (row >= p.rows) return;
-  const int heads = p.Hq + 2 * p.Hkv;
-  const int h = static_cast<int>(row % heads);
-  const long long t = row / heads;
+  const unsigned heads = p.Hq + 2 * p.Hkv;
+  const long long t = row / heads;              // (32 bits: a 64-bit division is a third of this kernel's instructions)
+  const int h = static_cast<int>(row - static_cast<unsigned>(t) * heads);
   long long slot = 0;
   if (h >= p.Hq) {
     slot = p.slot[t];
@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) rope_kv_write_fp8_kernel(const
   }
   const int kv = h < p.Hq + p.Hkv ? 0 : 1;
   const int hh = kv == 0 ? h - p.Hq : h - p.Hq - p.Hkv;
-  uint8_t* block = p.cache + ((slot / KV8_PAGE * 2 + kv) * p.Hkv + hh) * kv8_block_bytes(D);
+  uint8_t* block = p.cache + (((slot / KV8_PAGE) * 2 + kv) * p.Hkv + hh) * kv8_block_bytes(D);
   const int r = static_cast<int>(slot % KV8_PAGE);
   uint8_t* dst = block + r * D + c * 8;
   *reinterpret_cast<uint2*>(dst) = make_uint2(code[0], code[1]);
@@ -142,13 +142,14 @@ CS_API int cs_rope_kv_write_fp8(const void* qkv, long long ld, int T, int Hq, in
   p.slot = (const int*)slot;
   p.q_out = (__nv_bfloat16*)q_out;
   p.cache = (uint8_t*)cache;
-  p.rows = static_cast<long long>(T) * (Hq + 2 * Hkv);
+  const long long rows = static_cast<long long>(T) * (Hq + 2 * Hkv);
+  if (rows > 0x7fffffffLL) return -1;
+  p.rows = static_cast<unsigned>(rows);
   p.num_slots = num_pages * KV8_PAGE;
   p.Hq = Hq; p.Hkv = Hkv; p.eps = eps;
   p.err = cs_error_word();
   const int rows_per_block = APPEND_THREADS / (d / 16);
-  const long long blocks = (p.rows + rows_per_block - 1) / rows_per_block;
-  if (blocks > 0x7fffffffLL) return -1;
+  const long long blocks = (rows + rows_per_block - 1) / rows_per_block;
   cudaError_t e;
   if (d == 128) e = cs_launch_pdl(rope_kv_write_fp8_kernel<128>, dim3((unsigned)blocks), dim3(APPEND_THREADS), 0, (cudaStream_t)stream, p);
   else e = cs_launch_pdl(rope_kv_write_fp8_kernel<64>, dim3((unsigned)blocks), dim3(APPEND_THREADS), 0, (cudaStream_t)stream, p);
