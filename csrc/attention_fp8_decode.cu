@@ -10,9 +10,9 @@
 // The kernel is bound by the cache's bytes, and everything is arranged around reading them once, without a pause:
 //
 //   * Work is counted in units of 64 keys (128 for the narrow heads) of one (sequence, key head); the list of all units
-//     of the batch is cut into equal runs, one per CTA, on the device from kv_len.  So any mix of lengths loads every SM
-//     alike (a captured graph adapts to the lengths of each replay), and a single long sequence is spread over the whole
-//     GPU.  A CTA has at most two items that it does not own alone, the first and the last of its run: these leave partial
+//     of the batch is cut into runs of equal cost, one per CTA, on the device from kv_len.  So any mix of lengths loads
+//     every SM alike (a captured graph adapts to the lengths of each replay), and a single long sequence is spread over the
+//     whole GPU.  A CTA has at most two items that it does not own alone, the first and the last of its run: these leave partial
 //     sums in a workspace and a second small kernel joins them in the order of the CTAs (no atomics, the result does not
 //     depend on timing).
 //   * A CTA is three (or two) teams of four consumer warps and one producer warp.  A team has its own ring of stages, kept
@@ -34,6 +34,7 @@ int cs_encode_tmap_nd(CUtensorMap* out, int elem_bytes, int rank, const void* ba
 namespace {
 
 constexpr int MAX_CTAS = 512;
+constexpr int ITEM_COST = 3;                 // what an item costs beside its units, in units
 constexpr int SHARED_VISIT = 3;              // visits of at least this many units are shared by the teams of a CTA
 constexpr float M_NONE = -3.0e38f;           // running maximum before the first key (finite: differences stay defined)
 
@@ -147,33 +148,50 @@ __device__ __forceinline__ void store_head(const DecParams& p, int seq, int head
   }
 }
 
-// One visit of a CTA to an item: units [u, u + n) of `units` of sequence `seq`, head block `head` (of Hkv * head_blocks).
-// Every role of the CTA walks the same list of visits.
+// A place in the list of units: unit u of head block `head` (of Hkv * head_blocks) of a sequence.
+struct Place { int seq, head, u; };
+
+// The place at distance r (cost) into the items of a sequence.  Cuts that would leave less than two units of an item on one
+// side move to its edge.
+__device__ __forceinline__ Place place_at(int seq, int units, int heads, int r) {
+  Place at{seq, r / (units + ITEM_COST), 0};
+  const int u = r - at.head * (units + ITEM_COST) - ITEM_COST;
+  if (u < 2) return at;
+  if (units - u >= 2) { at.u = u; return at; }
+  if (++at.head == heads) { at.head = 0; ++at.seq; }
+  return at;
+}
+
+// One visit of a CTA to an item: units [u, u + n) of `units` of sequence `seq`, head block `head`.  Every role of the CTA
+// walks the same list of visits.
 template <int UNIT>
 struct Walk {
-  int seq, head, units, len, u, n;
-  int left;         // units of the CTA's run not yet handed out, this visit included
+  int seq, head, u;
+  Place end;
+  int len, units, n;
   uint32_t dealt;   // short visits and units of shared visits so far: deals the next ones to the teams in turn
-  __device__ __forceinline__ bool settle(const DecParams& p) {   // on to a sequence with keys
-    for (; seq < p.B; ++seq) {
+  __device__ __forceinline__ bool settle(const DecParams& p) {   // on to an item with units for this CTA
+    const int heads = p.Hkv * p.head_blocks;
+    while (seq < p.B) {
       len = dec_len(p, seq);
       units = (len + UNIT - 1) / UNIT;
-      if (u < units) {
-        n = min(units - u, left);
-        return true;
-      }
+      const bool last = seq == end.seq && head == end.head;
+      if (seq > end.seq || (last && u >= end.u)) return false;
+      n = (last ? min(end.u, units) : units) - u;
+      if (n > 0) return true;
+      u = 0;
+      if (units == 0 || ++head == heads) { head = 0; ++seq; }
     }
     return false;
   }
   __device__ __forceinline__ bool shared() const { return n >= SHARED_VISIT; }
   __device__ __forceinline__ bool next(const DecParams& p) {
     dealt += shared() ? n : 1;
-    left -= n;
-    if (left <= 0) return false;
+    if (seq == end.seq && head == end.head) return false;
     u = 0;
     if (++head == p.Hkv * p.head_blocks) { head = 0; ++seq; return settle(p); }
-    n = min(units, left);
-    return true;
+    n = (seq == end.seq && head == end.head) ? min(end.u, units) : units;
+    return n > 0;
   }
   // the units of this visit that belong to `team`: first, first + step, ... below u + n
   template <int TEAMS>
@@ -202,12 +220,13 @@ attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_codes, const 
   float* s_join = reinterpret_cast<float*>(s_q + TEAMS * QSLOTS * Shape::Q); // [warp][head][JOIN_LD]
   __shared__ uint64_t full[TEAMS][RING], empty[TEAMS][RING], q_full[TEAMS][QSLOTS], q_empty[TEAMS][QSLOTS];
   __shared__ float s_m[WARPS][HEADS], s_l[WARPS][HEADS];
-  __shared__ int abort_flag, s_warp_sum[ALL_WARPS], s_start[2];   // s_start: sequence and unit (of all its heads) the run begins with
+  __shared__ int abort_flag, s_warp_sum[ALL_WARPS];
+  __shared__ Place s_cut[2];       // where the run begins and ends
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     abort_flag = 0;
-    s_start[0] = s_start[1] = 0;
+    s_cut[0] = s_cut[1] = Place{p.B, 0, 0};
     for (int w = 0; w < TEAMS; ++w) {
       for (int s = 0; s < RING; ++s) { mbar_init(&full[w][s], 1); mbar_init(&empty[w][s], 4); }
       for (int s = 0; s < QSLOTS; ++s) { mbar_init(&q_full[w][s], 1); mbar_init(&q_empty[w][s], 4); }
@@ -222,12 +241,14 @@ attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_codes, const 
   if (threadIdx.x == 0) p.ws_item[blockIdx.x * 2] = p.ws_item[blockIdx.x * 2 + 1] = -1;
 
   // ------------------------------- this CTA's run of units -------------------------------
-  // Thread i counts the units of `per` consecutive sequences (one, unless the batch is huge); a scan over the threads
-  // gives the total and who owns the first unit of the run.  The host has checked that 32 bits hold every count.
+  // Thread i adds up the cost of `per` consecutive sequences (one, unless the batch is huge); a scan over the threads gives
+  // the total and who owns the two cuts.  The host has checked that 32 bits hold every sum.
   const int heads = p.Hkv * p.head_blocks, per = (p.B + THREADS - 1) / THREADS;
   auto units_of = [&](int b) { return b < p.B ? (dec_len(p, b) + UNIT - 1) / UNIT : 0; };
+  auto cost = [&](int units) { return units > 0 ? (units + ITEM_COST) * heads : 0; };
+  const int first = static_cast<int>(threadIdx.x) * per;
   int mine = 0;
-  for (int i = 0; i < per; ++i) mine += units_of(threadIdx.x * per + i);
+  for (int i = 0; i < per; ++i) mine += cost(units_of(first + i));
   int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -242,27 +263,30 @@ attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_codes, const 
     if (w == warp) incl += total;
     total += s_warp_sum[w];
   }
-  total *= heads;
-  // no CTA of the first `active` is without a unit, so the CTAs that share an item are consecutive
-  const int active = max(1, min(total, static_cast<int>(gridDim.x))), c = blockIdx.x;
+  // (runs of at least a unit per team: the CTAs that share an item are consecutive)
+  const int active = max(1, min(total / (ITEM_COST + TEAMS), static_cast<int>(gridDim.x))), c = blockIdx.x;
   const int quota = total / active, extra = total - quota * active;
-  const int r0 = quota * c + min(c, extra), run = c < active ? quota + (c < extra ? 1 : 0) : 0;
-  int at0 = (incl - mine) * heads;
-  if (run > 0 && r0 >= at0 && r0 < incl * heads) {
-    int b = static_cast<int>(threadIdx.x) * per;
-    for (int u; b < (static_cast<int>(threadIdx.x) + 1) * per - 1 && r0 >= at0 + (u = units_of(b) * heads); ++b) at0 += u;
-    s_start[0] = b;
-    s_start[1] = r0 - at0;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int r = c + e >= active ? total : quota * (c + e) + min(c + e, extra);
+    int at0 = incl - mine;
+    if (r >= at0 && r < incl) {
+      int i = 0, units = units_of(first);
+      while (i + 1 < per && r >= at0 + cost(units)) {
+        at0 += cost(units);
+        units = units_of(first + ++i);
+      }
+      s_cut[e] = place_at(first + i, units, heads, r - at0);
+    }
   }
   __syncthreads();
   volatile int* abortp = &abort_flag;
   Walk<UNIT> wk{};
-  wk.seq = s_start[0];
-  wk.left = run;
-  const int start_units = max(1, units_of(wk.seq));
-  wk.head = s_start[1] / start_units;
-  wk.u = s_start[1] - wk.head * start_units;
-  const bool any = run > 0 && wk.settle(p);
+  wk.seq = s_cut[0].seq;
+  wk.head = s_cut[0].head;
+  wk.u = s_cut[0].u;
+  wk.end = s_cut[1];
+  const bool any = wk.settle(p);
 
   if (warp >= WARPS) {
     // ------------------------------- producer of one team -------------------------------
@@ -638,8 +662,8 @@ int launch_decode(const void* cache, DecParams& p, int ctas, cudaStream_t stream
       return -10;
     attr_done[dev] = true;
   }
-  // no more CTAs than units that the tables could hold
-  const long long most = static_cast<long long>(p.B) * p.Hkv * p.head_blocks * p.bt_width * (KV8_PAGE / Shape::UNIT);
+  // no more CTAs than runs that full tables would make
+  const long long most = static_cast<long long>(p.B) * p.Hkv * p.head_blocks * (p.bt_width * (KV8_PAGE / Shape::UNIT) + ITEM_COST) / (ITEM_COST + Shape::TEAMS);
   if (most < ctas) ctas = most > 0 ? static_cast<int>(most) : 1;
   // one box = the K and V codes (or scales) of one unit of one head and page
   CUtensorMap tm_codes, tm_scales;
@@ -686,8 +710,8 @@ CS_API int cs_attention_decode_fp8(const void* q, long long q_tok, const void* c
   p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv;
   const int heads = p.G <= 8 ? 8 : 16;
   p.head_blocks = (p.G + heads - 1) / heads;
-  // units of the whole batch, were every table full: counted in 32 bits on the device
-  if (bt_width > 0 && static_cast<long long>(B) * Hkv * p.head_blocks > 0x7fffffffLL / (2LL * bt_width)) return -1;
+  // cost of the whole batch, were every table full: added up in 32 bits on the device
+  if (static_cast<long long>(B) * Hkv * p.head_blocks > 0x7fffffffLL / (2LL * bt_width + ITEM_COST)) return -1;
   if (static_cast<long long>(B) * Hkv * p.head_blocks > 0x7fffffffLL) return -1;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.err = cs_error_word();
