@@ -35,6 +35,7 @@ namespace {
 
 constexpr int MAX_CTAS = 512;
 constexpr int ITEM_COST = 3;                 // what an item costs beside its units, in units
+constexpr int MIN_RUN = 2;                   // no CTA for less
 constexpr int SHARED_VISIT = 3;              // visits of at least this many units are shared by the teams of a CTA
 constexpr float M_NONE = -3.0e38f;           // running maximum before the first key (finite: differences stay defined)
 
@@ -263,8 +264,8 @@ attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_codes, const 
     if (w == warp) incl += total;
     total += s_warp_sum[w];
   }
-  // (runs of at least a unit per team: the CTAs that share an item are consecutive)
-  const int active = max(1, min(total / (ITEM_COST + TEAMS), static_cast<int>(gridDim.x))), c = blockIdx.x;
+  // (at least MIN_RUN each: then the CTAs that share an item are consecutive)
+  const int active = max(1, min(total / MIN_RUN, static_cast<int>(gridDim.x))), c = blockIdx.x;
   const int quota = total / active, extra = total - quota * active;
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
@@ -663,7 +664,7 @@ int launch_decode(const void* cache, DecParams& p, int ctas, cudaStream_t stream
     attr_done[dev] = true;
   }
   // no more CTAs than runs that full tables would make
-  const long long most = static_cast<long long>(p.B) * p.Hkv * p.head_blocks * (p.bt_width * (KV8_PAGE / Shape::UNIT) + ITEM_COST) / (ITEM_COST + Shape::TEAMS);
+  const long long most = static_cast<long long>(p.B) * p.Hkv * p.head_blocks * (p.bt_width * (KV8_PAGE / Shape::UNIT) + ITEM_COST) / MIN_RUN;
   if (most < ctas) ctas = most > 0 ? static_cast<int>(most) : 1;
   // one box = the K and V codes (or scales) of one unit of one head and page
   CUtensorMap tm_codes, tm_scales;
