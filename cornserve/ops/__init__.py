@@ -547,9 +547,10 @@ def attention_paged_fp8(q: torch.Tensor, cache: torch.Tensor, block_table: torch
     ``[cu_q[s], cu_q[s + 1])`` of ``q``, at most ``max_q_len`` of them.  A causal query sees the keys up to its own
     position; one that sees none gives zeros.  Rows of ``out`` behind the last sequence are not written.
 
-    With one query per sequence (``max_q_len`` 1 and as many rows as sequences) keys and values take part exactly as they
-    are cached; with more they are rounded to fp16 once (code times scale, 11 bits).  The lengths are read on the device:
-    a captured call follows them from replay to replay, within the table's width and the number of queries.
+    With single tokens (``max_q_len`` 1 and as many rows as sequences) keys and values take part exactly as they are
+    cached; otherwise they are rounded to fp16 once: code times scale to 11 bits, or to within 2^-30 of the largest scale
+    of their page, and the value scales of a sequence have to lie within 2^100 of each other.  The lengths are read on the
+    device: a captured call follows them from replay to replay, within the table's width and the number of queries.
 
     Keys beyond the table or pages outside the cache raise on the CPU; on a GPU they are not read (the result of that
     sequence is then meaningless) and :func:`check_error` reports them."""
@@ -588,7 +589,7 @@ def attention_paged_fp8(q: torch.Tensor, cache: torch.Tensor, block_table: torch
         nbytes = lib.cs_attention_decode_fp8_ws_bytes(Hq, Hkv, d)
         ws = cache.new_empty(nbytes)
         _chk(lib.cs_attention_decode_fp8(q.data_ptr(), q.stride(0), cache.data_ptr(), pages, out.data_ptr(), out.stride(0),
-                                         out.stride(1), kv_len.data_ptr(), block_table.data_ptr(), block_table.stride(0), width, B, Hq,
+                                         out.stride(1), cu_q.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(), block_table.stride(0), width, B, Hq,
                                          Hkv, d, scale, ws.data_ptr(), nbytes, _stream()), "cs_attention_decode_fp8")
         _count(2)
         return out

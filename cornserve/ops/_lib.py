@@ -65,7 +65,7 @@ _SIGNATURES = {
     "cs_rope_kv_write_fp8": ([P, L, I, I, I, I, P, P, P, F, P, P, P, L, P], I),
     "cs_attention_prefill_fp8": ([P, L, P, L, P, L, L, P, P, P, L, I, I, I, I, I, I, F, I, P, L, P], I),
     "cs_attention_prefill_fp8_ws_bytes": ([L, L, I, I, I, L], L),
-    "cs_attention_decode_fp8": ([P, L, P, L, P, L, L, P, P, L, I, I, I, I, I, F, P, L, P], I),
+    "cs_attention_decode_fp8": ([P, L, P, L, P, L, L, P, P, P, L, I, I, I, I, I, F, P, L, P], I),
     "cs_attention_decode_fp8_ws_bytes": ([I, I, I], L),
     "cs_enable_peer_access": ([I], I),
     "cs_to_rgb8": ([P, L, P, L, P], I),

@@ -66,12 +66,11 @@ struct Seq {
   int q_beg, q_len, k_len, shift;           // causal: query i sees keys j <= i + shift
 };
 __device__ __forceinline__ Seq get_seq(const PrefillParams& p, int s) {
-  const int a = min(max(p.cu_q[s], 0), p.Tq), b = min(p.cu_q[s + 1], p.Tq), len = p.kv_len[s];
-  const long long cap = static_cast<long long>(p.bt_width) * KV8_PAGE;
+  const int a = min(max(p.cu_q[s], 0), p.Tq), b = min(p.cu_q[s + 1], p.Tq), len = max(p.kv_len[s], 0);
   Seq q;
   q.q_beg = a;
   q.q_len = max(b - a, 0);
-  q.k_len = len < 0 ? 0 : (len > cap ? static_cast<int>(cap) : len);
+  q.k_len = min(len, p.bt_width * KV8_PAGE);
   q.shift = len - q.q_len;
   return q;
 }
@@ -707,7 +706,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
     }
     // lengths that do not fit the table or the queries are reported
     for (int b = blockIdx.x * 256 + threadIdx.x; b < p.B; b += gridDim.x * 256)
-      if (p.kv_len[b] > static_cast<long long>(p.bt_width) * KV8_PAGE || p.cu_q[b] < 0 || p.cu_q[b + 1] < p.cu_q[b] || p.cu_q[b + 1] > p.Tq)
+      if (p.kv_len[b] < 0 || p.kv_len[b] > p.bt_width * KV8_PAGE || p.cu_q[b] < 0 || p.cu_q[b + 1] < p.cu_q[b] || p.cu_q[b + 1] > p.Tq)
         cs_set_error(p.err, CS_ERR_BAD_ARG);
   }
   tc_fence_before();
@@ -795,7 +794,9 @@ CS_API int cs_attention_prefill_fp8(const void* q, long long q_tok, const void* 
                                     int bt_width, int B, int Tq, int Hq, int Hkv, int d, float scale, int causal, void* ws,
                                     long long ws_bytes, void* stream) {
   if (B <= 0 || Tq <= 0) return 0;
-  if ((d != 64 && d != 128) || Hkv <= 0 || Hq <= 0 || Hq % Hkv != 0 || num_pages <= 0 || num_pages > 0x7fffffffLL) return -1;
+  if ((d != 64 && d != 128) || Hkv <= 0 || Hq <= 0 || Hq % Hkv != 0 || num_pages <= 0 || num_pages > 0x7fffffffLL || bt_width < 0 ||
+      bt_width > KV8_MAX_PAGES)
+    return -1;
   if ((reinterpret_cast<uintptr_t>(q) & 15) || (q_tok & 7)) return -1;
   if (ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 15) || ws_bytes < cs_attention_prefill_fp8_ws_bytes(Tq, B, Hq, Hkv, d, bt_width))
     return -5;

@@ -65,7 +65,7 @@ struct DecParams {
   __nv_bfloat16* o; long long o_tok, o_head; int o_vec; // o_vec: 8-byte stores are aligned
   int num_pages;
   const int* block_table; long long bt_stride; int bt_width;
-  const int* kv_len;
+  const int* kv_len; const int* cu_q;
   int B, Hq, Hkv, G, head_blocks;                      // G query heads per key head, in blocks of 8 NT
   float scale_log2;
   float* ws_o;        // [ctas, 2, HEADS, D] partial sums: slot 0 = the CTA's first item, slot 1 = its last
@@ -127,19 +127,27 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Keys of sequence b that can be read (a length beyond the table is cut and reported), and its units.
-__device__ __forceinline__ int dec_len(const DecParams& p, int b) {
-  const int n = p.kv_len[b];
-  const long long cap = static_cast<long long>(p.bt_width) * KV8_PAGE;
-  return n < 0 ? 0 : (n > cap ? static_cast<int>(cap) : n);
+// A sequence: the row of its query (-1: it has none) and the keys of it that can be read (none without a query; a length
+// beyond the table is cut).  What does not fit is reported.
+struct Seq { int row, len; };
+__device__ __forceinline__ Seq get_seq(const DecParams& p, int b) {
+  const int n = p.kv_len[b], beg = p.cu_q[b], end = p.cu_q[b + 1], cap = p.bt_width * KV8_PAGE;
+  Seq s;
+  s.row = end > beg && beg >= 0 && beg < p.B ? beg : -1;
+  s.len = s.row < 0 || n < 0 ? 0 : min(n, cap);
+  return s;
+}
+__device__ __forceinline__ bool fits(const DecParams& p, int b) {
+  const int n = p.kv_len[b], beg = p.cu_q[b], end = p.cu_q[b + 1];
+  return n >= 0 && n <= p.bt_width * KV8_PAGE && beg >= 0 && end <= p.B && (end == beg || end == beg + 1);
 }
 
 template <int N> struct Count { static constexpr int value = N; };
 
 // Four channels of one head: sums divided by the normaliser (0 when no key took part).
-__device__ __forceinline__ void store_head(const DecParams& p, int seq, int head, int ch4, const float4& acc, float sum) {
+__device__ __forceinline__ void store_head(const DecParams& p, int row, int head, int ch4, const float4& acc, float sum) {
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-  __nv_bfloat16* dst = p.o + seq * p.o_tok + head * p.o_head + ch4 * 4;
+  __nv_bfloat16* dst = p.o + row * p.o_tok + head * p.o_head + ch4 * 4;
   const uint2 v = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
   if (p.o_vec) {
     *reinterpret_cast<uint2*>(dst) = v;
@@ -169,12 +177,14 @@ template <int UNIT>
 struct Walk {
   int seq, head, u;
   Place end;
-  int len, units, n;
+  int row, len, units, n;
   uint32_t dealt;   // short visits and units of shared visits so far: deals the next ones to the teams in turn
   __device__ __forceinline__ bool settle(const DecParams& p) {   // on to an item with units for this CTA
     const int heads = p.Hkv * p.head_blocks;
     while (seq < p.B) {
-      len = dec_len(p, seq);
+      const Seq s = get_seq(p, seq);
+      row = s.row;
+      len = s.len;
       units = (len + UNIT - 1) / UNIT;
       const bool last = seq == end.seq && head == end.head;
       if (seq > end.seq || (last && u >= end.u)) return false;
@@ -245,7 +255,7 @@ attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_codes, const 
   // Thread i adds up the cost of `per` consecutive sequences (one, unless the batch is huge); a scan over the threads gives
   // the total and who owns the two cuts.  The host has checked that 32 bits hold every sum.
   const int heads = p.Hkv * p.head_blocks, per = (p.B + THREADS - 1) / THREADS;
-  auto units_of = [&](int b) { return b < p.B ? (dec_len(p, b) + UNIT - 1) / UNIT : 0; };
+  auto units_of = [&](int b) { return b < p.B ? (get_seq(p, b).len + UNIT - 1) / UNIT : 0; };
   auto cost = [&](int units) { return units > 0 ? (units + ITEM_COST) * heads : 0; };
   const int first = static_cast<int>(threadIdx.x) * per;
   int mine = 0;
@@ -308,7 +318,7 @@ attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_codes, const 
         if (ok) {
           const uint32_t bytes = min(HEADS, p.G - hb * HEADS) * D * 2;
           mbar_arrive_expect_tx(&q_full[team][slot], bytes);
-          bulk_load(smem_u32(s_q + (team * QSLOTS + slot) * Shape::Q), p.q + wk.seq * p.q_tok + (hk * p.G + hb * HEADS) * D, bytes,
+          bulk_load(smem_u32(s_q + (team * QSLOTS + slot) * Shape::Q), p.q + wk.row * p.q_tok + (hk * p.G + hb * HEADS) * D, bytes,
                     &q_full[team][slot]);
         }
       }
@@ -580,7 +590,7 @@ attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_codes, const 
             acc.x += v.x * e; acc.y += v.y * e; acc.z += v.z * e; acc.w += v.w * e;
           }
           if (whole) {
-            store_head(p, wk.seq, h0 + h, ch, acc, sum);
+            store_head(p, wk.row, h0 + h, ch, acc, sum);
           } else {
             *reinterpret_cast<float4*>(p.ws_o + (part + h) * D + ch * 4) = acc;
             if (ch == 0) { p.ws_ml[(part + h) * 2] = mx; p.ws_ml[(part + h) * 2 + 1] = sum; }
@@ -591,12 +601,12 @@ attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_codes, const 
       meet();   // the join area is written again at the end of the next visit
     } while (wk.next(p));
 
-    // sequences without keys give zeros; lengths that do not fit the table are reported
+    // queries without keys give zeros
     for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
-      const int len = p.kv_len[b];
-      if (len > static_cast<long long>(p.bt_width) * KV8_PAGE && threadIdx.x == 0) cs_set_error(p.err, CS_ERR_BAD_ARG);
-      if (dec_len(p, b) == 0)
-        for (int i = threadIdx.x; i < p.Hq * D; i += WARPS * 32) p.o[b * p.o_tok + (i / D) * p.o_head + i % D] = __float2bfloat16(0.f);
+      if (threadIdx.x == 0 && !fits(p, b)) cs_set_error(p.err, CS_ERR_BAD_ARG);
+      const Seq s = get_seq(p, b);
+      if (s.row >= 0 && s.len == 0)
+        for (int i = threadIdx.x; i < p.Hq * D; i += WARPS * 32) p.o[s.row * p.o_tok + (i / D) * p.o_head + i % D] = __float2bfloat16(0.f);
     }
   }
 }
@@ -649,7 +659,7 @@ __global__ void __launch_bounds__(128) attention_decode_fp8_join_kernel(const De
     l += s_ml[w][1] * e;
     acc.x += v.x * e; acc.y += v.y * e; acc.z += v.z * e; acc.w += v.w * e;
   }
-  store_head(p, seq, hk * p.G + hb * HEADS + h, lane, acc, l);
+  store_head(p, get_seq(p, seq).row, hk * p.G + hb * HEADS + h, lane, acc, l);
 }
 
 template <int D, int NT>
@@ -693,10 +703,11 @@ CS_API long long cs_attention_decode_fp8_ws_bytes(int Hq, int Hkv, int d) {
 }
 
 // q: [B, Hq, d] with contiguous heads, tokens q_tok elements apart and on 16-byte boundaries; o: [B, Hq, d] with token and
-// head strides in elements.  One query per sequence, which sees all kv_len[b] keys.  ws: cs_attention_decode_fp8_ws_bytes
+// head strides in elements.  Sequence b has the query of row cu_q[b], which sees all kv_len[b] keys, or none if cu_q[b + 1] is
+// the same; rows of no sequence are left as they are.  ws: cs_attention_decode_fp8_ws_bytes
 // of scratch that no call on another stream uses.
 CS_API int cs_attention_decode_fp8(const void* q, long long q_tok, const void* cache, long long num_pages, void* o, long long o_tok,
-                                   long long o_head, const void* kv_len, const void* block_table, long long bt_stride, int bt_width, int B,
+                                   long long o_head, const void* cu_q, const void* kv_len, const void* block_table, long long bt_stride, int bt_width, int B,
                                    int Hq, int Hkv, int d, float scale, void* ws, long long ws_bytes, void* stream) {
   if (B <= 0) return 0;
   if ((d != 64 && d != 128) || Hkv <= 0 || Hq <= 0 || Hq % Hkv != 0 || num_pages <= 0 || num_pages > 0x7fffffffLL) return -1;
@@ -707,13 +718,13 @@ CS_API int cs_attention_decode_fp8(const void* q, long long q_tok, const void* c
   p.o_vec = (reinterpret_cast<uintptr_t>(o) & 7) == 0 && (o_tok & 3) == 0 && (o_head & 3) == 0;
   p.num_pages = static_cast<int>(num_pages);
   p.block_table = (const int*)block_table; p.bt_stride = bt_stride; p.bt_width = bt_width;
-  p.kv_len = (const int*)kv_len;
+  p.kv_len = (const int*)kv_len; p.cu_q = (const int*)cu_q;
   p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv;
   const int heads = p.G <= 8 ? 8 : 16;
   p.head_blocks = (p.G + heads - 1) / heads;
-  // cost of the whole batch, were every table full: added up in 32 bits on the device
+  // lengths, and the cost of the whole batch were every table full, are added up in 32 bits on the device
+  if (bt_width < 0 || bt_width > KV8_MAX_PAGES) return -1;
   if (static_cast<long long>(B) * Hkv * p.head_blocks > 0x7fffffffLL / (2LL * bt_width + ITEM_COST)) return -1;
-  if (static_cast<long long>(B) * Hkv * p.head_blocks > 0x7fffffffLL) return -1;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.err = cs_error_word();
   if (ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 15) || ws_bytes < cs_attention_decode_fp8_ws_bytes(Hq, Hkv, d)) return -5;

@@ -16,16 +16,11 @@
 #include "common.cuh"
 
 constexpr int KV8_PAGE = 128;
+constexpr int KV8_MAX_PAGES = (1 << 24) - 16;   // of a sequence: positions, and a little more, fit 31 bits
 
 __host__ __device__ __forceinline__ constexpr long long kv8_block_bytes(int d) { return static_cast<long long>(KV8_PAGE) * (d + 4); }
 
-// Two e4m3 codes (low byte first) as two fp16 numbers: every finite code is exact in fp16.
-__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t two_codes) {
-  uint32_t r;
-  asm("{\n\t.reg .b16 lo;\n\tcvt.u16.u32 lo, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(two_codes));
-  return r;
-}
-// Four codes: the lower two and the upper two.
+// Four e4m3 codes as fp16 numbers (every finite code is exact in fp16): the lower two and the upper two.
 __device__ __forceinline__ void e4m3x4_to_half2x2(uint32_t codes, uint32_t& lo, uint32_t& hi) {
   asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
       : "=r"(lo), "=r"(hi)

@@ -340,6 +340,72 @@ def test_tables_and_lengths_that_do_not_fit_are_reported(new):
     _check(out[b:], q[b:], cache, table[2:], lens[2:], new[2:])
 
 
+def test_rows_of_no_sequence_are_left_as_they_were():
+    """A padded batch of single tokens: as many rows as sequences, but some sequences have no query."""
+    lens = [200, 50, 70, 0, 129]
+    q, cache, table, kv_len, _ = _setup(lens, [1] * 5, 8, 2, 64, seed=17)
+    for cu, rows in (([0, 1, 2, 2, 2, 2], {0: 0, 1: 1}), ([1, 2, 2, 3, 4, 5], {1: 0, 2: 2, 3: 3, 4: 4}), ([0] * 6, {})):
+        out = torch.full_like(q, 5.0)
+        ops.attention_paged_fp8(q, cache, table, kv_len, _i32(cu), 1, out=out)
+        for r in range(5):
+            if r in rows:
+                i = rows[r]
+                _check(out[r: r + 1], q[r: r + 1], cache, table[i: i + 1], lens[i: i + 1], [1])
+            else:
+                assert (out[r] == 5.0).all()
+    out = torch.full_like(q, 5.0)        # the same rows, for sequences of many queries: rows 0 and 4 are nobody's
+    ops.attention_paged_fp8(q, cache, table[1:3], _i32([50, 70]), _i32([1, 3, 4]), 2, out=out)
+    assert (out[0] == 5.0).all() and (out[4] == 5.0).all()
+    _check(out[1:4], q[1:4], cache, table[1:3], [50, 70], [2, 1])
+    for cu in ([0, 1, 2, 3, 4, 6], [0, 2, 2, 3, 4, 5], [-1, 0, 1, 2, 3, 4]):      # not one row each, or not in q
+        ops.attention_paged_fp8(q, cache, table, kv_len, _i32(cu), 1)
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="bad argument"):
+            ops.check_error("rows")
+    for n in (1, 2):
+        ops.attention_paged_fp8(q[:n], cache, table[:1], _i32([-3]), _i32([0, n]), n, out=out[:n])
+        assert not out[:n].any()
+        with pytest.raises(RuntimeError, match="bad argument"):
+            ops.check_error("length")
+
+
+@pytest.mark.parametrize("B", [479, 481, 1201])
+@pytest.mark.parametrize("new", [[1], [3, 0, 1, 2]])
+def test_more_sequences_than_threads(B, new):
+    """The lengths are added up by the threads of a block, several sequences each in a large batch."""
+    lens = [(7 * i * i + 3 * i) % 141 if i % 19 else 0 for i in range(B)]
+    new = [min(new[i % len(new)], lens[i]) if len(new) > 1 else 1 for i in range(B)]
+    q, cache, table, kv_len, cu = _setup(lens, new, 4, 2, 64, seed=B)
+    _check(ops.attention_paged_fp8(q, cache, table, kv_len, cu, max(new)), q, cache, table, lens, new)
+
+
+@pytest.mark.parametrize("Hq,Hkv,d", [(131, 1, 64), (256, 2, 128), (48, 2, 128)])
+@pytest.mark.parametrize("new", [[1, 1, 1], [5, 70, 1]])
+def test_very_many_heads_to_a_key_head(Hq, Hkv, d, new):
+    lens = [260, 70, 1]
+    q, cache, table, kv_len, cu = _setup(lens, new, Hq, Hkv, d, seed=Hq)
+    _check(ops.attention_paged_fp8(q, cache, table, kv_len, cu, max(new)), q, cache, table, lens, new)
+
+
+def test_pages_behind_4_gib_of_cache():
+    """Offsets of the cache that pass 32 bits: pages at the end of 4.5 GB (zeroed, so nothing but these pages holds a row)."""
+    Hkv, d, lens = 8, 128, [300, 129]
+    pages = (4608 << 20) // (2 * Hkv * 128 * (d + 4))
+    table = torch.arange(pages - 6, pages, device=DEV, dtype=torch.int32).view(2, 3)
+    cache = ops.kv_cache_fp8(pages, Hkv, d, DEV)
+    cs = _cs(429, d)
+    pos = torch.cat([torch.arange(n, device=DEV) for n in lens])
+    seq = torch.repeat_interleave(torch.arange(2, device=DEV), torch.tensor(lens, device=DEV))
+    slot = (table[seq, pos // 128].long() * 128 + pos % 128).int()
+    torch.manual_seed(3)
+    qkv = torch.randn(429, 32 * d, device=DEV).bfloat16()
+    q = ops.rope_kv_write_fp8_(qkv, 16, Hkv, d, cs, cache, slot)
+    assert not cache[: pages - 6].view(torch.int64).any()
+    _check(ops.attention_paged_fp8(q, cache, table, _i32(lens), _i32([0, 300, 429]), 300), q, cache, table, lens, lens)
+    last = q[[299, 428]]
+    _check(ops.attention_paged_fp8(last, cache, table, _i32(lens), _i32([0, 1, 2]), 1), last, cache, table, lens, [1, 1])
+
+
 def test_results_do_not_depend_on_the_run_or_the_batch_order():
     lens = [5, 2000, 700, 333, 128]
     q, cache, table, kv_len, cu = _setup(lens, [1] * 5, 28, 4, 128, seed=21)
