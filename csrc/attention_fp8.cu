@@ -675,6 +675,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
       const float inv = !it.whole ? 1.f : (l == 0.f ? 0.f : 1.f / l);
       __nv_bfloat16* dst = p.o + static_cast<long long>(it.q_beg + tok) * p.o_tok + (it.h0 + g) * p.o_head;
       float* part = p.ws_o + row * D;
+      const bool mate_ok = __shfl_xor_sync(0xffffffffu, row_ok, 1);
+      __nv_bfloat16* mate = reinterpret_cast<__nv_bfloat16*>(__shfl_xor_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), 1));
+      const bool even_ok = (lane & 1) ? mate_ok : row_ok, odd_ok = (lane & 1) ? row_ok : mate_ok;
+      __nv_bfloat16 *dst_even = ((lane & 1) ? mate + 8 : dst), *dst_odd = ((lane & 1) ? dst + 8 : mate);
 #pragma unroll 1
       for (int c = 0; c < D / 16; ++c) {
         uint32_t o[16];
@@ -685,7 +689,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[i] = 0u;
         }
-        if (!row_ok) continue;
+        if (!row_ok && !(it.whole && p.o_vec)) continue;
         float f[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(o[i]) * inv;
@@ -693,10 +697,19 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
 #pragma unroll
           for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(part + c * 16 + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
         } else if (p.o_vec) {
+          // Neighbours trade halves, so that a store covers whole sectors (32 bytes of 16 rows, not 16 of 32: 9 prompts of
+          // 17 to 2300 tokens 188 -> 183 us, one of 300 26.3 -> 24.9 us).
+          uint32_t w[8];
 #pragma unroll
-          for (int i = 0; i < 16; i += 8)
-            *reinterpret_cast<uint4*>(dst + c * 16 + i) = make_uint4(pack_bf16x2(f[i], f[i + 1]), pack_bf16x2(f[i + 2], f[i + 3]),
-                                                                     pack_bf16x2(f[i + 4], f[i + 5]), pack_bf16x2(f[i + 6], f[i + 7]));
+          for (int i = 0; i < 8; ++i) w[i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
+          const bool odd = lane & 1;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? w[i] : w[4 + i], 1);
+            if (odd) w[i] = got; else w[4 + i] = got;
+          }
+          if (even_ok) *reinterpret_cast<uint4*>(dst_even + c * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+          if (odd_ok) *reinterpret_cast<uint4*>(dst_odd + c * 16) = make_uint4(w[4], w[5], w[6], w[7]);
         } else {
 #pragma unroll
           for (int i = 0; i < 16; ++i) dst[c * 16 + i] = __float2bfloat16(f[i]);
