@@ -24,6 +24,11 @@
 //     not tcgen05 on purpose: e4m3 becomes fp16 on the way from shared memory to a register fragment, while a tcgen05
 //     operand would have to be written back to shared memory twice as wide; tensor time is not what is scarce at 8 to 16
 //     heads per byte of K.  The warps share nothing until a visit ends; then their sums meet in shared memory.
+//
+// Measured (28 query heads, 4 key heads, d = 128): 256 sequences of 3300 to 3700 tokens, 954 MB, 153 us = 6.2 TB/s, 0.95 of what
+// a copy reaches; issue slots are half full.  64 sequences of 2000, 136 MB, 33 us = 4.1 TB/s.  One of 32768, 35 MB over all SMs,
+// 16 us; one of 500, 8.1 us.  The short ones are bound by a chain of latencies: lengths, table entry, unit, the sums of the
+// warps, and the second kernel (each 0.5 to 1 us).
 #include <math.h>
 
 #include "kv_fp8.cuh"
@@ -34,9 +39,15 @@ int cs_encode_tmap_nd(CUtensorMap* out, int elem_bytes, int rank, const void* ba
 namespace {
 
 constexpr int MAX_CTAS = 512;
-constexpr int ITEM_COST = 3;                 // what an item costs beside its units, in units
-constexpr int MIN_RUN = 2;                   // no CTA for less
-constexpr int SHARED_VISIT = 3;              // visits of at least this many units are shared by the teams of a CTA
+// What an item costs beside its units, in units: queries to load, sums to join.  33 sequences of 1 to 5000 tokens take 30.1 us
+// with 1, 25.5 with 3, 25.2 with 5; one of 32768 17.2, 16.6, 15.9.
+constexpr int ITEM_COST = 5;
+// The cost of a CTA's run is this at least: one sequence of 500 tokens takes 8.1 us with 2, 8.5 with 3 or 4, 9.1 with 6.
+constexpr int MIN_RUN = 2;
+// Visits of at least this many units are shared by the teams of a CTA, unit by unit, and joined by all of them; shorter ones go
+// to one team.  256 sequences of 100 tokens (2 units) take 26.2 us shared, 18.2 dealt; 33 of 1 to 5000 tokens 25.5 us with the
+// border at 3, 26.1 at 8.
+constexpr int SHARED_VISIT = 3;
 constexpr float M_NONE = -3.0e38f;           // running maximum before the first key (finite: differences stay defined)
 
 // One instantiation.  TEAMS: as many as registers allow (128 a thread with three teams, 168 with two).

@@ -9,6 +9,11 @@
 // sine are cs[t].  All of it is fp32; nothing is rounded between the norm, the rotation and the quantisation, so a query
 // is rounded once and a cache row twice less than through bf16.  amax is at least 2^-40, so a scale is never zero; a row
 // that holds an infinity or NaN gets the scale NaN, which spreads into every score or output that reads the row.
+//
+// Bound by its bytes: 18944 tokens of 28 query and 4 key heads (d = 128), 339 MB, take 61.3 us = 5.5 TB/s, 0.85 of what a copy
+// reaches; most of a warp's time is the wait for its row.  Blocks of 128 threads, 12 to an SM (40 registers): 256 threads 70 us,
+// 64 threads 90, 512 threads 87, 16 blocks of 128 65.  Several rows of a token to a team, so that they share cos and sin: 72 to
+// 78 us against 71 for one, when blocks had 256 threads.  One token takes 1.9 us.
 #include "kv_fp8.cuh"
 
 namespace {
