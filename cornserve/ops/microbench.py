@@ -6,6 +6,9 @@
   python -m cornserve.ops.microbench attn-window 4 [1]        # Qwen2.5-VL windows of 4 1280x720 images (1: packed tiles)
   python -m cornserve.ops.microbench attn-full 16 80 4784 0   # heads, head_dim, length, causal
   python -m cornserve.ops.microbench attn-decode 48 3500      # sequences, context
+  python -m cornserve.ops.microbench attn-decode-fp8 128 3500 # the same over the 8-bit cache
+  python -m cornserve.ops.microbench attn-prefill-fp8 8 2000  # causal prompts over the 8-bit cache: sequences, length
+  python -m cornserve.ops.microbench kv-append-fp8 18944      # rotation, quantisation and append of that many tokens
   python -m cornserve.ops.microbench norm 19136 1280
   python -m cornserve.ops.microbench adaln 8192 3072          # LayerNorm + AdaLN modulation (two samples)
   python -m cornserve.ops.microbench qk-norm-rope 8704 24     # per-head RMSNorm + rotation of q and k, d = 128
@@ -197,6 +200,35 @@ def main() -> None:
         q = rnd(B, Hq, d)
         secs = t(lambda: ops.attention_paged(q, cache, bt, kv_len, cu, 1, causal=True, pack_gqa=True))
         report(f"attn-decode B={B} ctx={ctx}", secs, 4.0 * B * Hq * d * ctx, 2.0 * 2 * B * Hkv * ctx * d)
+    elif k in ("attn-decode-fp8", "attn-prefill-fp8", "kv-append-fp8"):
+        if k == "kv-append-fp8":
+            B, ctx = 1, a.args[0] if a.args else 18944
+        else:
+            B, ctx = (a.args + [128, 3500][len(a.args):])[:2]
+        Hq, Hkv, d = 28, 4, 128
+        blocks = -(-ctx // 128)
+        cache = ops.kv_cache_fp8(B * blocks, Hkv, d, dev)
+        bt = torch.arange(B * blocks, device=dev, dtype=torch.int32).view(B, blocks)
+        slot = (bt.long()[:, :, None] * 128 + torch.arange(128, device=dev)).flatten(1)[:, :ctx].flatten().int()
+        kv_len = torch.full((B,), ctx, device=dev, dtype=torch.int32)
+        ang = torch.arange(ctx, device=dev)[:, None] * 1e6 ** (-torch.arange(d // 2, device=dev) * 2 / d)
+        cs = torch.stack([ang.cos(), ang.sin()], dim=1).float().contiguous()
+        qkv = rnd(ctx, (Hq + 2 * Hkv) * d)
+        for b in range(B):
+            q = ops.rope_kv_write_fp8_(qkv, Hq, Hkv, d, cs, cache, slot[b * ctx: (b + 1) * ctx])
+        if k == "kv-append-fp8":
+            secs = t(lambda: ops.rope_kv_write_fp8_(qkv, Hq, Hkv, d, cs, cache, slot))
+            report(f"{k} {ctx} tokens", secs, 0.0, ctx * ((2 * Hq + 2 * Hkv) * d * 2.0 + d * 4 + 4 + 2 * Hkv * (d + 4)))
+        elif k == "attn-decode-fp8":
+            cu = torch.arange(B + 1, device=dev, dtype=torch.int32)
+            q = rnd(B, Hq, d)
+            secs = t(lambda: ops.attention_paged_fp8(q, cache, bt, kv_len, cu, 1))
+            report(f"{k} B={B} ctx={ctx}", secs, 4.0 * B * Hq * d * ctx, 2.0 * B * Hkv * ctx * (d + 4) + 4.0 * B * Hq * d)
+        else:
+            cu = torch.arange(B + 1, device=dev, dtype=torch.int32) * ctx
+            q = q.repeat(B, 1, 1)
+            secs = t(lambda: ops.attention_paged_fp8(q, cache, bt, kv_len, cu, ctx))
+            report(f"{k} B={B} length={ctx}", secs, 2.0 * B * Hq * d * ctx * (ctx + 1), 2.0 * B * Hkv * ctx * (d + 4) + 4.0 * B * ctx * Hq * d)
     elif k == "norm":
         rows, H = a.args[:2]
         x, r, w = rnd(rows, H), rnd(rows, H), rnd(H)
