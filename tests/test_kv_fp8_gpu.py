@@ -317,6 +317,36 @@ def test_a_nan_row_spreads_only_to_the_queries_that_see_it(n):
     assert not torch.isnan(out[: n - 1]).any() and not torch.isnan(out[n:]).any()
 
 
+@pytest.mark.parametrize("n", [1, 20])
+def test_a_query_that_is_no_number_spoils_its_own_row_only(n):
+    lens, new = [300, 70], [n, n]
+    q, cache, table, kv_len, cu = _setup(lens, new, 14, 2, 128, seed=15)
+    q[0, 3, 5] = float("nan")
+    q[0, 4, 127] = float("inf")
+    q[n, 13, 0] = float("-inf")
+    q[2 * n - 1, 0] = 0.0
+    out = ops.attention_paged_fp8(q, cache, table, kv_len, cu, n)
+    bad = torch.zeros(2 * n, 14, dtype=torch.bool, device=DEV)
+    bad[0, 3] = bad[0, 4] = bad[n, 13] = True
+    assert torch.isnan(out[bad]).all() and torch.isfinite(out[~bad]).all()
+    clean = q.clone()
+    clean[bad] = 0.0
+    got = torch.where(bad[..., None], ops.attention_paged_fp8(clean, cache, table, kv_len, cu, n), out)
+    _check(got, clean, cache, table, lens, new)
+
+
+@pytest.mark.parametrize("n", [1, 20])
+def test_pages_shared_by_sequences_and_tables_shared_by_all(n):
+    q, cache, table, kv_len, cu = _setup([333], [n], 8, 2, 64, seed=16)
+    lens = [333, 200, 129, 333]
+    big = torch.cat([q] * 4)
+    cu4 = _i32([0, n, 2 * n, 3 * n, 4 * n])
+    for shared in (table.expand(4, -1), table.repeat(4, 1)):
+        out = ops.attention_paged_fp8(big, cache, shared, _i32(lens), cu4, n)
+        _check(out, big, cache, table.repeat(4, 1), lens, [n] * 4)
+        assert torch.equal(shared, table.repeat(4, 1))
+
+
 @pytest.mark.parametrize("new", [[1] * 6, [64, 3, 0, 5, 129, 40]])
 def test_tables_and_lengths_that_do_not_fit_are_reported(new):
     lens = [300, 64, 10, 129, 500, 40]
