@@ -383,7 +383,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
     const int my_row = (warp & 3) * RPW + lane % RPW + STEP * (lane / RPW);
     uint32_t n = 0, n_item = 0;                    // running counts: pages, items
     // A tile in registers: codes, the scale of row `my_row` (with keys that of the value row too), the scales of keys 4 lane .. + 3
-    uint4 code[ITER];
+    constexpr int PART = 4, PARTS = ITER / PART;   // a tile is converted in parts, with the next part's codes on their way
+    uint4 code[PART];
     float row_s, row_vs = 0.f;
     float4 all_s;
     int rows = 0;                                  // rows that are keys of the sequence (may exceed 128)
@@ -405,8 +406,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         row_vs = __ldg(values + my_row);
       }
     };
-    auto fetch_codes = [&](const uint8_t* block, int i) {
-      code[i] = __ldg(reinterpret_cast<const uint4*>(block + row0 * D + c0 * 16 + i * STEP * D));
+    auto fetch_codes = [&](const uint8_t* from, int i) {
+      code[i] = __ldg(reinterpret_cast<const uint4*>(from + row0 * D + c0 * 16 + i * STEP * D));
     };
     auto finite_bits = [](float f) { const uint32_t b = __float_as_uint(f) & 0x7fffffffu; return b < 0x7f800000u ? b : 0u; };
     auto is_finite = [](float f) { return (__float_as_uint(f) & 0x7fffffffu) < 0x7f800000u; };
@@ -447,30 +448,36 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
       }
       mbar_arrive(&sc_full[s]);
     };
-    // Convert the tile in hand and, chunk by chunk, fetch the next one into the registers that become free.
-    auto convert = [&](uint32_t parts, const uint8_t* next, int e, float cq, bool pub) {
+    // Convert a tile and, chunk by chunk, fetch the next part into the registers that become free.  (Parts of 64 of 128 rows at
+    // d = 128: half the registers and code of a whole tile at once, 9 prompts of 17 to 2300 tokens 180 -> 178 us; quarters 182.)
+    auto convert = [&](uint32_t parts, const uint8_t* block, const uint8_t* next, int e, float cq, bool pub) {
       const uint32_t slot = n % RING;
       mbar_wait(&kv_empty[kv][slot], ((n / RING) & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
       if (pub) publish(e, cq);
       uint8_t* tile = s_kv + (kv * RING + slot) * TILE;
-      if (rows < KV8_PAGE) {                       // what lies behind the keys may be anything
+#pragma unroll 1
+      for (int k = 0; k < PARTS; ++k, tile += PART * STEP * 128) {
+        const uint8_t* from = k + 1 < PARTS ? block + (k + 1) * PART * STEP * D : next;
+        const int row = row0 + k * PART * STEP, first = k * PART * RPW + row0 % RPW;
+        if (rows < KV8_PAGE) {                     // what lies behind the keys may be anything
 #pragma unroll
-        for (int i = 0; i < ITER; ++i)
-          if (row0 + i * STEP >= rows) code[i] = make_uint4(0, 0, 0, 0);
-      }
+          for (int i = 0; i < PART; ++i)
+            if (row + i * STEP >= rows) code[i] = make_uint4(0, 0, 0, 0);
+        }
 #pragma unroll
-      for (int i = 0; i < ITER; ++i) {
-        const uint32_t f = __shfl_sync(0xffffffffu, parts, i * RPW + row0 % RPW);
-        const uint32_t hi = __byte_perm(f, 0, 0x1010), lo = __byte_perm(f, 0, 0x3232);
-        const uint32_t w[4] = {code[i].x, code[i].y, code[i].z, code[i].w};
-        fetch_codes(next, i);
-        uint32_t h[8];
+        for (int i = 0; i < PART; ++i) {
+          const uint32_t f = __shfl_sync(0xffffffffu, parts, first + i * RPW);
+          const uint32_t hi = __byte_perm(f, 0, 0x1010), lo = __byte_perm(f, 0, 0x3232);
+          const uint32_t w[4] = {code[i].x, code[i].y, code[i].z, code[i].w};
+          fetch_codes(from, i);
+          uint32_t h[8];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) e4m3x4_to_half2x2(w[k], h[2 * k], h[2 * k + 1]);
+          for (int c = 0; c < 4; ++c) e4m3x4_to_half2x2(w[c], h[2 * c], h[2 * c + 1]);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) h[k] = scaled(h[k], hi, lo);
-        *reinterpret_cast<uint4*>(tile + off_a + i * STEP * 128) = make_uint4(h[0], h[1], h[2], h[3]);
-        *reinterpret_cast<uint4*>(tile + off_b + i * STEP * 128) = make_uint4(h[4], h[5], h[6], h[7]);
+          for (int c = 0; c < 8; ++c) h[c] = scaled(h[c], hi, lo);
+          *reinterpret_cast<uint4*>(tile + off_a + i * STEP * 128) = make_uint4(h[0], h[1], h[2], h[3]);
+          *reinterpret_cast<uint4*>(tile + off_b + i * STEP * 128) = make_uint4(h[4], h[5], h[6], h[7]);
+        }
       }
       fence_proxy_async_smem();
       mbar_arrive(&kv_full[kv][slot]);
@@ -483,7 +490,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
       const uint8_t* block = block_of(head, page_of(it, it.j0));
       fetch_scales(block);
 #pragma unroll
-      for (int i = 0; i < ITER; ++i) fetch_codes(block, i);
+      for (int i = 0; i < PART; ++i) fetch_codes(block, i);
       int page = page_of(it, it.j0 + 1);
       float cq = 0.f;
 #pragma unroll 1
@@ -492,10 +499,11 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         uint32_t parts;
         rows = it.k_len - j * KV8_PAGE;
         const int e = multiplier(parts);
+        const uint8_t* here = block;
         if (j + 1 < it.j0 + it.n) block = block_of(head, page);   // (behind the last page the same one is read again)
         fetch_scales(block);
         page = page_of(it, j + 2);
-        convert(parts, block, e, cq, j > it.j0);
+        convert(parts, here, block, e, cq, j > it.j0);
         if (j > it.j0) continue;
         // The queries come behind the first tile, which does not need them: the item before is still at work on its own.
         // Queries, one tile per group, D / 8 lanes per row: copied as they are to the place where their fp16 form will be, all
@@ -576,6 +584,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
       const int tok = it.t0 + t * p.tok_per_tile + tl;
       const bool row_ok = tl < p.tok_per_tile && tok < it.q_len && g < it.n_heads;
       const int lim = p.causal ? min(it.k_len, tok + it.shift + 1) : it.k_len;     // keys [0, lim) are visible
+      const int wmin = __reduce_min_sync(0xffffffffu, lim);                        // ... to all rows of the warp
       float m = M_NONE;
       float l = 0.f;
       for (int j = 0; j < it.n; ++j, ++n_step) {
@@ -585,10 +594,11 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         tc_fence_after();
         const float4 sc = s_scale[s];
         const int nvalid = lim - (it.j0 + j) * KV8_PAGE;       // visible keys of the page (may be negative or beyond 128)
+        const int wvalid = wmin - (it.j0 + j) * KV8_PAGE;      // the same for every row of the warp: no divergent branch
         // first pass: the largest S of the row
         float mx0 = -INFINITY, mx1 = -INFINITY;
         auto largest = [&](uint32_t (&x)[32], int c) {
-          if (nvalid < c + 32) {                     // hidden keys: whatever is there
+          if (wvalid < c + 32) {                     // hidden keys: whatever is there
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (c + i >= nvalid) x[i] = 0xff800000u;
@@ -632,7 +642,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         const uint64_t mul2 = pack2(sc.x, sc.x), ref2 = pack2(add, add);
         uint64_t sum_a = pack2(0.f, 0.f), sum_b = sum_a;
         auto weigh = [&](uint32_t (&x)[32], int c) {
-          if (nvalid < c + 32) {
+          if (wvalid < c + 32) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (c + i >= nvalid) x[i] = 0xff800000u;
@@ -649,7 +659,6 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
             pk[i >> 1] = half2_bits(e0, e1);
             pk[(i >> 1) + 1] = half2_bits(e2, e3);
           }
-          __syncwarp();
           tmem_st16(tS + (c >> 1), pk);
         };
 #pragma unroll 1
