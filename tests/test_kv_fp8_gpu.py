@@ -531,6 +531,20 @@ def test_graphs_replayed_at_once_on_two_streams_and_with_new_lengths(n):
     _check(out, q, cache, table, lens, [n] * B)
 
 
+def test_pages_pulled_into_another_cache_give_the_same_attention():
+    lens = [300, 129]
+    q, cache, table, kv_len, cu = _setup(lens, [1, 1], 28, 4, 128, seed=41)
+    src = torch.stack([cache, cache.flip(0)])                       # two layers
+    dst = torch.zeros(2, 9, *cache.shape[1:], device=DEV, dtype=torch.uint8)
+    old = [int(p) for row, n in zip(table.tolist(), lens) for p in row[: -(-n // 128)]]
+    new = [8, 1, 4, 6, 2]
+    ops.kv_copy_pages(dst, src, _i32(old), _i32(new))
+    moved = _i32([new[:3], new[3:] + [-7]])
+    a = ops.attention_paged_fp8(q, cache, table, kv_len, cu, 1)
+    assert torch.equal(a, ops.attention_paged_fp8(q, dst[0], moved, kv_len, cu, 1))
+    assert torch.equal(dst[1, new], src[1, old]) and not dst[:, 0].any()
+
+
 def test_engine_with_an_8_bit_cache_decodes_from_graphs_like_it_does_eagerly():
     import numpy as np
 
