@@ -188,15 +188,18 @@ template <int UNIT>
 struct Walk {
   int seq, head, u;
   Place end;
-  int row, len, units, n;
+  int known, row, len, units, n;   // row, len and units are those of sequence `known`
   uint32_t dealt;   // short visits and units of shared visits so far: deals the next ones to the teams in turn
   __device__ __forceinline__ bool settle(const DecParams& p) {   // on to an item with units for this CTA
     const int heads = p.Hkv * p.head_blocks;
     while (seq < p.B) {
-      const Seq s = get_seq(p, seq);
-      row = s.row;
-      len = s.len;
-      units = (len + UNIT - 1) / UNIT;
+      if (known != seq) {
+        const Seq s = get_seq(p, seq);
+        known = seq;
+        row = s.row;
+        len = s.len;
+        units = (len + UNIT - 1) / UNIT;
+      }
       const bool last = seq == end.seq && head == end.head;
       if (seq > end.seq || (last && u >= end.u)) return false;
       n = (last ? min(end.u, units) : units) - u;
@@ -244,11 +247,14 @@ attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_codes, const 
   __shared__ float s_m[WARPS][HEADS], s_l[WARPS][HEADS];
   __shared__ int abort_flag, s_warp_sum[ALL_WARPS];
   __shared__ Place s_cut[2];       // where the run begins and ends
+  __shared__ Seq s_first;          // the sequence it begins in (or ahead of)
+  __shared__ int s_first_seq;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     abort_flag = 0;
     s_cut[0] = s_cut[1] = Place{p.B, 0, 0};
+    s_first_seq = -1;
     for (int w = 0; w < TEAMS; ++w) {
       for (int s = 0; s < RING; ++s) { mbar_init(&full[w][s], 1); mbar_init(&empty[w][s], 4); }
       for (int s = 0; s < QSLOTS; ++s) { mbar_init(&q_full[w][s], 1); mbar_init(&q_empty[w][s], 4); }
@@ -266,11 +272,13 @@ attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_codes, const 
   // Thread i adds up the cost of `per` consecutive sequences (one, unless the batch is huge); a scan over the threads gives
   // the total and who owns the two cuts.  The host has checked that 32 bits hold every sum.
   const int heads = p.Hkv * p.head_blocks, per = (p.B + THREADS - 1) / THREADS;
-  auto units_of = [&](int b) { return b < p.B ? (get_seq(p, b).len + UNIT - 1) / UNIT : 0; };
+  auto seq_of = [&](int b) { return b < p.B ? get_seq(p, b) : Seq{-1, 0}; };
+  auto units_of = [&](const Seq& q) { return (q.len + UNIT - 1) / UNIT; };
   auto cost = [&](int units) { return units > 0 ? (units + ITEM_COST) * heads : 0; };
   const int first = static_cast<int>(threadIdx.x) * per;
-  int mine = 0;
-  for (int i = 0; i < per; ++i) mine += cost(units_of(first + i));
+  const Seq seq0 = seq_of(first);
+  int mine = cost(units_of(seq0));
+  for (int i = 1; i < per; ++i) mine += cost(units_of(seq_of(first + i)));
   int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -279,12 +287,9 @@ attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_codes, const 
   }
   if (lane == 31) s_warp_sum[warp] = incl;
   __syncthreads();
-  int total = 0;
-#pragma unroll
-  for (int w = 0; w < ALL_WARPS; ++w) {
-    if (w == warp) incl += total;
-    total += s_warp_sum[w];
-  }
+  const int of_lane = lane < ALL_WARPS ? s_warp_sum[lane] : 0;
+  const int total = __reduce_add_sync(0xffffffffu, of_lane);
+  incl += __reduce_add_sync(0xffffffffu, lane < warp ? of_lane : 0);
   // (at least MIN_RUN each: then the CTAs that share an item are consecutive)
   const int active = max(1, min(total / MIN_RUN, static_cast<int>(gridDim.x))), c = blockIdx.x;
   const int quota = total / active, extra = total - quota * active;
@@ -293,12 +298,14 @@ attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_codes, const 
     const int r = c + e >= active ? total : quota * (c + e) + min(c + e, extra);
     int at0 = incl - mine;
     if (r >= at0 && r < incl) {
-      int i = 0, units = units_of(first);
-      while (i + 1 < per && r >= at0 + cost(units)) {
-        at0 += cost(units);
-        units = units_of(first + ++i);
+      int i = 0;
+      Seq q = seq0;
+      while (i + 1 < per && r >= at0 + cost(units_of(q))) {
+        at0 += cost(units_of(q));
+        q = seq_of(first + ++i);
       }
-      s_cut[e] = place_at(first + i, units, heads, r - at0);
+      s_cut[e] = place_at(first + i, units_of(q), heads, r - at0);
+      if (e == 0) { s_first = q; s_first_seq = first + i; }
     }
   }
   __syncthreads();
@@ -308,6 +315,10 @@ attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_codes, const 
   wk.head = s_cut[0].head;
   wk.u = s_cut[0].u;
   wk.end = s_cut[1];
+  wk.known = s_first_seq;
+  wk.row = s_first.row;
+  wk.len = s_first.len;
+  wk.units = units_of(s_first);
   const bool any = wk.settle(p);
 
   if (warp >= WARPS) {
