@@ -108,8 +108,7 @@ struct Pos { int seq, blk, pair, page; };
 
 // The place at distance r (cost units) into the row blocks of sequence `seq`.  Cuts that would leave less than two pages of
 // an item on one side move to its edge.
-__device__ __forceinline__ Pos place_at(const PrefillParams& p, int seq, long long r) {
-  const Seq q = get_seq(p, seq);
+__device__ __forceinline__ Pos place_at(const PrefillParams& p, int seq, const Seq& q, long long r) {
   const int pairs = pairs_of(p, q);
   const long long per_blk = cost_of(p, q, pairs);
   Pos at{seq, static_cast<int>(quotient(r, per_blk)), 0, 0};
@@ -239,6 +238,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
   __shared__ Pos s_pos[2];
   __shared__ long long s_sum[THREADS / 32], s_cut[2];
   __shared__ int s_cut_seq[2];
+  __shared__ Seq s_cut_q[2];
   __shared__ uint32_t s_max[8], s_row[128];   // s_row: token in tile | head << 16 of a tile row
   __shared__ float4 s_scale[SRING];     // of a page: factor from S to base-2 exponents, F, 2^-F
 
@@ -266,9 +266,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
   // the total and who owns the two cuts.
   {
     const int per = (p.B + THREADS - 1) / THREADS, b0 = min(static_cast<int>(threadIdx.x) * per, p.B), b1 = min(b0 + per, p.B);
-    auto seq_cost = [&](int b) { const Seq q = get_seq(p, b); return cost_of(p, q, pairs_of(p, q)) * p.blocks; };
-    long long mine = 0;
-    for (int b = b0; b < b1; ++b) mine += seq_cost(b);
+    auto seq_cost = [&](const Seq& q) { return cost_of(p, q, pairs_of(p, q)) * p.blocks; };
+    const Seq first = b0 < b1 ? get_seq(p, b0) : Seq{0, 0, 0, 0};
+    long long mine = seq_cost(first);
+    for (int b = b0 + 1; b < b1; ++b) mine += seq_cost(get_seq(p, b));
     long long incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -289,17 +290,20 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
       if (r >= incl - mine && r < incl) {
         long long at = incl - mine;
         int b = b0;
-        for (; b + 1 < b1; ++b) {
-          const long long x = seq_cost(b);
+        Seq q = first;
+        while (b + 1 < b1) {
+          const long long x = seq_cost(q);
           if (r < at + x) break;
           at += x;
+          q = get_seq(p, ++b);
         }
         s_cut_seq[e] = b;
         s_cut[e] = r - at;
+        s_cut_q[e] = q;
       }
     }
     __syncthreads();
-    if (warp < 2 && lane == 0) s_pos[warp] = s_cut_seq[warp] < p.B ? place_at(p, s_cut_seq[warp], s_cut[warp]) : Pos{p.B, 0, 0, 0};
+    if (warp < 2 && lane == 0) s_pos[warp] = s_cut_seq[warp] < p.B ? place_at(p, s_cut_seq[warp], s_cut_q[warp], s_cut[warp]) : Pos{p.B, 0, 0, 0};
     __syncthreads();
     if (lane == 0) s_walk[warp] = Walk{s_pos[0], s_pos[1]};
     __syncwarp();
