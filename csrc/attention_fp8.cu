@@ -486,10 +486,30 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
       fence_proxy_async_smem();
       mbar_arrive(&kv_full[kv][slot]);
     };
+    // Queries, one tile per group, D / 8 lanes per row: copied as they are to the place where their fp16 form will be, all
+    // in flight at once.
+    constexpr int LANES = D / 8, PER = 32 / LANES, PASSES = 32 / PER;     // lanes per row, rows per warp and pass, passes
+    const int ch = lane % LANES, row_w = (warp & 3) * PER + lane / LANES;
+    // row i * 4 * PER + row_w: its swizzle is the same in all passes (4 * PER is a multiple of 8)
+    uint8_t* q_at = s_q + kv * TILE + (ch >> 3) * ATOM + row_w * 128 + (((ch & 7) ^ (row_w & 7)) << 4);
+    auto fetch_queries = [&](const Item& it) {
+      const int t0 = it.t0 + kv * p.tok_per_tile, n_tok = min(p.tok_per_tile, it.q_len - t0);
+      const __nv_bfloat16* src0 = p.q + (it.q_beg + (n_tok > 0 ? t0 : 0)) * p.q_tok + it.h0 * D + ch * 8;
+      const uint32_t q_sm = smem_u32(q_at);
+#pragma unroll 8
+      for (int i = 0; i < PASSES; ++i) {
+        const uint32_t rc = s_row[i * 4 * PER + row_w];                   // token in tile | head << 16
+        const int tl = rc & 0xffff, g = rc >> 16;
+        const bool ok = tl < n_tok && g < it.n_heads;
+        const __nv_bfloat16* src = ok ? src0 + tl * p.q_tok + g * D : src0;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(q_sm + i * 4 * PER * 128), "l"(src), "r"(ok ? 16 : 0) : "memory");
+      }
+    };
     Item visit;
     while (next_visit(p, walk, &visit)) {
       const Item it = visit;
       if (it.n == 0) continue;
+      if (n_item == 0) fetch_queries(it);            // their place is free (one prompt of 300 tokens: 24.5 -> 24.1 us)
       const uint8_t* head = p.cache + (static_cast<long long>(kv) * p.Hkv + it.hk) * kv8_block_bytes(D);
       const uint8_t* block = block_of(head, page_of(it, it.j0));
       fetch_scales(block);
@@ -509,28 +529,13 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         page = page_of(it, j + 2);
         convert(parts, here, block, e, cq, j > it.j0);
         if (j > it.j0) continue;
-        // The queries come behind the first tile, which does not need them: the item before is still at work on its own.
-        // Queries, one tile per group, D / 8 lanes per row: copied as they are to the place where their fp16 form will be, all
-        // in flight at once; then the largest finite magnitude of both tiles, and fp16 with a common scale in place.
-        constexpr int LANES = D / 8, PER = 32 / LANES, PASSES = 32 / PER;     // lanes per row, rows per warp and pass, passes
-        const int ch = lane % LANES, row_w = (warp & 3) * PER + lane / LANES;
-        // row i * 4 * PER + row_w: its swizzle is the same in all passes (4 * PER is a multiple of 8)
-        uint8_t* q_at = s_q + kv * TILE + (ch >> 3) * ATOM + row_w * 128 + (((ch & 7) ^ (row_w & 7)) << 4);
-        mbar_wait(&q_empty, (n_item & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
-        ++n_item;
-        {
-          const int t0 = it.t0 + kv * p.tok_per_tile, n_tok = min(p.tok_per_tile, it.q_len - t0);
-          const __nv_bfloat16* src0 = p.q + (it.q_beg + (n_tok > 0 ? t0 : 0)) * p.q_tok + it.h0 * D + ch * 8;
-          const uint32_t q_sm = smem_u32(q_at);
-#pragma unroll 8
-          for (int i = 0; i < PASSES; ++i) {
-            const uint32_t rc = s_row[i * 4 * PER + row_w];                   // token in tile | head << 16
-            const int tl = rc & 0xffff, g = rc >> 16;
-            const bool ok = tl < n_tok && g < it.n_heads;
-            const __nv_bfloat16* src = ok ? src0 + tl * p.q_tok + g * D : src0;
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(q_sm + i * 4 * PER * 128), "l"(src), "r"(ok ? 16 : 0) : "memory");
-          }
+        // The queries of later items come behind the first tile, which does not need them: the item before is still at work on
+        // its own.  Then the largest finite magnitude of both tiles, and fp16 with a common scale in place.
+        if (n_item > 0) {
+          mbar_wait(&q_empty, (n_item & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
+          fetch_queries(it);
         }
+        ++n_item;
         asm volatile("cp.async.wait_all;" ::: "memory");
         auto largest = [&](bool finite_only) {
           uint32_t m2 = 0;                           // two 16-bit maxima
