@@ -27,7 +27,7 @@
 //
 // Measured (28 query heads, 4 key heads, d = 128): 256 sequences of 3300 to 3700 tokens, 954 MB, 153 us = 6.2 TB/s, 0.95 of what
 // a copy reaches; issue slots are half full.  64 sequences of 2000, 136 MB, 33 us = 4.1 TB/s.  One of 32768, 35 MB over all SMs,
-// 16 us; one of 500, 8.1 us.  The short ones are bound by a chain of latencies: lengths, table entry, unit, the sums of the
+// 15.6 us; one of 500, 7.7 us.  The short ones are bound by a chain of latencies: lengths, table entry, unit, the sums of the
 // warps, and the second kernel (each 0.5 to 1 us).
 #include <math.h>
 
