@@ -8,6 +8,7 @@ PyTorch-kernel fallback for CUDA tensors: a missing library raises.
 
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -522,8 +523,10 @@ def rope_kv_write_fp8_(qkv: torch.Tensor, Hq: int, Hkv: int, d: int, cs: torch.T
     if not qkv.is_cuda:
         return reference.rope_kv_write_fp8(qkv, Hq, Hkv, d, cs, cache, slot, q_norm, k_norm, eps)
     _check_kv_fp8_cuda(cache, d, qkv)
-    if qkv.stride(1) != 1 or qkv.stride(0) % 8 or qkv.data_ptr() % 16:
+    ld, step = qkv.stride()
+    if step != 1 or ld % 8 or qkv.data_ptr() % 16:
         qkv = qkv.clone(memory_format=torch.contiguous_format)
+        ld = qkv.stride(0)
     q = qkv.new_empty((T, Hq, d))
     if T == 0:
         return q
@@ -532,10 +535,15 @@ def rope_kv_write_fp8_(qkv: torch.Tensor, Hq: int, Hkv: int, d: int, cs: torch.T
     if cs.data_ptr() % 16:
         cs = cs.clone()
     lib = _lib.load()
-    _chk(lib.cs_rope_kv_write_fp8(qkv.data_ptr(), qkv.stride(0), T, Hq, Hkv, d, cs.data_ptr(), _ptr(q_norm), _ptr(k_norm), eps,
+    _chk(lib.cs_rope_kv_write_fp8(qkv.data_ptr(), ld, T, Hq, Hkv, d, cs.data_ptr(), _ptr(q_norm), _ptr(k_norm), eps,
                                   slot.data_ptr(), q.data_ptr(), cache.data_ptr(), pages, _stream()), "cs_rope_kv_write_fp8")
     _count()
     return q
+
+
+@functools.lru_cache(maxsize=None)
+def _decode_fp8_ws_bytes(Hq: int, Hkv: int, d: int, device: torch.device) -> int:
+    return _lib.load().cs_attention_decode_fp8_ws_bytes(Hq, Hkv, d)     # goes by the SMs of `device`, the current one
 
 
 def attention_paged_fp8(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, kv_len: torch.Tensor, cu_q: torch.Tensor,
@@ -563,8 +571,8 @@ def attention_paged_fp8(q: torch.Tensor, cache: torch.Tensor, block_table: torch
         raise ValueError(f"{Hq} query heads cannot share {Hkv} key heads")
     _check_i32("kv_len", kv_len, B, dev)
     _check_i32("cu_q", cu_q, B + 1, dev)
-    if block_table.dtype is not torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B or block_table.device != dev or \
-            (block_table.stride(1) != 1 and block_table.shape[1] > 1):
+    rows, width = block_table.shape if block_table.dim() == 2 else (-1, 0)
+    if block_table.dtype is not torch.int32 or rows != B or block_table.device != dev or (width > 1 and block_table.stride(1) != 1):
         raise ValueError(f"block_table must be int32 [{B}, blocks] on {dev} with contiguous rows; got {block_table.dtype} "
                          f"{list(block_table.shape)} on {block_table.device}")
     if max_q_len < 0:
@@ -576,27 +584,29 @@ def attention_paged_fp8(q: torch.Tensor, cache: torch.Tensor, block_table: torch
     if not q.is_cuda:
         return reference.attention_paged_fp8(q, cache, block_table, kv_len, cu_q, scale, causal, out)
     _check_kv_fp8_cuda(cache, d, q)
-    if q.stride(2) != 1 or q.stride(1) != d or q.stride(0) % 8 or q.data_ptr() % 16:
+    q_tok, q_head, step = q.stride()
+    if step != 1 or q_head != d or q_tok % 8 or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
+        q_tok = Hq * d
     if out is None:
         out = q.new_empty((Tq, Hq, d))
     if Tq == 0 or B == 0 or max_q_len == 0:
         return out
     lib = _lib.load()
-    width = block_table.shape[1]
+    o_tok, o_head, _ = out.stride()
     # scratch belongs to the call: calls on several streams, and captured graphs, never share it
     if max_q_len == 1 and Tq == B:
-        nbytes = lib.cs_attention_decode_fp8_ws_bytes(Hq, Hkv, d)
+        nbytes = _decode_fp8_ws_bytes(Hq, Hkv, d, dev)
         ws = cache.new_empty(nbytes)
-        _chk(lib.cs_attention_decode_fp8(q.data_ptr(), q.stride(0), cache.data_ptr(), pages, out.data_ptr(), out.stride(0),
-                                         out.stride(1), cu_q.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(), block_table.stride(0), width, B, Hq,
+        _chk(lib.cs_attention_decode_fp8(q.data_ptr(), q_tok, cache.data_ptr(), pages, out.data_ptr(), o_tok, o_head,
+                                         cu_q.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(), block_table.stride(0), width, B, Hq,
                                          Hkv, d, scale, ws.data_ptr(), nbytes, _stream()), "cs_attention_decode_fp8")
         _count(2)
         return out
     nbytes = lib.cs_attention_prefill_fp8_ws_bytes(Tq, B, Hq, Hkv, d, width)
     ws = cache.new_empty(nbytes)
-    _chk(lib.cs_attention_prefill_fp8(q.data_ptr(), q.stride(0), cache.data_ptr(), pages, out.data_ptr(), out.stride(0),
-                                      out.stride(1), cu_q.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(), block_table.stride(0),
+    _chk(lib.cs_attention_prefill_fp8(q.data_ptr(), q_tok, cache.data_ptr(), pages, out.data_ptr(), o_tok, o_head,
+                                      cu_q.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(), block_table.stride(0),
                                       width, B, Tq, Hq, Hkv, d, scale, 1 if causal else 0, ws.data_ptr(), nbytes, _stream()),
          "cs_attention_prefill_fp8")
     _count(2)
