@@ -8,8 +8,9 @@
 // enter in fp32 as scalars.  (Scales could stay exact as a vector over the keys that the softmax applies, but every row's
 // thread would have to read it from shared memory: 3 x 128 values per row and page made that the slowest part, at 8400
 // cycles a page and tile pair.)  M_i follows the largest weight, not the largest score, so weights fit fp16 whatever the
-// value scales are.  Queries become fp16 too, scaled by a power of two common to a tile pair (exact for every element
-// within 2^-38 of the pair's largest).
+// value scales are.  Queries become fp16 too, with a power of two per row that brings the row's largest element to the top of
+// the range (every element within 2^-31 of that one is exact); its inverse is part of the row's factor in the softmax, so that
+// rows do not touch each other, however far apart they are.
 //
 // One CTA works on 2 x 128 query rows of one sequence and one key head (rows = tokens x the query heads that share the
 // key head) against pages of 128 keys:
@@ -239,8 +240,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
   __shared__ long long s_sum[THREADS / 32], s_cut[2];
   __shared__ int s_cut_seq[2];
   __shared__ Seq s_cut_q[2];
-  __shared__ uint32_t s_max[8], s_row[128];   // s_row: token in tile | head << 16 of a tile row
-  __shared__ float4 s_scale[SRING];     // of a page: factor from S to base-2 exponents, F, 2^-F
+  __shared__ uint32_t s_row[128];       // token in tile | head << 16 of a tile row
+  __shared__ float s_qscale[2][2][128]; // [item parity][tile][row]: factor from S 2^E to base-2 exponents
+  __shared__ float4 s_scale[SRING];     // of a page: 2^E, F, 2^-F
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -439,13 +441,12 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
     };
     // The scalars of page n, once its tile's place was free.  Their own place was that of page n - SRING, which both softmax
     // groups are done with: the tile of page n - RING is free only behind products that waited for the weights of page
-    // n - RING - 1 or a later one.  (The factor is not 0, also for a scale of 0: a hidden key's -inf times the factor has to
-    // stay -inf.)
-    auto publish = [&](int e, float cq) {
+    // n - RING - 1 or a later one.
+    auto publish = [&](int e) {
       if (tid != 0) return;
       const uint32_t s = n % SRING;
       if (kv == 0) {
-        s_scale[s].x = fmaxf(cq * __uint_as_float(static_cast<uint32_t>(127 + e) << 23), 1e-37f);
+        s_scale[s].x = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
       } else {
         s_scale[s].y = static_cast<float>(e);
         s_scale[s].z = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
@@ -454,10 +455,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
     };
     // Convert a tile and, chunk by chunk, fetch the next part into the registers that become free.  (Parts of 64 of 128 rows at
     // d = 128: half the registers and code of a whole tile at once, 9 prompts of 17 to 2300 tokens 180 -> 178 us; quarters 182.)
-    auto convert = [&](uint32_t parts, const uint8_t* block, const uint8_t* next, int e, float cq, bool pub) {
+    auto convert = [&](uint32_t parts, const uint8_t* block, const uint8_t* next, int e, bool pub) {
       const uint32_t slot = n % RING;
       mbar_wait(&kv_empty[kv][slot], ((n / RING) & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
-      if (pub) publish(e, cq);
+      if (pub) publish(e);
       uint8_t* tile = s_kv + (kv * RING + slot) * TILE;
 #pragma unroll 1
       for (int k = 0; k < PARTS; ++k, tile += PART * STEP * 128) {
@@ -516,7 +517,6 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
 #pragma unroll
       for (int i = 0; i < PART; ++i) fetch_codes(block, i);
       int page = page_of(it, it.j0 + 1);
-      float cq = 0.f;
 #pragma unroll 1
       for (int j = it.j0; j < it.j0 + it.n; ++j, ++n) {
         // the tile of a page, and the next page's scales and codes on their way
@@ -527,57 +527,47 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         if (j + 1 < it.j0 + it.n) block = block_of(head, page);   // (behind the last page the same one is read again)
         fetch_scales(block);
         page = page_of(it, j + 2);
-        convert(parts, here, block, e, cq, j > it.j0);
+        convert(parts, here, block, e, j > it.j0);
         if (j > it.j0) continue;
         // The queries of later items come behind the first tile, which does not need them: the item before is still at work on
-        // its own.  Then the largest finite magnitude of both tiles, and fp16 with a common scale in place.
+        // its own.  Then the largest magnitude of every row, and fp16 scaled by the row's power of two in place.
         if (n_item > 0) {
           mbar_wait(&q_empty, (n_item & 1) ^ 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
           fetch_queries(it);
         }
+        // (two sets of factors: the item before the last is done with its own, since the wait above is behind its softmax)
+        float* row_scale = s_qscale[n_item & 1][kv];
         ++n_item;
         asm volatile("cp.async.wait_all;" ::: "memory");
-        auto largest = [&](bool finite_only) {
-          uint32_t m2 = 0;                           // two 16-bit maxima
-#pragma unroll 8
-          for (int i = 0; i < PASSES; ++i) {
-            const uint4 v = *reinterpret_cast<const uint4*>(q_at + i * 4 * PER * 128);
-            uint32_t w[4] = {v.x & 0x7fff7fffu, v.y & 0x7fff7fffu, v.z & 0x7fff7fffu, v.w & 0x7fff7fffu};
-            if (finite_only) {
-#pragma unroll
-              for (int k = 0; k < 4; ++k) w[k] = ((w[k] & 0xffffu) < 0x7f80u ? w[k] & 0xffffu : 0u) | ((w[k] >> 16) < 0x7f80u ? w[k] & 0xffff0000u : 0u);
-            }
-            m2 = __vmaxu2(m2, __vmaxu2(__vmaxu2(w[0], w[1]), __vmaxu2(w[2], w[3])));
-          }
-          const uint32_t mx = __reduce_max_sync(0xffffffffu, max(m2 & 0xffffu, m2 >> 16));
-          if (lane == 0) s_max[warp - 8] = mx;
-          asm volatile("bar.sync 1, 256;" ::: "memory");
-          uint32_t all = 0;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) all = max(all, s_max[i]);
-          asm volatile("bar.sync 1, 256;" ::: "memory");
-          return all;
-        };
-        uint32_t mx = largest(false);
-        if (mx >= 0x7f80u) mx = largest(true);       // (an infinity or NaN makes its own row NaN and nothing else)
-        const int shift = min(max(127 + 14 - static_cast<int>(mx >> 7), -110), 110);   // the largest element into [2^14, 2^15)
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + kv) : "memory");     // the rows of this tile are there
+        uint8_t* row_at = s_q + kv * TILE + tid * 128;                  // one thread per row
+        const int swizzle = (tid & 7) << 4;
+        auto chunk = [&](int c) { return reinterpret_cast<uint4*>(row_at + (c >> 3) * ATOM + (((c & 7) << 4) ^ swizzle)); };
+        uint32_t m2 = 0;                             // largest magnitudes as bf16, of even and odd channels
+#pragma unroll 4
+        for (int c = 0; c < D / 8; ++c) {
+          const uint4 v = *chunk(c);
+          m2 = __vmaxu2(m2, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
+        }
+        const int ex = static_cast<int>(max(m2 & 0xffffu, m2 >> 16) >> 7);     // (255: the row is no number)
+        const int shift = min(127 + 14 - ex, 120);                             // the largest element into [2^14, 2^15)
         // a negative scale turns the queries around, so that the largest score is the largest S
         const float up = copysignf(__uint_as_float(static_cast<uint32_t>(127 + shift) << 23), p.scale_log2);
-        cq = fabsf(p.scale_log2) * __uint_as_float(static_cast<uint32_t>(127 - shift) << 23);
+        row_scale[tid] = fabsf(p.scale_log2) * __uint_as_float(static_cast<uint32_t>(127 - shift) << 23);
 #pragma unroll 1
-        for (int i0 = 0; i0 < PASSES; i0 += 4) {
+        for (int c = 0; c < D / 8; c += 4) {
           uint4 v[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint4*>(q_at + (i0 + i) * 4 * PER * 128);
+          for (int i = 0; i < 4; ++i) v[i] = *chunk(c + i);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<uint4*>(q_at + (i0 + i) * 4 * PER * 128) =
-                make_uint4(half2_bits(bf16lo(v[i].x) * up, bf16hi(v[i].x) * up), half2_bits(bf16lo(v[i].y) * up, bf16hi(v[i].y) * up),
-                           half2_bits(bf16lo(v[i].z) * up, bf16hi(v[i].z) * up), half2_bits(bf16lo(v[i].w) * up, bf16hi(v[i].w) * up));
+            *chunk(c + i) = make_uint4(half2_bits(bf16lo(v[i].x) * up, bf16hi(v[i].x) * up), half2_bits(bf16lo(v[i].y) * up, bf16hi(v[i].y) * up),
+                                       half2_bits(bf16lo(v[i].z) * up, bf16hi(v[i].z) * up), half2_bits(bf16lo(v[i].w) * up, bf16hi(v[i].w) * up));
         }
         fence_proxy_async_smem();
         mbar_arrive(&q_full);
-        publish(e, cq);
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + kv) : "memory");     // the factors of all rows of this tile
+        publish(e);
       }
     }
   } else {
@@ -602,6 +592,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         mbar_wait(&s_full[t], n_step & 1, abortp, p.err, CS_ERR_TIMEOUT_MMA);
         tc_fence_after();
         const float4 sc = s_scale[s];
+        // (not 0, also for a scale of 0: a hidden key's -inf times the factor has to stay -inf)
+        const float factor = fmaxf(s_qscale[n_item & 1][t][r] * sc.x, 1e-37f);
         const int nvalid = lim - (it.j0 + j) * KV8_PAGE;       // visible keys of the page (may be negative or beyond 128)
         const int wvalid = wmin - (it.j0 + j) * KV8_PAGE;      // the same for every row of the warp: no divergent branch
         // first pass: the largest S of the row
@@ -627,7 +619,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
           largest(x, c);
           largest(y, c + 32);
         }
-        const float mx = fmaxf(mx0, mx1) * sc.x + sc.y;
+        const float mx = fmaxf(mx0, mx1) * factor + sc.y;
         // The reference m - 6 moves only when a weight would pass 2^14
         const float m_new = mx > m + 8.f ? mx : m;
         if (__any_sync(0xffffffffu, m_new != m)) {   // tcgen05.ld / st are warp-wide: the warp decides together
@@ -648,7 +640,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         m = m_new;
         // second pass: weights and their sum; the weights of 32 keys take 16 columns and stay behind the scores still to be read
         const float add = sc.y + (6.f - m);
-        const uint64_t mul2 = pack2(sc.x, sc.x), ref2 = pack2(add, add);
+        const uint64_t mul2 = pack2(factor, factor), ref2 = pack2(add, add);
         uint64_t sum_a = pack2(0.f, 0.f), sum_b = sum_a;
         auto weigh = [&](uint32_t (&x)[32], int c) {
           if (wvalid < c + 32) {

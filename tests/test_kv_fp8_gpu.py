@@ -336,6 +336,36 @@ def test_a_query_that_is_no_number_spoils_its_own_row_only(n):
 
 
 @pytest.mark.parametrize("n", [1, 20])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("scale", [None, -0.1])
+def test_queries_of_very_different_sizes_leave_each_other_alone(n, d, scale):
+    """Queries of one tile 2^20 to 2^100 times larger or smaller than their neighbours, which stay right.
+
+    In the prompt kernel rows share nothing, so they keep every bit.  Where single tokens are decoded, a head that moves the
+    reference of its weights moves those of the other heads of its warp with it, which rounds their weights anew: they are held
+    to the definition instead (an error e of a weight relative to it is at most 2^-11, as everywhere here)."""
+    lens, new = [300, 70], [n, n]
+    q, cache, table, kv_len, cu = _setup(lens, new, 14, 2, d, seed=18)
+    want = ops.attention_paged_fp8(q, cache, table, kv_len, cu, n, scale=scale)
+    _check(want, q, cache, table, lens, new, scale=scale)
+    mine = torch.zeros(2 * n, 14, dtype=torch.bool, device=DEV)
+    mine[0, 3] = mine[n - 1, 9] = mine[2 * n - 1, 13] = True
+
+    def others_are_right(x):
+        got = ops.attention_paged_fp8(x, cache, table, kv_len, cu, n, scale=scale)
+        _check(torch.where(mine[..., None], want, got), q, cache, table, lens, new, scale=scale)
+        assert n == 1 or torch.equal(got[~mine], want[~mine])
+        return got
+
+    for power in (20, 28, 32, 40, 60, 100):
+        others_are_right(torch.where(mine[..., None], q * 2.0 ** power, q))
+    others_are_right(torch.where(mine[..., None], torch.full_like(q, torch.finfo(q.dtype).max), q))
+    for power in (20, 60, 100):     # and the small ones are right themselves: all their scores are next to zero
+        quiet = torch.where(mine[..., None], q * 2.0 ** -power, q)
+        _check(others_are_right(quiet), quiet, cache, table, lens, new, scale=scale)
+
+
+@pytest.mark.parametrize("n", [1, 20])
 def test_pages_shared_by_sequences_and_tables_shared_by_all(n):
     q, cache, table, kv_len, cu = _setup([333], [n], 8, 2, 64, seed=16)
     lens = [333, 200, 129, 333]
