@@ -590,6 +590,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         const uint32_t s = n_step % SRING;
         mbar_wait(&sc_full[s], (n_step / SRING) & 1, abortp, p.err, CS_ERR_TIMEOUT_SLOT);
         mbar_wait(&s_full[t], n_step & 1, abortp, p.err, CS_ERR_TIMEOUT_MMA);
+        __syncwarp();                                // every lane polls for itself; tcgen05.ld / st below are warp-wide
         tc_fence_after();
         const float4 sc = s_scale[s];
         // (not 0, also for a scale of 0: a hidden key's -inf times the factor has to stay -inf)
@@ -681,6 +682,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
       // ---------------------------------- output ------------------------------------
       if (it.n > 0) {
         mbar_wait(&o_full[t], n_item & 1, abortp, p.err, CS_ERR_TIMEOUT_MMA);
+        __syncwarp();
         ++n_item;
         tc_fence_after();
       }
@@ -708,13 +710,14 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[i] = 0u;
         }
-        if (!row_ok && !(it.whole && p.o_vec)) continue;
         float f[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(o[i]) * inv;
         if (!it.whole) {
+          if (row_ok) {
 #pragma unroll
-          for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(part + c * 16 + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+            for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(part + c * 16 + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+          }
         } else if (p.o_vec) {
           // Neighbours trade halves, so that a store covers whole sectors (32 bytes of 16 rows, not 16 of 32: 9 prompts of
           // 17 to 2300 tokens 188 -> 183 us, one of 300 26.3 -> 24.9 us).
@@ -729,10 +732,11 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
           }
           if (even_ok) *reinterpret_cast<uint4*>(dst_even + c * 16) = make_uint4(w[0], w[1], w[2], w[3]);
           if (odd_ok) *reinterpret_cast<uint4*>(dst_odd + c * 16) = make_uint4(w[4], w[5], w[6], w[7]);
-        } else {
+        } else if (row_ok) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) dst[c * 16 + i] = __float2bfloat16(f[i]);
         }
+        __syncwarp();                              // the next read of TMEM is the whole warp's
       }
       tc_fence_before();
     }

@@ -442,6 +442,7 @@ attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_codes, const 
         const uint32_t codes = smem_u32(s_codes + (team * RING + s) * 2 * TILE);
         const uint32_t scale = smem_u32(s_scale + (team * RING + s) * 2 * UNIT * 4);
         mbar_wait(&full[team][s], (n / RING) & 1, abortp, p.err, CS_ERR_TIMEOUT_TMA);
+        __syncwarp();                          // every lane polls for itself; the products below are warp-wide
         const int valid = wk.len - u * UNIT;   // keys of the unit that exist (may exceed UNIT)
         if (kw < valid) {
           // ---- S^T = K Q^T for KT tiles of 16 keys; two chains of products per tile

@@ -285,6 +285,21 @@ def test_strides_given_output_rows_behind_the_last_sequence_and_scale(new, scale
         _check(out[:T, :, 9:73], q, cache, table, lens, new, scale=scale)
 
 
+@pytest.mark.parametrize("Hq,Hkv,d", [(5, 1, 128), (14, 2, 64)])
+@pytest.mark.parametrize("offset,width", [(0, 0), (8, 8), (1, 1)])     # 16-byte stores, and single elements
+def test_outputs_of_warps_with_rows_that_are_no_queries(Hq, Hkv, d, offset, width):
+    """Tiles that end inside a warp (5 and 7 heads do not divide 128 rows, and few tokens do not fill a tile), in items of one
+    CTA and in items that are cut: every lane of such a warp takes part in reading the sums, and only queries are written."""
+    lens, new = [4100, 130, 70], [37, 3, 26]
+    q, cache, table, kv_len, cu = _setup(lens, new, Hq, Hkv, d, seed=19)
+    T = q.shape[0]
+    out = torch.full((T + 2, Hq, d + width), 7.0, device=DEV, dtype=torch.bfloat16)
+    mine = out[..., offset: offset + d]
+    ops.attention_paged_fp8(torch.cat([q, q[:2]]), cache, table, kv_len, cu, max(new), out=mine)
+    assert (out[T:] == 7.0).all() and (out[..., :offset] == 7.0).all() and (out[..., offset + d:] == 7.0).all()
+    _check(mine[:T], q, cache, table, lens, new)
+
+
 @pytest.mark.parametrize("n", [1, 20])
 def test_extreme_scores_scales_and_queries(n):
     """One key that outweighs all others; value rows whose sizes differ by 2^60; queries of 2^-60 and 2^60."""
