@@ -381,6 +381,34 @@ def test_queries_of_very_different_sizes_leave_each_other_alone(n, d, scale):
 
 
 @pytest.mark.parametrize("n", [1, 20])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_too_large_for_fractions_pick_the_best_key(n, d, sign):
+    """Scores from 2^10 to 2^118, where fp32 has no fraction bits left for an exponent.  The best key is 1/17 ahead of all others,
+    so it takes all the weight: the result is its value row, rounded to bf16 once (and to fp16 before, in the prompt kernel)."""
+    lens, new = [300, 300, 70], [n] * 3
+    best = [20, 210, 45]                                # in the first, the second and the only page; the last page lowers nothing
+    q, cache, table, kv_len, cu = _setup(lens, new, 14, 2, d, seed=20, poison=False)
+    codes, scales = ops.kv_cache_fp8_views(cache)
+    scales[:, 0] = 1 / 256
+    # a negative query is best answered by the smallest key
+    codes[:, 0] = 256.0 if sign > 0 else 288.0
+    for i, b in enumerate(best):
+        codes[int(table[i, b // 128]), 0, :, b % 128] = 288.0 if sign > 0 else 256.0
+    want, top = [], []
+    for i, b in enumerate(best):
+        page = int(table[i, b // 128])
+        want.append((codes[page, 1, :, b % 128].double() * scales[page, 1, :, b % 128, None].double()).repeat_interleave(7, 0).expand(n, 14, d))
+        top.append(scales[page, 1].double().amax(-1).repeat_interleave(7)[None, :, None].expand(n, 14, d))
+    want, top = torch.cat(want), torch.cat(top)
+    for power in (10, 16, 20, 22, 24, 26, 28, 32, 40, 60, 100, 111):
+        got = ops.attention_paged_fp8(torch.full_like(q, sign * 2.0 ** power), cache, table, kv_len, cu, n)
+        # bf16 output, fp16 weight (numerator only), fp16 value row
+        tol = want.abs() * (2.0 ** -8 + 2 * 2.0 ** -11 + 2.0 ** -18) + top * 2.0 ** -30
+        assert ((got.double() - want).abs() <= tol).all(), power
+
+
+@pytest.mark.parametrize("n", [1, 20])
 def test_pages_shared_by_sequences_and_tables_shared_by_all(n):
     q, cache, table, kv_len, cu = _setup([333], [n], 8, 2, 64, seed=16)
     lens = [333, 200, 129, 333]
