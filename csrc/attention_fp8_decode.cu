@@ -49,6 +49,9 @@ constexpr int MIN_RUN = 2;
 // border at 3, 26.1 at 8.
 constexpr int SHARED_VISIT = 3;
 constexpr float M_NONE = -3.0e38f;           // running maximum before the first key (finite: differences stay defined)
+// Where the maximum passes this, scores and value scales are no longer added up: from 2^24 on the sum is rounded to integers,
+// and a weight that is taken relative to it is too large for fp16, or far too small.
+constexpr float LARGE_EXPONENT = 1048576.f;
 
 // One instantiation.  TEAMS: as many as registers allow (128 a thread with three teams, 168 with two).
 template <int D, int NT>
@@ -428,10 +431,13 @@ attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_codes, const 
         qs[nt][1] = __shfl_sync(0xffffffffu, down, t * 8 + 4);
       }
       if (lane == 0) mbar_arrive(&q_empty[team][slot]);
-      float o[NT][MT][4], m[NT][2], l[NT][2];   // m: the reference exponent is m - 6, so weights reach up to 2^14
+      // Weights are relative to the exponent r, 6 below the maximum m, so they reach up to 2^14.  Of large scores m itself is taken
+      // first, and r is what is left to take.
+      float o[NT][MT][4], m[NT][2], r[NT][2], l[NT][2];
+      bool large = false;                       // of the warp
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        m[nt][0] = m[nt][1] = M_NONE;
+        m[nt][0] = m[nt][1] = r[nt][0] = r[nt][1] = M_NONE;
         l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
         for (int i = 0; i < MT; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
@@ -521,19 +527,46 @@ attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_codes, const 
 #pragma unroll
               for (int j = 0; j < 4; ++j) grow |= c[kt][nt][j] + lv[kt][j >> 1] > m[nt][j & 1] + 8.f;
           // The reference moves only when a weight would pass 2^14, which after the first tiles is rare
-          if (__any_sync(0xffffffffu, grow)) {
+          if (__any_sync(0xffffffffu, grow || large)) {
+            auto all_keys = [](float x) {            // the maximum over the lanes of a head
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+              return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            };
+            const bool was_large = large;
+            bool far = false;
+            float mx[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int j = 0; j < 2; ++j) {
-                float mx = m[nt][j];
+                mx[nt][j] = m[nt][j];
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt) mx = fmaxf(mx, fmaxf(c[kt][nt][j] + lv[kt][0], c[kt][nt][2 + j] + lv[kt][1]));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                const float alpha = ex2(m[nt][j] - mx);
-                m[nt][j] = mx;
+                for (int kt = 0; kt < KT; ++kt) mx[nt][j] = fmaxf(mx[nt][j], fmaxf(c[kt][nt][j] + lv[kt][0], c[kt][nt][2 + j] + lv[kt][1]));
+                mx[nt][j] = all_keys(mx[nt][j]);
+                far |= fabsf(mx[nt][j]) > LARGE_EXPONENT && mx[nt][j] != M_NONE;
+              }
+            large = __any_sync(0xffffffffu, far);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const float had = was_large ? -r[nt][j] : 6.f;
+                float room = 6.f;
+                if (large) {
+                  float top = -INFINITY;             // the largest weight relative to mx
+#pragma unroll
+                  for (int kt = 0; kt < KT; ++kt) {
+                    c[kt][nt][j] -= mx[nt][j];
+                    c[kt][nt][2 + j] -= mx[nt][j];
+                    top = fmaxf(top, fmaxf(c[kt][nt][j] + lv[kt][0], c[kt][nt][2 + j] + lv[kt][1]));
+                  }
+                  top = all_keys(top);
+                  room = mx[nt][j] > m[nt][j] || top + had > 14.f ? 6.f - top : had;
+                }
+                const float alpha = ex2((m[nt][j] - mx[nt][j]) + (room - had));
+                m[nt][j] = mx[nt][j];
+                r[nt][j] = large ? -room : mx[nt][j] - 6.f;
                 l[nt][j] *= alpha;
 #pragma unroll
                 for (int i = 0; i < MT; ++i) { o[nt][i][j] *= alpha; o[nt][i][2 + j] *= alpha; }
@@ -547,7 +580,7 @@ attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_codes, const 
               float w[4];
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
-                const float e = c[kt][nt][j] - (m[nt][j & 1] - 6.f);
+                const float e = c[kt][nt][j] - r[nt][j & 1];
                 l[nt][j & 1] += ex2(e);
                 w[j] = ex2(e + lv[kt][j >> 1]);
               }
@@ -580,7 +613,7 @@ attention_decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_codes, const 
           l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], 8);
           l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], 16);
           const int h = nt * 8 + 2 * t + j;
-          if (g == 0) { s_m[warp][h] = m[nt][j]; s_l[warp][h] = l[nt][j]; }
+          if (g == 0) { s_m[warp][h] = large ? m[nt][j] + r[nt][j] : r[nt][j]; s_l[warp][h] = l[nt][j]; }
           float* dst = s_join + (warp * HEADS + h) * JOIN_LD + g * VPER;
 #pragma unroll
           for (int i = 0; i < MT; i += 2)

@@ -383,7 +383,8 @@ def test_queries_of_very_different_sizes_leave_each_other_alone(n, d, scale):
 @pytest.mark.parametrize("n", [1, 20])
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("sign", [1, -1])
-def test_scores_too_large_for_fractions_pick_the_best_key(n, d, sign):
+@pytest.mark.parametrize("size", [1.0, 2.0 ** -24, 2.0 ** 24])
+def test_scores_too_large_for_fractions_pick_the_best_key(n, d, sign, size):
     """Scores from 2^10 to 2^118, where fp32 has no fraction bits left for an exponent.  The best key is 1/17 ahead of all others,
     so it takes all the weight: the result is its value row, rounded to bf16 once (and to fp16 before, in the prompt kernel)."""
     lens, new = [300, 300, 70], [n] * 3
@@ -391,6 +392,7 @@ def test_scores_too_large_for_fractions_pick_the_best_key(n, d, sign):
     q, cache, table, kv_len, cu = _setup(lens, new, 14, 2, d, seed=20, poison=False)
     codes, scales = ops.kv_cache_fp8_views(cache)
     scales[:, 0] = 1 / 256
+    scales[:, 1] *= size
     # a negative query is best answered by the smallest key
     codes[:, 0] = 256.0 if sign > 0 else 288.0
     for i, b in enumerate(best):
