@@ -722,7 +722,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         if (row_ok) { p.ws_ml[row * 2] = m; p.ws_ml[row * 2 + 1] = l; }
         if (threadIdx.x == 0) p.ws_item[slot] = make_int4(it.seq, it.h0, it.t0, 0);
       }
-      const float inv = !it.whole ? 1.f : (l == 0.f ? 0.f : 1.f / l);
+      // (a row that sees no key is 0; one whose scores are all -inf has a sum of 0 and becomes 0 / 0)
+      const float inv = !it.whole ? 1.f : (lim > 0 ? 1.f / l : 0.f);
       __nv_bfloat16* dst = p.o + static_cast<long long>(it.q_beg + tok) * p.o_tok + (it.h0 + g) * p.o_head;
       float* part = p.ws_o + row * D;
       const bool mate_ok = __shfl_xor_sync(0xffffffffu, row_ok, 1);
@@ -808,7 +809,8 @@ __global__ void __launch_bounds__(256) attention_prefill_fp8_join_kernel(const P
     acc.x = acc.x * a + v.x * b; acc.y = acc.y * a + v.y * b; acc.z = acc.z * a + v.z * b; acc.w = acc.w * a + v.w * b;
   }
   if (lane * 4 >= D) return;
-  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  const bool sees_keys = (p.causal ? min(q.k_len, tok + q.shift + 1) : q.k_len) > 0;
+  const float inv = sees_keys ? 1.0f / l : 0.f;
   __nv_bfloat16* dst = p.o + static_cast<long long>(q.q_beg + tok) * p.o_tok + (item.y + g) * p.o_head + lane * 4;
   const float f[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
   if (p.o_vec) {

@@ -158,9 +158,10 @@ __device__ __forceinline__ bool fits(const DecParams& p, int b) {
 
 template <int N> struct Count { static constexpr int value = N; };
 
-// Four channels of one head: sums divided by the normaliser (0 when no key took part).
+// Four channels of one head: sums divided by the normaliser.  (Only sequences with keys come here; the sum is 0 when all their
+// scores are -inf, and 0 / 0 is the result.)
 __device__ __forceinline__ void store_head(const DecParams& p, int row, int head, int ch4, const float4& acc, float sum) {
-  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  const float inv = 1.0f / sum;
   __nv_bfloat16* dst = p.o + row * p.o_tok + head * p.o_head + ch4 * 4;
   const uint2 v = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
   if (p.o_vec) {

@@ -352,6 +352,24 @@ def test_a_query_that_is_no_number_spoils_its_own_row_only(n):
 
 @pytest.mark.parametrize("n", [1, 20])
 @pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("L", [1, 12, 300, 5000])
+def test_scores_that_are_all_minus_infinity_give_nan_and_no_keys_give_zero(n, d, L):
+    """As the definition has it (0 / 0), in items of one CTA and in items that are cut; the other head is not touched."""
+    blocks = -(-L // 128)
+    cache = ops.kv_cache_fp8(blocks, 1, d, DEV)
+    codes, scales = ops.kv_cache_fp8_views(cache)
+    codes.view(torch.uint8).fill_(0x38)      # 1.0
+    scales.fill_(1.0)
+    q = torch.zeros(n, 2, d, device=DEV, dtype=torch.bfloat16)
+    q[:, 0, 0] = float("-inf")
+    out = ops.attention_paged_fp8(q, cache, torch.arange(blocks, device=DEV, dtype=torch.int32)[None], _i32([L]), _i32([0, n]), n)
+    unseeing = max(0, n - L)                 # queries ahead of the first key
+    assert not out[:unseeing].any()
+    assert torch.isnan(out[unseeing:, 0]).all() and (out[unseeing:, 1] == 1.0).all()
+
+
+@pytest.mark.parametrize("n", [1, 20])
+@pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("scale", [None, -0.1])
 def test_queries_of_very_different_sizes_leave_each_other_alone(n, d, scale):
     """Queries of one tile 2^20 to 2^100 times larger or smaller than their neighbours, which stay right.
