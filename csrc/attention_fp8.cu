@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_prefill_fp8_kernel(const
         tc_fence_after();
         const float4 sc = s_scale[s];
         // (not 0, also for a scale of 0: a hidden key's -inf times the factor has to stay -inf)
-        const float factor = fmaxf(s_qscale[n_item & 1][t][r] * sc.x, 1e-37f);
+        const float product = s_qscale[n_item & 1][t][r] * sc.x, factor = product < 1e-37f ? 1e-37f : product;   // (a NaN stays one)
         const int nvalid = lim - (it.j0 + j) * KV8_PAGE;       // visible keys of the page (may be negative or beyond 128)
         const int wvalid = wmin - (it.j0 + j) * KV8_PAGE;      // the same for every row of the warp: no divergent branch
         // first pass: the largest S of the row

@@ -369,6 +369,12 @@ def test_scores_that_are_all_minus_infinity_give_nan_and_no_keys_give_zero(n, d,
 
 
 @pytest.mark.parametrize("n", [1, 20])
+def test_a_scale_that_is_no_number_gives_nan(n):
+    q, cache, table, kv_len, cu = _setup([300, 70], [n, n], 14, 2, 128, seed=22)
+    assert torch.isnan(ops.attention_paged_fp8(q, cache, table, kv_len, cu, n, scale=math.nan)).all()
+
+
+@pytest.mark.parametrize("n", [1, 20])
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("scale", [None, -0.1])
 def test_queries_of_very_different_sizes_leave_each_other_alone(n, d, scale):
