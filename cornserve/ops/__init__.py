@@ -605,11 +605,11 @@ def attention_paged_fp8(q: torch.Tensor, cache: torch.Tensor, block_table: torch
         return out
     nbytes = lib.cs_attention_prefill_fp8_ws_bytes(Tq, B, Hq, Hkv, d, width)
     ws = cache.new_empty(nbytes)
-    _chk(lib.cs_attention_prefill_fp8(q.data_ptr(), q_tok, cache.data_ptr(), pages, out.data_ptr(), o_tok, o_head,
-                                      cu_q.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(), block_table.stride(0),
-                                      width, B, Tq, Hq, Hkv, d, scale, 1 if causal else 0, ws.data_ptr(), nbytes, _stream()),
-         "cs_attention_prefill_fp8")
-    _count(2)
+    launched = lib.cs_attention_prefill_fp8(q.data_ptr(), q_tok, cache.data_ptr(), pages, out.data_ptr(), o_tok, o_head,
+                                            cu_q.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(), block_table.stride(0),
+                                            width, B, Tq, Hq, Hkv, d, scale, 1 if causal else 0, ws.data_ptr(), nbytes, _stream())
+    _chk(min(launched, 0), "cs_attention_prefill_fp8")
+    _count(launched)     # one where a single CTA has no partial sums to join
     return out
 
 

@@ -832,8 +832,8 @@ int launch_prefill(const PrefillParams& p, int grid, cudaStream_t stream) {
     ready[dev] = true;
   }
   if (cs_launch_pdl(attention_prefill_fp8_kernel<D>, dim3(grid), dim3(THREADS), Shape<D>::SMEM, stream, p) != cudaSuccess) return -10;
-  if (grid == 1) return 0;
-  return cs_launch_pdl(attention_prefill_fp8_join_kernel<D>, dim3(grid, PAIR_ROWS / 8), dim3(256), 0, stream, p, grid) == cudaSuccess ? 0 : -10;
+  if (grid == 1) return 1;
+  return cs_launch_pdl(attention_prefill_fp8_join_kernel<D>, dim3(grid, PAIR_ROWS / 8), dim3(256), 0, stream, p, grid) == cudaSuccess ? 2 : -10;
 }
 
 // CTAs of a call: no more than runs of the least length that the queries and tables could make up.
@@ -855,7 +855,7 @@ CS_API long long cs_attention_prefill_fp8_ws_bytes(long long Tq, long long B, in
 
 // q: [Tq, Hq, d] with contiguous heads, tokens q_tok elements apart and on 16-byte boundaries; o: [Tq, Hq, d] with token and
 // head strides in elements; d is 64 or 128.  ws: cs_attention_prefill_fp8_ws_bytes of scratch that no call on another stream
-// uses.
+// uses.  Returns how many kernels were launched, or a negative error.
 CS_API int cs_attention_prefill_fp8(const void* q, long long q_tok, const void* cache, long long num_pages, void* o, long long o_tok,
                                     long long o_head, const void* cu_q, const void* kv_len, const void* block_table, long long bt_stride,
                                     int bt_width, int B, int Tq, int Hq, int Hkv, int d, float scale, int causal, void* ws,

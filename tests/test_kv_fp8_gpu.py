@@ -543,6 +543,16 @@ def test_results_do_not_depend_on_the_run_or_the_batch_order():
         assert torch.equal(a, ops.attention_paged_fp8(q, cache, table, kv_len, cu, 1))
 
 
+def test_launches_are_counted_as_they_are_made():
+    """A call that one CTA does alone leaves no partial sums, and the kernel that joins them is not launched."""
+    for lens, new, Hq, launches in (([2], [2], 64, 1), ([300], [300], 8, 2), ([300, 5], [1, 1], 8, 2)):
+        q, cache, table, kv_len, cu = _setup(lens, new, Hq, 1, 128, seed=23)
+        before = ops.kernel_launches()
+        out = ops.attention_paged_fp8(q, cache, table[:, : -(-max(lens) // 128)], kv_len, cu, max(new))
+        assert ops.kernel_launches() - before == launches
+        _check(out, q, cache, table, lens, new)
+
+
 def test_empty_calls():
     q, cache, table, kv_len, cu = _setup([5], [1], 4, 2, 64)
     assert ops.attention_paged_fp8(q[:0], cache, table[:0], kv_len[:0], cu[:1], 0).shape == (0, 4, 64)
