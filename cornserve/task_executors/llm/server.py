@@ -81,7 +81,7 @@ def parse_args(argv: list[str] | None = None) -> argparse.Namespace:
                     help="fp8: attention and MLP projections as e4m3 with 128x128 block scales (also chosen when the "
                          "checkpoint's quantization_config says fp8)")
     ap.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "fp8"],
-                    help="fp8: keys and values cached as e4m3 with one scale per token and head (about twice the tokens)")
+                    help="fp8: keys and values cached as e4m3 with one scale per token and head (about twice the tokens); not with --run-talker")
     ap.add_argument("--gpu-memory-utilization", type=float, default=0.9)
     ap.add_argument("--num-kv-pages", type=int, default=0, help="0 = size the cache from free memory")
     ap.add_argument("--decode-burst", type=int, default=4)
@@ -93,7 +93,10 @@ def parse_args(argv: list[str] | None = None) -> argparse.Namespace:
     for flag in ("--trust-remote-code", "--enforce-eager", "--no-enable-prefix-caching", "--disable-mm-preprocessor-cache",
                  "--no-enable-chunked-prefill", "--disable-chunked-mm-input"):
         ap.add_argument(flag, action="store_true", help="accepted for compatibility")
-    return ap.parse_args(argv)
+    args = ap.parse_args(argv)
+    if args.run_talker and args.kv_cache_dtype != "auto":
+        ap.error("--kv-cache-dtype is not available with --run-talker: the talker's caches keep the model's type")
+    return args
 
 
 def pick_device() -> torch.device:

@@ -230,3 +230,13 @@ def test_server_option_reaches_the_engine():
     assert parse_args(["m", "--kv-cache-dtype", "fp8"]).kv_cache_dtype == "fp8"
     with pytest.raises(SystemExit):
         parse_args(["m", "--kv-cache-dtype", "int4"])
+
+
+def test_the_option_is_refused_where_it_would_do_nothing(capsys):
+    """The talker allocates its caches in the model's type."""
+    from cornserve.task_executors.llm.server import parse_args
+
+    with pytest.raises(SystemExit):
+        parse_args(["m", "--run-talker", "--kv-cache-dtype", "fp8"])
+    assert "--run-talker" in capsys.readouterr().err
+    assert parse_args(["m", "--run-talker"]).run_talker and parse_args(["m", "--run-talker", "--kv-cache-dtype", "auto"]).run_talker
