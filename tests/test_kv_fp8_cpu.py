@@ -1,6 +1,10 @@
 """The 8-bit paged key-value cache on the CPU: layout, quantisation, attention, refusals, and the engine on top of it."""
 
+import json
 import math
+import os
+import subprocess
+import sys
 import types
 
 import numpy as np
@@ -10,6 +14,7 @@ import torch
 from cornserve import ops
 from cornserve.models.qwen_llm import BatchMeta, LLMConfig, QwenLLM
 from cornserve.ops import reference as ref
+from cornserve.services.process import free_port
 from cornserve.task_executors.llm.engine import EngineConfig, LLMEngine, PrefilledKV, SamplingParams, Sequence
 
 
@@ -240,3 +245,47 @@ def test_the_option_is_refused_where_it_would_do_nothing(capsys):
         parse_args(["m", "--run-talker", "--kv-cache-dtype", "fp8"])
     assert "--run-talker" in capsys.readouterr().err
     assert parse_args(["m", "--run-talker"]).run_talker and parse_args(["m", "--run-talker", "--kv-cache-dtype", "auto"]).run_talker
+
+
+@pytest.mark.timeout(600)
+def test_two_tensor_parallel_ranks_cache_their_heads():
+    """Two gloo ranks: each caches its own key heads, and the engine's hidden states are those of one process."""
+    script = os.path.join(os.path.dirname(__file__), "kv_fp8_tp_cpu.py")
+    env = dict(os.environ, OMP_NUM_THREADS="2", CUDA_VISIBLE_DEVICES="")
+    port = str(free_port())
+    procs = [subprocess.Popen([sys.executable, script, str(r), "2", port], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, env=env)
+             for r in range(2)]
+    outs = [p.communicate(timeout=500)[0] for p in procs]
+    assert all(p.returncode == 0 for p in procs) and "KV_FP8_TP_OK" in outs[0], "\n".join(o[-3000:] for o in outs)
+
+
+def test_server_builds_an_engine_with_the_option(tmp_path, monkeypatch):
+    """From the command line to the cache: its type, and as many pages as a GPU's free memory holds at 8 bits."""
+    from cornserve.task_executors.llm import server
+
+    (tmp_path / "config.json").write_text(json.dumps({
+        "model_type": "qwen2", "architectures": ["Qwen2ForCausalLM"], "hidden_size": 64, "num_hidden_layers": 2, "num_attention_heads": 4,
+        "num_key_value_heads": 2, "head_dim": 16, "intermediate_size": 128, "vocab_size": 512, "rms_norm_eps": 1e-6, "rope_theta": 10000.0,
+        "max_position_embeddings": 512, "tie_word_embeddings": False, "eos_token_id": 511, "torch_dtype": "float32"}))
+    monkeypatch.setenv("CORNSERVE_DEVICE", "cpu")
+    args = [str(tmp_path), "--num-kv-pages", "16", "--max-model-len", "512"]
+    eng, _ = server.build_engine(server.parse_args([*args, "--kv-cache-dtype", "fp8"]))
+    assert eng.cfg.kv_cache_dtype == "fp8" and eng.kv_backing.dtype == torch.uint8 and eng.kv_backing.shape == (2, 16, 2, 2, 128 * 20)
+    seqs = lambda: [Sequence("s", np.arange(3, 150, dtype=np.int32), SamplingParams(max_tokens=3, ignore_eos=True))]  # noqa: E731
+    assert len(eng.generate(seqs())["s"]) == 3 and eng.kv_backing[:, 1:].any()
+    plain, _ = server.build_engine(server.parse_args(args))
+    assert plain.kv_backing.dtype == torch.float32 and plain.kv_backing.shape == (2, 16, 2, 2, 128, 16)
+    # without --num-kv-pages the pages come from the free memory of the GPU
+    made = []
+    monkeypatch.setattr(server, "pick_device", lambda: types.SimpleNamespace(type="cuda"))
+    monkeypatch.setattr(server.torch.cuda, "set_device", lambda d: None)
+    monkeypatch.setattr(server.torch.cuda, "mem_get_info", lambda d: (100 << 30, 180 << 30))
+    monkeypatch.setattr(server, "QwenLLM", lambda cfg, group, device: QwenLLM(cfg, group=group, device="cpu").float())
+    monkeypatch.setattr(server, "LLMEngine", lambda model, cfg: made.append((model, cfg)) or types.SimpleNamespace(capture_decode_graphs=lambda: 0))
+    for kind in ("auto", "fp8"):
+        server.build_engine(server.parse_args([str(tmp_path), "--kv-cache-dtype", kind]))
+    for model, cfg in made:
+        budget = int((100 << 30) * 0.9) - (4 << 30)
+        row = 16 + 4 if cfg.kv_cache_dtype == "fp8" else 2 * 16        # bytes of a token and head
+        assert cfg.num_pages == budget // (2 * 2 * 2 * 128 * row)
+    assert [cfg.kv_cache_dtype for _, cfg in made] == ["auto", "fp8"]
