@@ -543,6 +543,41 @@ def test_results_do_not_depend_on_the_run_or_the_batch_order():
         assert torch.equal(a, ops.attention_paged_fp8(q, cache, table, kv_len, cu, 1))
 
 
+@pytest.mark.parametrize("Hq,Hkv,d", [(16, 16, 64), (16, 8, 128), (32, 2, 128)])
+def test_decode_runs_of_one_cta_over_more_than_32_pages(Hq, Hkv, d):
+    """The producers hold 32 table entries at a time: long visits reload them.  (24 x 8 or more items of about 41 pages, and one
+    batch whose items fill a CTA's whole run.)"""
+    lens = [4500 + 67 * i % 1500 for i in range(24 if Hkv > 2 else 90)]
+    q, cache, table, kv_len, cu = _setup(lens, [1] * len(lens), Hq, Hkv, d, seed=24)
+    _check(ops.attention_paged_fp8(q, cache, table, kv_len, cu, 1), q, cache, table, lens, [1] * len(lens))
+
+
+@pytest.mark.parametrize("Hq,d", [(7, 128), (3, 64), (16, 128), (16, 64)])
+def test_decode_item_shared_by_more_than_128_ctas(Hq, d):
+    """One key head and 40000 keys: every CTA of the GPU leaves a part of the same item, which the join looks for in blocks of 128."""
+    assert torch.cuda.get_device_properties(0).multi_processor_count > 129
+    q, cache, table, kv_len, cu = _setup([40000], [1], Hq, 1, d, seed=25)
+    _check(ops.attention_paged_fp8(q, cache, table, kv_len, cu, 1), q, cache, table, [40000], [1])
+
+
+@pytest.mark.parametrize("new", [[1] * 5, [5, 300, 64, 33, 128]])
+def test_same_call_same_bits_and_any_batch_order_within_tolerance(new):
+    """Sums do not depend on timing.  Where a sequence is cut depends on the batch, so another order may change last bits."""
+    lens = [5, 2000, 700, 333, 128]
+    q, cache, table, kv_len, cu = _setup(lens, new, 28, 4, 128, seed=26)
+    a = ops.attention_paged_fp8(q, cache, table, kv_len, cu, max(new))
+    for _ in range(5):
+        assert torch.equal(a, ops.attention_paged_fp8(q, cache, table, kv_len, cu, max(new)))
+    starts = [sum(new[:i]) for i in range(6)]
+    for order in ([4, 3, 2, 1, 0], [1, 4, 0, 2, 3]):
+        rows = torch.cat([torch.arange(starts[i], starts[i + 1], device=DEV) for i in order])
+        lens2, new2 = [lens[i] for i in order], [new[i] for i in order]
+        table2, cu2 = table[order].contiguous(), _i32([sum(new2[:i]) for i in range(6)])
+        got = ops.attention_paged_fp8(q[rows], cache, table2, _i32(lens2), cu2, max(new))
+        _check(got, q[rows], cache, table2, lens2, new2)
+        assert torch.equal(got, ops.attention_paged_fp8(q[rows], cache, table2, _i32(lens2), cu2, max(new)))
+
+
 def test_launches_are_counted_as_they_are_made():
     """A call that one CTA does alone leaves no partial sums, and the kernel that joins them is not launched."""
     for lens, new, Hq, launches in (([2], [2], 64, 1), ([300], [300], 8, 2), ([300, 5], [1, 1], 8, 2)):
@@ -674,3 +709,48 @@ def test_engine_with_an_8_bit_cache_decodes_from_graphs_like_it_does_eagerly():
     # the graph pads the batch to its bucket, which changes no row of the attention but may change the projections' kernel
     same = sum(a == b for k in got[0] for a, b in zip(got[0][k], got[1][k]))
     assert same >= 3 and got[0]["s0"][0] == got[1]["s0"][0]
+
+
+def _tiny_engine(model, graph, **kw):
+    from cornserve.task_executors.llm.engine import EngineConfig, LLMEngine
+
+    return LLMEngine(model, EngineConfig(num_pages=32, decode_burst=4, max_model_len=512, kv_cache_dtype="fp8", use_cuda_graph=graph, **kw))
+
+
+@pytest.mark.parametrize("count", [3, 4])
+def test_tokens_decoded_from_graphs_over_an_8_bit_cache(count):
+    """Four sequences fill their bucket: graph and eager run the same kernels on the same rows, so every token is the same.  Three
+    leave a padding row, which reads and writes the scratch page.  Each decoded token is also held to one pass over all tokens
+    before it: the roundings that differ (about 20 to 2^-9 in a row of the hidden states, which add up like their squares)
+    move a logit by 2^-7 of the logits' deviation, so half a deviation is far beyond them; a token picked by anything but
+    these logits lies there once in some hundred times."""
+    import numpy as np
+
+    from cornserve.models.qwen_llm import BatchMeta, LLMConfig, QwenLLM
+    from cornserve.task_executors.llm.engine import SamplingParams, Sequence
+
+    torch.manual_seed(0)
+    cfg = LLMConfig(hidden_size=512, num_hidden_layers=2, num_attention_heads=8, num_key_value_heads=2, head_dim=64, intermediate_size=1024,
+                    vocab_size=1024, mrope_section=None, qk_norm=True, attention_bias=False, eos_token_id=1023)
+    model = QwenLLM(cfg, device=DEV).eval()
+    prompts = [np.arange(3 + 11 * i, 3 + 11 * i + n, dtype=np.int32) for i, n in enumerate((5, 140, 260, 127)[:count])]
+    new = 21                             # the fourth crosses a page while it decodes
+    got = []
+    for graph in (True, False):
+        eng = _tiny_engine(model, graph)
+        got.append(eng.generate([Sequence(f"s{i}", p, SamplingParams(max_tokens=new, ignore_eos=True)) for i, p in enumerate(prompts)]))
+        assert graph == any(st.graph is not None for st in eng._decode_states.values())
+    if count == 4:
+        assert got[0] == got[1]
+    for tokens in got:
+        for i, p in enumerate(prompts):
+            ids = torch.tensor([*p.tolist(), *tokens[f"s{i}"]], dtype=torch.int32, device=DEV)
+            T = ids.numel() - 1
+            meta = BatchMeta(ids[:-1], torch.arange(T, dtype=torch.int32, device=DEV).expand(3, T).contiguous(),
+                             (128 + torch.arange(T, device=DEV)).int(), _i32([0, T]), _i32([T]),
+                             torch.arange(1, 2 + T // 128, dtype=torch.int32, device=DEV)[None], _i32([T - 1]), T)
+            with torch.inference_mode():
+                logits = model.compute_logits(model.forward_hidden(meta, model.alloc_kv_cache(2 + T // 128, "fp8")))[len(p):]
+            picked = logits.gather(1, ids[len(p) + 1:, None].long())[:, 0]
+            assert picked.numel() == new - 1
+            assert (picked >= logits.amax(1) - 0.5 * logits.std(1)).all()
