@@ -578,6 +578,19 @@ def test_same_call_same_bits_and_any_batch_order_within_tolerance(new):
         assert torch.equal(got, ops.attention_paged_fp8(q[rows], cache, table2, _i32(lens2), cu2, max(new)))
 
 
+@pytest.mark.parametrize("Hq,Hkv,d", [(28, 4, 128), (131, 1, 64)])
+@pytest.mark.parametrize("new", [[1, 1, 1], [300, 64, 37]])
+def test_the_output_may_be_the_queries_themselves(Hq, Hkv, d, new):
+    """Every row and head is read by those CTAs alone that work on its item, and written when they have read it."""
+    lens = [3000, 64, 700]
+    q, cache, table, kv_len, cu = _setup(lens, new, Hq, Hkv, d, seed=27)
+    want = ops.attention_paged_fp8(q, cache, table, kv_len, cu, max(new))
+    _check(want, q, cache, table, lens, new)
+    x = q.clone()
+    assert ops.attention_paged_fp8(x, cache, table, kv_len, cu, max(new), out=x) is x
+    assert torch.equal(x, want)
+
+
 def test_launches_are_counted_as_they_are_made():
     """A call that one CTA does alone leaves no partial sums, and the kernel that joins them is not launched."""
     for lens, new, Hq, launches in (([2], [2], 64, 1), ([300], [300], 8, 2), ([300, 5], [1, 1], 8, 2)):
