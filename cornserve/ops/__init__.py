@@ -553,8 +553,9 @@ def attention_paged_fp8(q: torch.Tensor, cache: torch.Tensor, block_table: torch
     ``block_table [B, blocks]``, ``kv_len [B]`` and ``cu_q [B + 1]`` (int32) are those of :func:`attention_paged`:
     ``kv_len[s]`` counts the keys of sequence ``s`` including the ones just appended for its queries, which are rows
     ``[cu_q[s], cu_q[s + 1])`` of ``q``, at most ``max_q_len`` of them.  A causal query sees the keys up to its own
-    position; one that sees none gives zeros.  Rows of ``out`` behind the last sequence are not written.
+    position; one that sees none gives zeros.  Rows of ``out`` behind the last sequence are not written.  ``out`` may be ``q``.
 
+    Queries take part exactly, but for elements that are more than 2^31 times smaller than the largest of their token and head.
     With single tokens (``max_q_len`` 1 and as many rows as sequences) keys and values take part exactly as they are
     cached; otherwise they are rounded to fp16 once: code times scale to 11 bits, or to within 2^-30 of the largest scale
     of their page, and the value scales of a sequence have to lie within 2^100 of each other.  The lengths are read on the

@@ -382,7 +382,8 @@ class LLMEngine:
         return old
 
     def read_pages(self, pages: list[int]) -> torch.Tensor:
-        """The pages themselves, on the host: ``[layers, len(pages), 2, heads, 128, d]`` (network fallback)."""
+        """The pages themselves, on the host (network fallback): ``[layers, len(pages), 2, heads, 128, d]``, of an 8-bit cache
+        ``[layers, len(pages), 2, heads, 128 * (d + 4)]`` bytes."""
         idx = torch.as_tensor(pages, device=self.device, dtype=torch.long)
         return self.kv_backing[:, idx].cpu()
 

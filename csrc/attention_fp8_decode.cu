@@ -3,9 +3,10 @@
 //   o = sum_j w_j vc_j / sum_j 2^(s_j - M),   w_j = 2^(s_j + log2 vs_j - M),   s_j = scale * log2(e) * ks_j * (q . kc_j)
 //
 // kc, vc are the e4m3 codes and ks, vs the scales of key j.  Codes are exact in fp16, so the two products run on fp16
-// fragments: the query is scaled by a power of two per head (exact for every element within 2^-38 of the largest), and M
+// fragments: the query is scaled by a power of two per head (exact for every element within 2^-31 of the largest), and M
 // follows the maximum of s_j + log2 vs_j, the weight that the second product sees, so that a weight is never too large
-// for fp16 whatever the value scales are.  The normaliser needs no vs: it takes its own exponential, in fp32.
+// for fp16 whatever the value scales are.  The normaliser needs no vs: it takes its own exponential, in fp32.  (Of scores beyond
+// 2^20 the largest is taken off first, see LARGE_EXPONENT.)
 //
 // The kernel is bound by the cache's bytes, and everything is arranged around reading them once, without a pause:
 //
@@ -25,10 +26,12 @@
 //     operand would have to be written back to shared memory twice as wide; tensor time is not what is scarce at 8 to 16
 //     heads per byte of K.  The warps share nothing until a visit ends; then their sums meet in shared memory.
 //
-// Measured (28 query heads, 4 key heads, d = 128): 256 sequences of 3300 to 3700 tokens, 954 MB, 153 us = 6.2 TB/s, 0.95 of what
-// a copy reaches; issue slots are half full.  64 sequences of 2000, 136 MB, 33 us = 4.1 TB/s.  One of 32768, 35 MB over all SMs,
-// 15.6 us; one of 500, 7.7 us.  The short ones are bound by a chain of latencies: lengths, table entry, unit, the sums of the
-// warps, and the second kernel (each 0.5 to 1 us).
+// Measured inside a graph (28 query heads, 4 key heads, d = 128): 256 sequences of 3300 to 3700 tokens, 954 MB, 151 us =
+// 6.3 TB/s, 0.97 of what a copy reaches; issue slots are half full.  64 sequences of 2000, 136 MB, 33 us = 4.1 TB/s.  One of
+// 32768, 35 MB over all SMs, 15.5 us; one of 500, 7.7 us.  The short ones are bound by a chain of latencies: lengths, table
+// entry, unit, the sums of the warps, and the second kernel (each 0.5 to 1 us).  With 64 query heads (16 to a key head, two n
+// tiles) the large batch takes 233 us = 4.1 TB/s, at d = 64 130 us = 3.8 TB/s: twice the exponentials, products and
+// accumulators for the same bytes, with spills of about 100 bytes a thread.
 #include <math.h>
 
 #include "kv_fp8.cuh"
