@@ -31,8 +31,13 @@ EncodeTiledFn get_encode() {
 int* cs_error_word() {
   std::lock_guard<std::mutex> lk(g_mu);
   if (g_err_host == nullptr) {
-    if (cudaHostAlloc(reinterpret_cast<void**>(&g_err_host), 64,
-                      cudaHostAllocPortable | cudaHostAllocMapped) != cudaSuccess) {
+    // The first call that needs the word may be one that is captured into a graph.  The allocation is no part of the graph,
+    // and a stream capture does not allow it unless this thread says so.
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    const bool exchanged = cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess;
+    const cudaError_t e = cudaHostAlloc(reinterpret_cast<void**>(&g_err_host), 64, cudaHostAllocPortable | cudaHostAllocMapped);
+    if (exchanged) cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess) {
       g_err_host = nullptr;
       return nullptr;
     }

@@ -688,6 +688,49 @@ def test_graphs_replayed_at_once_on_two_streams_and_with_new_lengths(n):
     _check(out, q, cache, table, lens, [n] * B)
 
 
+FIRST_CALLS = """
+import torch
+from cornserve import ops
+d, T, Hq, Hkv = {d}, 40, {Hq}, 2
+dev = torch.device("cuda")
+i32 = lambda a: torch.tensor(a, dtype=torch.int32, device=dev)
+torch.manual_seed(0)
+qkv = torch.randn(T, (Hq + 2 * Hkv) * d, device=dev).bfloat16()
+ang = torch.arange(T, device=dev)[:, None] * 1e4 ** (-torch.arange(d // 2, device=dev) * 2 / d)
+cs = torch.stack([ang.cos(), ang.sin()], dim=1).float().contiguous()
+cache, table, slot = ops.kv_cache_fp8(1, Hkv, d, dev), i32([[0]]), torch.arange(T, device=dev, dtype=torch.int32)
+lens, cu, one = i32([T]), i32([0, T]), i32([0, 1])
+
+def step():
+    q = ops.rope_kv_write_fp8_(qkv, Hq, Hkv, d, cs, cache, slot)
+    return ops.attention_paged_fp8(q, cache, table, lens, cu, T), ops.attention_paged_fp8(q[-1:], cache, table, lens, one, 1)
+
+ops.rms_norm(torch.randn(4, 64, device=dev).bfloat16(), torch.ones(64, device=dev).bfloat16())    # the library is in use
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = step()
+g.replay()
+torch.cuda.synchronize()
+got = [o.clone() for o in out]
+assert all(torch.equal(a, b) for a, b in zip(got, step())) and got[0].any() and got[1].any()
+ops.check_error("captured")
+print("CAPTURED_OK")
+"""
+
+
+@pytest.mark.parametrize("d,Hq", [(128, 14), (64, 32)])
+def test_first_calls_of_a_process_may_be_captured(d, Hq):
+    """Append, prompt and decode attention in one graph, none of which ran in this process before."""
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS.format(d=d, Hq=Hq)], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "CAPTURED_OK" in r.stdout, r.stdout + r.stderr[-3000:]
+
+
 def test_pages_pulled_into_another_cache_give_the_same_attention():
     lens = [300, 129]
     q, cache, table, kv_len, cu = _setup(lens, [1, 1], 28, 4, 128, seed=41)
