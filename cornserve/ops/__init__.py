@@ -461,7 +461,7 @@ def kv_cache_fp8(num_pages: int, kv_heads: int, d: int, device: torch.device | s
 
 def kv_cache_fp8_views(cache: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """``(codes [pages, 2, kv_heads, 128, d] float8_e4m3fn, scales [pages, 2, kv_heads, 128] fp32)``, views of ``cache``:
-    row ``r`` of a page stands for ``codes[..., r, :] * scales[..., r]``."""
+    row ``r`` of a page stands for ``codes[..., r, :] * scales[..., r]``.  Scales are never negative."""
     pages, heads, d = _kv_fp8_shape(cache)
     return reference.kv_cache_fp8_views(cache, pages, heads, d)
 
