@@ -591,6 +591,19 @@ def test_the_output_may_be_the_queries_themselves(Hq, Hkv, d, new):
     assert torch.equal(x, want)
 
 
+@pytest.mark.parametrize("Hq,Hkv,d", [(8, 1, 64), (7, 1, 128)])
+@pytest.mark.parametrize("n", [1, 20])
+def test_four_million_keys(Hq, Hkv, d, n):
+    """A table that names the same 16 pages 2048 times over: the softmax is that over the 16 pages alone."""
+    q, cache, table, kv_len, cu = _setup([2048], [n], Hq, Hkv, d, seed=28)
+    table = table[:, :16]
+    out = ops.attention_paged_fp8(q, cache, table.repeat(1, 2048), _i32([2048 * 2048]), cu, n, causal=False)
+    _check(out, q, cache, table, [2048], [n], causal=False)
+    # causal: the first query misses 19 keys, one of 2048 occurrences each: 2^-11 of their weights, like a weight's rounding
+    out = ops.attention_paged_fp8(q, cache, table.repeat(1, 2048), _i32([2048 * 2048]), cu, n)
+    _check(out, q, cache, table, [2048], [n], causal=False)
+
+
 def test_launches_are_counted_as_they_are_made():
     """A call that one CTA does alone leaves no partial sums, and the kernel that joins them is not launched."""
     for lens, new, Hq, launches in (([2], [2], 64, 1), ([300], [300], 8, 2), ([300, 5], [1, 1], 8, 2)):
