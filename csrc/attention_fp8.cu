@@ -31,9 +31,10 @@
 //
 // Measured inside a graph (28 query heads, 4 key heads, d = 128): one prompt of 16000 tokens 1.91 ms = 0.96 PFLOP/s (called for
 // seconds, at the power limit, 2.16 ms = 0.85), 8 of 2000 tokens 358 us = 0.64 PFLOP/s, one of 300 24.4 us; 16 query and 2 key
-// heads, d = 64: 3 chunks of 500 to 2100 tokens over 1000 to 9000 cached ones 214 us = 0.45 PFLOP/s.  A page of a tile pair takes 4300 cycles, of which the products are 2048 (1024 with d = 64) and the
-// exponentials keep their unit busy for 2048; each softmax warp spends 1500 cycles waiting for its next scores, 600 on their
-// maximum and 2000 on the weights.  An item costs 8000 to 13000 cycles beside its pages, a good half of it for the output.
+// heads, d = 64: 3 chunks of 500 to 2100 tokens over 1000 to 9000 cached ones 214 us = 0.45 PFLOP/s.  A page of a tile pair takes
+// 4300 cycles, of which the products are 2048 (1024 with d = 64) and the exponentials keep their unit busy for 2048; each softmax
+// warp spends 1500 cycles waiting for its next scores, 600 on their maximum and 2000 on the weights.  An item costs 8000 to 13000
+// cycles beside its pages, a good half of it for the output.
 #include <math.h>
 
 #include "kv_fp8.cuh"
